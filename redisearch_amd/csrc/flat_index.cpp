@@ -750,6 +750,30 @@ void FlatIndex::read_rows(uint32_t row_begin, size_t n, void *host_out) {
                         hipMemcpyDeviceToHost));
 }
 
+void FlatIndex::cache_rows(size_t row_begin, size_t n, const RowCacheArgs &cache, const int64_t *slots) {
+  flush_if_needed();
+  std::shared_lock<std::shared_mutex> g(mu);   // held until the rows have been read: a writer may move them
+  HIP_CHECK(hipSetDevice(device));
+  if (row_begin > n_rows_ || n > n_rows_ - row_begin) throw std::runtime_error("cache_rows: range beyond the stored rows");
+  if (!n) return;
+  launch_row_write(cache, d_rows_ + row_begin * stride_, stride_ / type_size(type), slots, (uint32_t)n, wstream_);
+  HIP_CHECK(hipStreamSynchronize(wstream_));
+}
+
+int FlatIndex::add_cached_rows(const RowCacheArgs &cache, const int64_t *slots, size_t n, size_t first_label) {
+  std::unique_lock<std::shared_mutex> g(mu);
+  HIP_CHECK(hipSetDevice(device));
+  flush();
+  if (!n) return 0;
+  check_bulk_labels(n, first_label);
+  grow((size_t)n_rows_ + n);
+  uint8_t *dst = d_rows_ + (size_t)n_rows_ * stride_;
+  if (stride_ != elem_bytes_) HIP_CHECK(hipMemsetAsync(dst, 0, n * stride_, wstream_));
+  launch_row_read(cache, slots, (uint32_t)n, dst, stride_ / type_size(type), wstream_);
+  commit_bulk_rows(n, first_label);
+  return (int)n;
+}
+
 size_t FlatIndex::size() {
   std::shared_lock<std::shared_mutex> g(mu);
   return (size_t)n_rows_ + stage_n_;

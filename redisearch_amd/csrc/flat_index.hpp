@@ -25,6 +25,7 @@
 #include "grow_buffer.hpp"
 #include "kernels.hpp"
 #include "label_table.hpp"
+#include "rows.hpp"
 
 namespace rsgpu {
 
@@ -179,6 +180,8 @@ class FlatIndex {
   int add_philox_rows(uint64_t seed, uint64_t first_index, size_t n, size_t first_label);
   // stored rows [row_begin, row_begin+n) as they are in HBM (cosine: normalised), tightly packed, to host memory
   void read_rows(uint32_t row_begin, size_t n, void *host_out);
+  void cache_rows(size_t row_begin, size_t n, const RowCacheArgs &cache, const int64_t *slots);   // both return when done
+  int add_cached_rows(const RowCacheArgs &cache, const int64_t *slots, size_t n, size_t first_label);
 
   size_t size();
   size_t label_count();

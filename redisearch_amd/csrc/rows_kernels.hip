@@ -1,0 +1,812 @@
+// rows_kernels.hip -- the row cache (include/rsgpu_rows.h) on gfx950: rows quantised into their slots and read back, the products
+// of ragged groups of queries with the paged rows of their partitions, and the rules on a batch's scores.
+#include <hip/hip_runtime.h>
+
+#include "rows.hpp"
+
+namespace rsgpu {
+namespace {
+
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+// the caller's rows may begin at any element: gfx950 loads 16 bytes from any address its element type allows
+typedef u4 u4_any __attribute__((aligned(2)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int F32 = VecSimType_FLOAT32, BF16 = VecSimType_BFLOAT16, F16 = VecSimType_FLOAT16;
+constexpr int NATIVE = RSGPU_ROWS_NATIVE, INT8 = RSGPU_ROWS_INT8, E4M3 = RSGPU_ROWS_E4M3, INT4 = RSGPU_ROWS_INT4;
+
+template <int T>
+constexpr int elem_size = T == F32 ? 4 : 2;
+
+// n / d for n, d < 2^31 without a division: m = ceil(2^(32 + l) / d), l = ceil(log2 d) (Granlund and Montgomery, 1994)
+struct FastDiv {
+  uint32_t d, m, l;
+  explicit FastDiv(uint32_t div) : d(div), l(0) {
+    while ((1ull << l) < d) l++;
+    m = (uint32_t)(((1ull << 32) * ((1ull << l) - d)) / d + 1);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const {
+    return (uint32_t)(((uint64_t)__umulhi(n, m) + n) >> l);
+  }
+};
+
+__device__ __forceinline__ float bf16_to_f32(uint32_t low16) { return __uint_as_float(low16 << 16); }
+__device__ __forceinline__ float f16_to_f32(uint32_t low16) {
+  const uint16_t h = (uint16_t)low16;
+  _Float16 x;
+  __builtin_memcpy(&x, &h, 2);
+  return (float)x;
+}
+
+// eight elements as fp32; those from `valid` on are zeros and not read
+template <int T>
+__device__ __forceinline__ void load8(const void *row, uint32_t at, uint32_t valid, float (&v)[8]) {
+  if (valid >= 8) {
+    if constexpr (T == F32) {
+      const u4_any *p = reinterpret_cast<const u4_any *>(static_cast<const float *>(row) + at);
+      const u4 a = p[0], b = p[1];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        v[i] = __uint_as_float(a[i]);
+        v[4 + i] = __uint_as_float(b[i]);
+      }
+    } else {
+      const u4 a = *reinterpret_cast<const u4_any *>(static_cast<const uint16_t *>(row) + at);
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        v[2 * i] = T == BF16 ? __uint_as_float(a[i] << 16) : f16_to_f32(a[i] & 0xffffu);
+        v[2 * i + 1] = T == BF16 ? __uint_as_float(a[i] & 0xffff0000u) : f16_to_f32(a[i] >> 16);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    float x = 0.0f;
+    if ((uint32_t)i < valid) {
+      if constexpr (T == F32) x = static_cast<const float *>(row)[at + i];
+      else x = T == BF16 ? bf16_to_f32(static_cast<const uint16_t *>(row)[at + i]) : f16_to_f32(static_cast<const uint16_t *>(row)[at + i]);
+    }
+    v[i] = x;
+  }
+}
+
+// ---- writing ---------------------------------------------------------------------------------------------------------------
+
+// the bits of the largest magnitude: as integers, so that an infinity or a NaN is larger than every number
+__device__ __forceinline__ uint32_t most8(const float (&v)[8]) {
+  uint32_t a = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
+    a = a > b ? a : b;
+  }
+  return a;
+}
+
+constexpr uint32_t SMALLEST = (127 - 100) << 23;   // 2^-100: below, a block is kept as zeros
+
+// the scale of a block from the bits of its largest magnitude, and the factor its codes are found with (0: all codes are 0)
+template <int FMT>
+__device__ __forceinline__ void scale_of(uint32_t most, float &s, float &inv) {
+  s = inv = 0.0f;
+  if (most < SMALLEST) return;
+  if (most >= 0x7f800000u) {
+    s = __uint_as_float(0x7fc00000u);
+    return;
+  }
+  if constexpr (FMT == E4M3) {
+    // 2^e with e the smallest so that most <= 1.75 * 2^8 * 2^e
+    const uint32_t e = (most >> 23) - 8 + ((most & 0x7fffffu) > 0x600000u ? 1u : 0u);
+    s = __uint_as_float(e << 23);
+    inv = __uint_as_float((254 - e) << 23);
+  } else {
+    s = __uint_as_float(most) / (FMT == INT8 ? 127.0f : 7.0f);
+    inv = 1.0f / s;
+  }
+}
+
+// x / s to the nearest integer, ties to even, as if divided exactly.  x * inv is off by at most two ulps, so its rounding t is
+// the answer or next to it; r = x - t s is exact (one fused step: |r| is at most about s / 2 and a multiple of the smaller ulp of
+// x and s), so |r| against s / 2 says which.
+__device__ __forceinline__ float settle(float x, float s, float t) {
+  const float h = 0.5f * s;
+  const float r = __builtin_fmaf(-t, s, x);
+  const float a = __builtin_fabsf(r);
+  const float next = t + (r > 0.0f ? 1.0f : -1.0f);
+  const bool odd = ((int)t & 1) != 0;
+  return a > h || (a == h && odd) ? next : t;
+}
+
+template <int FMT>
+__device__ __forceinline__ void encode8(const float (&v)[8], float s, float inv, uint32_t (&c)[2]) {
+  c[0] = c[1] = 0;
+  if (inv == 0.0f) return;   // nothing to keep, or a NaN: codes are 0
+  if constexpr (FMT == E4M3) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      int w = 0;
+      w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i] * inv, v[4 * i + 1] * inv, w, false);
+      w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2] * inv, v[4 * i + 3] * inv, w, true);
+      c[i] = (uint32_t)w;
+    }
+  } else {
+    int q[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) q[i] = (int)settle(v[i], s, __builtin_rintf(v[i] * inv));
+    if constexpr (FMT == INT8) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) c[i / 4] |= ((uint32_t)q[i] & 255u) << (8 * (i % 4));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) c[0] |= ((uint32_t)q[i] & 15u) << (4 * i);
+    }
+  }
+}
+
+template <int FMT>
+__device__ __forceinline__ void store_codes8(uint8_t *row, uint32_t chunk, const uint32_t (&c)[2]) {
+  if constexpr (FMT == INT4) *reinterpret_cast<uint32_t *>(row + chunk * 4) = c[0];
+  else *reinterpret_cast<u2 *>(row + chunk * 8) = u2{c[0], c[1]};
+}
+
+// blocks of 8 L elements: L neighbouring lanes have a block, eight elements each
+template <int T, int FMT, int L>
+__global__ __launch_bounds__(256) void row_write_kernel(RowCacheArgs c, const void *rows, size_t stride, const int64_t *slots, uint32_t n,
+                                                        uint32_t rows_per_wg, FastDiv chunks) {
+  for (uint64_t first = (uint64_t)blockIdx.x * rows_per_wg; first < n; first += (uint64_t)gridDim.x * rows_per_wg) {
+    const uint32_t mine = n - first < rows_per_wg ? (uint32_t)(n - first) : rows_per_wg;
+    const uint32_t padded = (c.dim + 31) / 32 * 32;
+    for (uint32_t i = threadIdx.x; i < mine * chunks.d; i += 256) {
+      const uint32_t r = chunks.div(i), chunk = i - r * chunks.d;
+      const int64_t slot = slots[first + r];
+      if (slot < 0 || (uint64_t)slot >= c.capacity) continue;   // the same for all lanes of a block
+      const void *row = static_cast<const uint8_t *>(rows) + (size_t)(first + r) * stride * elem_size<T>;
+      const uint32_t at = chunk * 8;
+      float v[8];
+      load8<T>(row, at, at < c.dim ? c.dim - at : 0, v);
+      uint32_t most = most8(v);
+#pragma unroll
+      for (int k = 1; k < L; k *= 2) {
+        const uint32_t o = __shfl_xor(most, k, 64);
+        most = most > o ? most : o;
+      }
+      float s, inv;
+      scale_of<FMT>(most, s, inv);
+      uint32_t code[2];
+      encode8<FMT>(v, s, inv, code);
+      if (at < padded) store_codes8<FMT>(c.codes + (size_t)slot * c.row_bytes, chunk, code);
+      if (chunk % L == 0) c.scales[(size_t)slot * c.nb + chunk / L] = s;
+    }
+  }
+}
+
+// one scale a row: a wavefront has a row, and reads it again (from the caches) once its largest magnitude is known
+template <int T, int FMT>
+__global__ __launch_bounds__(256) void row_write_whole_kernel(RowCacheArgs c, const void *rows, size_t stride, const int64_t *slots, uint32_t n) {
+  const uint32_t lane = threadIdx.x % 64;
+  for (uint64_t r = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64; r < n; r += (uint64_t)gridDim.x * 4) {
+    const int64_t slot = slots[r];
+    if (slot < 0 || (uint64_t)slot >= c.capacity) continue;
+    const void *row = static_cast<const uint8_t *>(rows) + (size_t)r * stride * elem_size<T>;
+    const uint32_t padded = (c.dim + 31) / 32 * 32;
+    float v[8];
+    uint32_t most = 0;
+    for (uint32_t at = lane * 8; at < c.dim; at += 512) {
+      load8<T>(row, at, c.dim - at, v);
+      const uint32_t o = most8(v);
+      most = most > o ? most : o;
+    }
+#pragma unroll
+    for (int k = 1; k < 64; k *= 2) {
+      const uint32_t o = __shfl_xor(most, k, 64);
+      most = most > o ? most : o;
+    }
+    float s, inv;
+    scale_of<FMT>(most, s, inv);
+    for (uint32_t at = lane * 8; at < padded; at += 512) {
+      load8<T>(row, at, at < c.dim ? c.dim - at : 0, v);
+      uint32_t code[2];
+      encode8<FMT>(v, s, inv, code);
+      store_codes8<FMT>(c.codes + (size_t)slot * c.row_bytes, at / 8, code);
+    }
+    if (lane == 0) c.scales[slot] = s;
+  }
+}
+
+// rows kept as they are: sixteen bytes a thread
+template <int T>
+__global__ __launch_bounds__(256) void row_copy_in_kernel(RowCacheArgs c, const void *rows, size_t stride, const int64_t *slots, uint32_t n,
+                                                          uint32_t rows_per_wg, FastDiv chunks) {
+  constexpr int E = 16 / elem_size<T>;
+  for (uint64_t first = (uint64_t)blockIdx.x * rows_per_wg; first < n; first += (uint64_t)gridDim.x * rows_per_wg) {
+    const uint32_t mine = n - first < rows_per_wg ? (uint32_t)(n - first) : rows_per_wg;
+    for (uint32_t i = threadIdx.x; i < mine * chunks.d; i += 256) {
+      const uint32_t r = chunks.div(i), chunk = i - r * chunks.d, at = chunk * E;
+      const int64_t slot = slots[first + r];
+      if (slot < 0 || (uint64_t)slot >= c.capacity) continue;
+      const uint8_t *row = static_cast<const uint8_t *>(rows) + (size_t)(first + r) * stride * elem_size<T>;
+      u4 w = {0, 0, 0, 0};
+      if (at + E <= c.dim) {
+        w = *reinterpret_cast<const u4_any *>(row + at * elem_size<T>);
+      } else {
+#pragma unroll
+        for (int k = 0; k < E; k++)
+          if (at + k < c.dim) {
+            if constexpr (T == F32) w[k] = reinterpret_cast<const uint32_t *>(row)[at + k];
+            else w[k / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(row)[at + k] << (16 * (k % 2));
+          }
+      }
+      *reinterpret_cast<u4 *>(c.codes + (size_t)slot * c.row_bytes + chunk * 16) = w;
+    }
+  }
+}
+
+// ---- reading ---------------------------------------------------------------------------------------------------------------
+
+template <int FMT>
+__device__ __forceinline__ void decode8(const uint8_t *row, uint32_t chunk, float (&v)[8]) {
+  if constexpr (FMT == INT4) {
+    const uint32_t w = *reinterpret_cast<const uint32_t *>(row + chunk * 4);
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = (float)((int32_t)(w << (28 - 4 * i)) >> 28);
+  } else {
+    const u2 w = *reinterpret_cast<const u2 *>(row + chunk * 8);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      if constexpr (FMT == INT8) {
+        v[i] = (float)(int8_t)(w[i / 4] >> (8 * (i % 4)));
+      } else {
+        switch (i % 4) {
+          case 0: v[i] = __builtin_amdgcn_cvt_f32_fp8((int)w[i / 4], 0); break;
+          case 1: v[i] = __builtin_amdgcn_cvt_f32_fp8((int)w[i / 4], 1); break;
+          case 2: v[i] = __builtin_amdgcn_cvt_f32_fp8((int)w[i / 4], 2); break;
+          default: v[i] = __builtin_amdgcn_cvt_f32_fp8((int)w[i / 4], 3); break;
+        }
+      }
+    }
+  }
+}
+
+// two fp32 -> two 16-bit elements in a dword, nearest even
+template <int T>
+__device__ __forceinline__ uint32_t narrow2(float a, float b) {
+  uint32_t w;
+  if constexpr (T == F16) {
+    const half2v h = {(_Float16)a, (_Float16)b};
+    __builtin_memcpy(&w, &h, 4);
+  } else {
+    const bf16x2 h = {(__bf16)a, (__bf16)b};
+    __builtin_memcpy(&w, &h, 4);
+  }
+  return w;
+}
+
+template <int T, int FMT>
+__global__ __launch_bounds__(256) void row_read_kernel(RowCacheArgs c, const int64_t *slots, uint32_t n, void *out, size_t stride,
+                                                       uint32_t rows_per_wg, FastDiv chunks, FastDiv block) {
+  for (uint64_t first = (uint64_t)blockIdx.x * rows_per_wg; first < n; first += (uint64_t)gridDim.x * rows_per_wg) {
+    const uint32_t mine = n - first < rows_per_wg ? (uint32_t)(n - first) : rows_per_wg;
+    for (uint32_t i = threadIdx.x; i < mine * chunks.d; i += 256) {
+      const uint32_t r = chunks.div(i), chunk = i - r * chunks.d, at = chunk * 8;
+      const int64_t slot = slots[first + r];
+      float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (slot >= 0 && (uint64_t)slot < c.capacity) {
+        const uint8_t *row = c.codes + (size_t)slot * c.row_bytes;
+        if constexpr (FMT == NATIVE) {
+          load8<T>(row, at, 8, v);   // the row's memory is whole units
+        } else {
+          const float s = c.scales[(size_t)slot * c.nb + block.div(at)];   // a block begins at a multiple of eight
+          decode8<FMT>(row, chunk, v);
+#pragma unroll
+          for (int k = 0; k < 8; k++) v[k] *= s;
+          // a block whose codes reach past the type's range (a largest magnitude next to its end): nothing finite becomes infinite
+          constexpr float most = T == F32 ? 3.40282347e38f : T == BF16 ? 3.38953139e38f : 65504.0f;
+          if (s > most / (FMT == E4M3 ? 448.0f : FMT == INT8 ? 128.0f : 8.0f)) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = __builtin_fabsf(v[k]) > most ? __builtin_copysignf(most, v[k]) : v[k];
+          }
+        }
+      }
+      uint8_t *dst = static_cast<uint8_t *>(out) + ((size_t)(first + r) * stride + at) * elem_size<T>;
+      if constexpr (T == F32) {
+        if (at + 8 <= c.dim) {
+          reinterpret_cast<u4_any *>(dst)[0] = u4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+          reinterpret_cast<u4_any *>(dst)[1] = u4{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])};
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; k++)
+            if (at + k < c.dim) reinterpret_cast<float *>(dst)[k] = v[k];
+        }
+      } else {
+        const u4 w = {narrow2<T>(v[0], v[1]), narrow2<T>(v[2], v[3]), narrow2<T>(v[4], v[5]), narrow2<T>(v[6], v[7])};
+        if (at + 8 <= c.dim) {
+          *reinterpret_cast<u4_any *>(dst) = w;
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; k++)
+            if (at + k < c.dim) reinterpret_cast<uint16_t *>(dst)[k] = (uint16_t)(w[k / 2] >> (16 * (k % 2)));
+        }
+      }
+    }
+  }
+}
+
+// ---- products with a partition's rows --------------------------------------------------------------------------------------
+//
+// p[m][j] = sum_k q[m][k] c[j][k] s[j][k / block].  The codes are integers or e4m3 values that a 16-bit float holds exactly, so the
+// matrix cores multiply codes with queries, and a block's sum is multiplied by its scale in fp32: no operand is rounded.
+// fp32 operands go in as three bf16 each (8 + 8 + 8 bits of the significand, cut off exactly).
+
+template <int Q>
+__device__ __forceinline__ f32x16 mfma(u4 a, u4 b, f32x16 c) {
+  if constexpr (Q == F16) {
+    half8 x, y;
+    __builtin_memcpy(&x, &a, 16);
+    __builtin_memcpy(&y, &b, 16);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0);
+  } else {
+    bf16x8 x, y;
+    __builtin_memcpy(&x, &a, 16);
+    __builtin_memcpy(&y, &b, 16);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
+  }
+}
+
+// x = hi + mid + lo, each a bf16 in the upper half of its dword.  An infinity or a NaN is hi alone.
+__device__ __forceinline__ void split3(uint32_t x, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
+  hi = x & 0xffff0000u;
+  if ((x & 0x7f800000u) == 0x7f800000u) {
+    if (x & 0xffffu) hi |= 0x400000u;   // a NaN whose payload sits in the bits cut off
+    mid = lo = 0;
+    return;
+  }
+  const float r = __uint_as_float(x) - __uint_as_float(hi);
+  mid = __float_as_uint(r) & 0xffff0000u;
+  lo = __float_as_uint(r - __uint_as_float(mid));
+}
+__device__ __forceinline__ uint32_t upper2(uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
+
+// eight fp32 -> eight bf16 in each of three planes
+__device__ __forceinline__ void planes8(const float (&v)[8], u4 (&p)[3]) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    uint32_t a[3], b[3];
+    split3(__float_as_uint(v[2 * i]), a[0], a[1], a[2]);
+    split3(__float_as_uint(v[2 * i + 1]), b[0], b[1], b[2]);
+#pragma unroll
+    for (int k = 0; k < 3; k++) p[k][i] = upper2(a[k], b[k]);
+  }
+}
+
+// eight codes -> eight 16-bit floats
+template <int FMT, int Q>
+__device__ __forceinline__ u4 widen8(uint32_t w0, uint32_t w1) {
+  u4 r;
+  if constexpr (FMT == E4M3) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int w = (int)(i < 2 ? w0 : w1);
+      if constexpr (Q == F16) {
+        const half2v h = i % 2 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false);
+        uint32_t x;
+        __builtin_memcpy(&x, &h, 4);
+        r[i] = x;
+      } else {
+        const bf16x2 h = i % 2 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false);
+        uint32_t x;
+        __builtin_memcpy(&x, &h, 4);
+        r[i] = x;
+      }
+    }
+  } else {
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      if constexpr (FMT == INT8) f[i] = (float)(int8_t)((i < 4 ? w0 : w1) >> (8 * (i % 4)));
+      else f[i] = (float)((int32_t)(w0 << (28 - 4 * i)) >> 28);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if constexpr (Q == F16) r[i] = narrow2<F16>(f[2 * i], f[2 * i + 1]);
+      else r[i] = upper2(__float_as_uint(f[2 * i]), __float_as_uint(f[2 * i + 1]));
+    }
+  }
+  return r;
+}
+
+constexpr int ROW_TILE = 128;   // rows of a workgroup: 32 for each of its four wavefronts
+
+// what a lane holds of one row and one unit of 32 elements: the 16 elements of its half, as two fragments (in up to three planes)
+template <int FMT, int Q>
+struct Unit {
+  static constexpr int BYTES = FMT == NATIVE ? 32 * elem_size<Q> : FMT == INT4 ? 16 : 32;
+  static constexpr int PLANES = FMT == NATIVE && Q == F32 ? 3 : 1;
+  uint32_t raw[BYTES / 8];
+
+  __device__ __forceinline__ void load(const uint8_t *row, uint32_t unit, uint32_t half) {
+    const uint8_t *p = row + unit * BYTES + half * (BYTES / 2);
+    if constexpr (BYTES == 16) {
+      const u2 w = *reinterpret_cast<const u2 *>(p);
+      raw[0] = w[0];
+      raw[1] = w[1];
+    } else {
+#pragma unroll
+      for (int i = 0; i < BYTES / 32; i++) {
+        const u4 w = reinterpret_cast<const u4 *>(p)[i];
+#pragma unroll
+        for (int k = 0; k < 4; k++) raw[4 * i + k] = w[k];
+      }
+    }
+  }
+  __device__ __forceinline__ void fragment(int f, u4 (&out)[PLANES]) const {
+    if constexpr (FMT == NATIVE && Q == F32) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = __uint_as_float(raw[8 * f + i]);
+      planes8(v, out);
+    } else if constexpr (FMT == NATIVE) {
+      out[0] = u4{raw[4 * f], raw[4 * f + 1], raw[4 * f + 2], raw[4 * f + 3]};
+    } else if constexpr (FMT == INT4) {
+      out[0] = widen8<INT4, Q>(raw[f], 0);
+    } else {
+      out[0] = widen8<FMT, Q>(raw[2 * f], raw[2 * f + 1]);
+    }
+  }
+};
+
+__device__ __forceinline__ int32_t cut(int32_t x, int32_t most) { return x < 0 ? 0 : x > most ? most : x; }
+
+// queries [lo, lo + m) and rows of partition g
+__device__ __forceinline__ void partition(const PartitionArgs &a, uint32_t g, uint32_t &lo, uint32_t &m, uint32_t &n) {
+  const int32_t from = cut(a.query_offsets[g], (int32_t)a.n_queries), to = cut(a.query_offsets[g + 1], (int32_t)a.n_queries);
+  lo = (uint32_t)from;
+  m = to > from ? (uint32_t)(to - from) : 0;
+  n = (uint32_t)cut(a.row_counts[g], (int32_t)a.most_rows);
+}
+
+__device__ __noinline__ float plain_product(const float *row, const float *query, uint32_t dim) {
+  float p = 0.0f;
+  for (uint32_t k = 0; k < dim; k++) p = __builtin_fmaf(query[k], row[k], p);
+  return p;
+}
+
+// Each workgroup works through tiles of TQ = 32 QT queries x 128 rows, tile t of workgroup b being b, b + gridDim.x, ...  Which
+// partition a tile belongs to is found from the offsets and counts themselves (they are on the device): every workgroup sums the
+// partitions' tiles once, 256 threads a share each.
+template <int FMT, int Q, int QT>
+__global__ __launch_bounds__(256) void partition_scores_kernel(PartitionArgs a, FastDiv page) {
+  constexpr int TQ = 32 * QT;
+  constexpr int QP = Q == F32 ? 3 : 1;                          // planes of a query
+  constexpr int KU = (QT == 1 ? 48 : 64) * 1024 / (2048 * QP * QT);   // units of 32 elements staged at a time: 48 / 64 KiB
+  typedef Unit<FMT, Q> U;
+  __shared__ u4 staged[KU * 2 * QP * QT * 64];
+  __shared__ uint32_t before[257];
+
+  const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+  const uint32_t per = (a.n_partitions + 255) / 256;
+  {
+    uint32_t sum = 0;
+    for (uint32_t i = 0; i < per; i++) {
+      const uint32_t g = tid * per + i;
+      if (g >= a.n_partitions) break;
+      uint32_t lo, m, n;
+      partition(a, g, lo, m, n);
+      sum += (m + TQ - 1) / TQ * ((n + ROW_TILE - 1) / ROW_TILE);
+    }
+    before[tid + 1] = sum;
+    if (tid == 0) before[0] = 0;
+    __syncthreads();
+    for (uint32_t k = 1; k < 256; k *= 2) {
+      const uint32_t v = tid >= k ? before[tid + 1 - k] : 0;
+      __syncthreads();
+      before[tid + 1] += v;
+      __syncthreads();
+    }
+  }
+  const uint32_t total = before[256];
+  const uint32_t units = (a.c.dim + 31) / 32;
+  const uint32_t block_units = FMT == NATIVE || a.c.block >= a.c.dim ? units : a.c.block / 32;
+  const float gone = a.form == RSGPU_SCORES_DISTANCE ? __builtin_inff() : -__builtin_inff();
+
+  for (uint32_t t = blockIdx.x; t < total; t += gridDim.x) {
+    uint32_t low = 0, high = 256;                               // before[low] <= t < before[high]
+    while (high - low > 1) {
+      const uint32_t mid = (low + high) / 2;
+      if (before[mid] <= t) low = mid;
+      else high = mid;
+    }
+    uint32_t left = t - before[low], g = low * per, lo, m, n, qt;
+    for (;; g++) {
+      partition(a, g, lo, m, n);
+      qt = (m + TQ - 1) / TQ;
+      const uint32_t tiles = qt * ((n + ROW_TILE - 1) / ROW_TILE);
+      if (left < tiles) break;
+      left -= tiles;
+    }
+    const uint32_t row_tile = left / qt, q0 = lo + (left - row_tile * qt) * TQ, q_end = lo + m;
+    const uint32_t j = row_tile * ROW_TILE + wave * 32 + lane % 32, half = lane / 32;
+
+    // the row of this lane; one that is not there is read from slot 0 and not used
+    const uint8_t *row = a.c.codes;
+    const float *scale = a.c.scales;
+    bool there = false;
+    if (j < n) {
+      const uint32_t p = page.div(j);
+      const int32_t id = a.pages[(size_t)g * a.max_pages + p];
+      const uint64_t slot = (uint64_t)(uint32_t)id * page.d + (j - p * page.d);
+      if (id >= 0 && slot < a.c.capacity) {
+        there = true;
+        row += slot * a.c.row_bytes;
+        scale += slot * a.c.nb;
+      }
+    }
+
+    f32x16 acc[QT], part[QT];
+#pragma unroll
+    for (int i = 0; i < QT; i++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[i][r] = part[i][r] = 0.0f;
+
+    for (uint32_t u0 = 0; u0 < units; u0 += KU) {
+      const uint32_t nu = units - u0 < KU ? units - u0 : KU;
+      __syncthreads();
+      for (uint32_t i = tid; i < nu * 4 * TQ; i += 256) {
+        const uint32_t q = i % TQ, chunk = i / TQ, at = u0 * 32 + chunk * 8;   // chunk: unit, half, fragment
+        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        u4 w[QP];
+        const bool some = q0 + q < q_end && at < a.c.dim;
+        const uint8_t *src = static_cast<const uint8_t *>(a.queries) + (size_t)(q0 + q) * a.stride * elem_size<Q>;
+        if constexpr (Q == F32) {
+          if (some) load8<F32>(src, at, a.c.dim - at, v);
+          planes8(v, w);
+        } else {
+          w[0] = u4{0, 0, 0, 0};
+          if (some) {
+            if (at + 8 <= a.c.dim) {
+              w[0] = *reinterpret_cast<const u4_any *>(src + at * 2);
+            } else {
+              for (uint32_t k = 0; at + k < a.c.dim; k++) {
+                const uint32_t x = (uint32_t)reinterpret_cast<const uint16_t *>(src)[at + k] << (16 * (k % 2));
+                if (k / 2 == 0) w[0][0] |= x;
+                else if (k / 2 == 1) w[0][1] |= x;
+                else if (k / 2 == 2) w[0][2] |= x;
+                else w[0][3] |= x;
+              }
+            }
+          }
+        }
+        const uint32_t u = chunk / 4, h = chunk / 2 % 2, f = chunk % 2;
+#pragma unroll
+        for (int p = 0; p < QP; p++) staged[(((u * 2 + f) * QP + p) * QT + q / 32) * 64 + h * 32 + q % 32] = w[p];
+      }
+      __syncthreads();
+      for (uint32_t u = 0; u < nu; u++) {
+        U x;
+        x.load(row, u0 + u, half);
+#pragma unroll
+        for (int f = 0; f < 2; f++) {
+          u4 b[U::PLANES];
+          x.fragment(f, b);
+#pragma unroll
+          for (int i = 0; i < QT; i++)
+#pragma unroll
+            for (int p = 0; p < QP; p++) {
+              const u4 q = staged[(((u * 2 + f) * QP + p) * QT + i) * 64 + lane];
+#pragma unroll
+              for (int k = 0; k < U::PLANES; k++)
+                if (p + k < 3) part[i] = mfma<Q>(q, b[k], part[i]);   // the planes left out are below 2^-24 of the product
+            }
+        }
+        if ((u0 + u + 1) % block_units == 0 || u0 + u + 1 == units) {
+          const float s = FMT == NATIVE ? 1.0f : scale[(u0 + u) / block_units];
+#pragma unroll
+          for (int i = 0; i < QT; i++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+              acc[i][r] = __builtin_fmaf(s, part[i][r], acc[i][r]);
+              part[i][r] = 0.0f;
+            }
+        }
+      }
+    }
+
+    if (j < n) {
+#pragma unroll
+      for (int i = 0; i < QT; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          const uint32_t q = q0 + i * 32 + 8 * (r / 4) + 4 * half + r % 4;
+          if (q < q_end) {
+            float p = acc[i][r];
+            if constexpr (FMT == NATIVE && Q == F32) {
+              // an infinity meets the other side's planes, some of them 0: the sum is taken again, element by element
+              if (p != p && there) p = plain_product(reinterpret_cast<const float *>(row), static_cast<const float *>(a.queries) + q * a.stride, a.c.dim);
+            }
+            if (a.form == RSGPU_SCORES_DISTANCE) p = 1.0f - p;
+            a.scores[(size_t)q * a.ld + j] = there ? p : gone;
+          }
+        }
+    }
+  }
+}
+
+// ---- rules on scores -------------------------------------------------------------------------------------------------------
+
+constexpr uint32_t COLUMNS = 4096;   // columns of a workgroup, whose counts of a query's two lists are kept in LDS
+
+// A workgroup finds in the lists what falls among its columns (sums and maxima of integers: the same in any order), then goes over
+// them once.
+__global__ __launch_bounds__(256) void adjust_scores_kernel(AdjustArgs a, uint32_t tiles, uint64_t work) {
+  __shared__ uint32_t times[COLUMNS];   // how often a column was shown
+  __shared__ uint32_t boost[COLUMNS];   // 1 + the place in the list of a column's last boost, 0: none
+  const uint32_t tid = threadIdx.x;
+  for (uint64_t w = blockIdx.x; w < work; w += gridDim.x) {
+    const uint32_t m = (uint32_t)(w / tiles), c0 = (uint32_t)(w - (uint64_t)m * tiles) * COLUMNS;
+    uint32_t n = a.n_columns;
+    if (a.counts) n = (uint32_t)cut(a.counts[m], (int32_t)n);
+    if (c0 >= n) continue;   // the same for the whole workgroup
+    const uint32_t mine = n - c0 < COLUMNS ? n - c0 : COLUMNS;
+    int32_t s0 = 0, s1 = 0, b0 = 0, b1 = 0;
+    if (a.r.seen_offsets) {
+      s0 = cut(a.r.seen_offsets[m], (int32_t)a.r.n_seen);
+      s1 = cut(a.r.seen_offsets[m + 1], (int32_t)a.r.n_seen);
+    }
+    if (a.r.bias_offsets) {
+      b0 = cut(a.r.bias_offsets[m], (int32_t)a.r.n_bias);
+      b1 = cut(a.r.bias_offsets[m + 1], (int32_t)a.r.n_bias);
+    }
+    const bool lists = s1 > s0 || b1 > b0;
+    if (lists) {
+      __syncthreads();   // the last piece's counts have been read
+      for (uint32_t i = tid; i < mine; i += 256) times[i] = boost[i] = 0;
+      __syncthreads();
+      for (int32_t i = s0 + (int32_t)tid; i < s1; i += 256) {
+        const uint32_t c = (uint32_t)a.r.seen_ids[i] - c0;
+        if (c < mine) atomicAdd(&times[c], 1u);
+      }
+      for (int32_t i = b0 + (int32_t)tid; i < b1; i += 256) {
+        const uint32_t c = (uint32_t)a.r.bias_ids[i] - c0;
+        if (c < mine) atomicMax(&boost[c], (uint32_t)(i - b0) + 1);
+      }
+      __syncthreads();
+    }
+    const bool distance = a.r.form == RSGPU_SCORES_DISTANCE;
+    const float rep = a.r.repetition ? a.r.repetition[m] : 1.0f;
+    const float freq = a.r.frequency ? a.r.frequency[m] : 0.0f;
+    const float pres = a.r.presence ? a.r.presence[m] : 0.0f;
+    const uint32_t *mask = nullptr;
+    if (a.r.mask) {
+      const int64_t which = a.r.mask_rows ? a.r.mask_rows[m] : (int64_t)m;
+      if (which >= 0 && (uint64_t)which < a.r.n_masks) mask = a.r.mask + (size_t)which * a.r.mask_words;
+    }
+    const float *in = a.in + (size_t)m * a.ld + c0;
+    float *out = a.out + (size_t)m * a.ld + c0;
+    for (uint32_t i = tid; i < mine; i += 256) {
+      float v = in[i];
+      if (lists) {
+        const uint32_t k = times[i], b = boost[i];
+        if (k | b) {
+          float p = distance ? 1.0f - v : v;
+          if (k) {
+            p = p > 0.0f ? p / rep : p * rep;
+            p -= __builtin_fmaf((float)k, freq, pres);
+          }
+          if (b) p += a.r.bias_values[b0 + b - 1];
+          v = distance ? 1.0f - p : p;
+        }
+      }
+      if (mask && !((mask[(c0 + i) / 32] >> ((c0 + i) % 32)) & 1u)) v = distance ? __builtin_inff() : -__builtin_inff();
+      out[i] = v;
+    }
+  }
+}
+
+// a grid holds fewer than 2^32 threads; kernels go round when there is more work
+constexpr uint64_t MOST_WORKGROUPS = 1 << 20;
+uint32_t workgroups(uint64_t work) { return (uint32_t)(work < MOST_WORKGROUPS ? work : MOST_WORKGROUPS); }
+
+// rows of a workgroup so that it has a few chunks a thread, with enough workgroups to fill the chip first
+uint32_t rows_a_workgroup(uint32_t n, uint32_t chunks) {
+  uint32_t rows = (1024 + chunks - 1) / chunks;
+  while (rows > 1 && (n + rows - 1) / rows < 2048) rows = (rows + 1) / 2;
+  return rows;
+}
+
+template <int T, int FMT>
+void write_as(const RowCacheArgs &c, const void *rows, size_t stride, const int64_t *slots, uint32_t n, hipStream_t s) {
+  if (c.block != 32 && c.block != 64 && c.block != 128) {
+    hipLaunchKernelGGL((row_write_whole_kernel<T, FMT>), dim3(workgroups(((uint64_t)n + 3) / 4)), dim3(256), 0, s, c, rows, stride, slots, n);
+    return;
+  }
+  const uint32_t chunks = c.nb * (c.block / 8), per = rows_a_workgroup(n, chunks);
+  const dim3 grid(workgroups(((uint64_t)n + per - 1) / per));
+  const FastDiv d(chunks);
+  if (c.block == 32) hipLaunchKernelGGL((row_write_kernel<T, FMT, 4>), grid, dim3(256), 0, s, c, rows, stride, slots, n, per, d);
+  else if (c.block == 64) hipLaunchKernelGGL((row_write_kernel<T, FMT, 8>), grid, dim3(256), 0, s, c, rows, stride, slots, n, per, d);
+  else hipLaunchKernelGGL((row_write_kernel<T, FMT, 16>), grid, dim3(256), 0, s, c, rows, stride, slots, n, per, d);
+}
+
+template <int T>
+void write_from(const RowCacheArgs &c, const void *rows, size_t stride, const int64_t *slots, uint32_t n, hipStream_t s) {
+  switch (c.format) {
+    case INT8: return write_as<T, INT8>(c, rows, stride, slots, n, s);
+    case E4M3: return write_as<T, E4M3>(c, rows, stride, slots, n, s);
+    case INT4: return write_as<T, INT4>(c, rows, stride, slots, n, s);
+    default: {
+      const uint32_t chunks = c.row_bytes / 16, per = rows_a_workgroup(n, chunks);
+      hipLaunchKernelGGL((row_copy_in_kernel<T>), dim3(workgroups(((uint64_t)n + per - 1) / per)), dim3(256), 0, s, c, rows, stride, slots, n, per, FastDiv(chunks));
+    }
+  }
+}
+
+template <int T>
+void read_to(const RowCacheArgs &c, const int64_t *slots, uint32_t n, void *out, size_t stride, hipStream_t s) {
+  const uint32_t chunks = (c.dim + 7) / 8, per = rows_a_workgroup(n, chunks);
+  const dim3 grid(workgroups(((uint64_t)n + per - 1) / per));
+  const FastDiv d(chunks), b(c.block);
+  switch (c.format) {
+    case INT8: hipLaunchKernelGGL((row_read_kernel<T, INT8>), grid, dim3(256), 0, s, c, slots, n, out, stride, per, d, b); break;
+    case E4M3: hipLaunchKernelGGL((row_read_kernel<T, E4M3>), grid, dim3(256), 0, s, c, slots, n, out, stride, per, d, b); break;
+    case INT4: hipLaunchKernelGGL((row_read_kernel<T, INT4>), grid, dim3(256), 0, s, c, slots, n, out, stride, per, d, b); break;
+    default: hipLaunchKernelGGL((row_read_kernel<T, NATIVE>), grid, dim3(256), 0, s, c, slots, n, out, stride, per, d, b); break;
+  }
+}
+
+template <int FMT, int Q>
+void scores_as(const PartitionArgs &a, hipStream_t s) {
+  const FastDiv page(a.page_rows);
+  const bool many = a.n_queries / a.n_partitions >= 48;
+  const uint64_t tq = many ? 128 : 32, asked = a.n_partitions < a.n_queries ? a.n_partitions : a.n_queries;
+  const uint64_t most = (a.n_queries / tq + asked) * ((a.most_rows + ROW_TILE - 1) / ROW_TILE);
+  const dim3 grid((uint32_t)(most < 2048 ? most : 2048));
+  if (many) hipLaunchKernelGGL((partition_scores_kernel<FMT, Q, 4>), grid, dim3(256), 0, s, a, page);
+  else hipLaunchKernelGGL((partition_scores_kernel<FMT, Q, 1>), grid, dim3(256), 0, s, a, page);
+}
+
+template <int Q>
+void scores_from(const PartitionArgs &a, hipStream_t s) {
+  switch (a.c.format) {
+    case INT8: return scores_as<INT8, Q>(a, s);
+    case E4M3: return scores_as<E4M3, Q>(a, s);
+    case INT4: return scores_as<INT4, Q>(a, s);
+    default: return scores_as<NATIVE, Q>(a, s);
+  }
+}
+
+}  // namespace
+
+void launch_row_write(const RowCacheArgs &c, const void *rows, size_t stride, const int64_t *slots, uint32_t n, hipStream_t s) {
+  if (c.type == F32) write_from<F32>(c, rows, stride, slots, n, s);
+  else if (c.type == F16) write_from<F16>(c, rows, stride, slots, n, s);
+  else write_from<BF16>(c, rows, stride, slots, n, s);
+  HIP_CHECK(hipGetLastError());
+}
+
+void launch_row_read(const RowCacheArgs &c, const int64_t *slots, uint32_t n, void *out, size_t stride, hipStream_t s) {
+  if (c.type == F32) read_to<F32>(c, slots, n, out, stride, s);
+  else if (c.type == F16) read_to<F16>(c, slots, n, out, stride, s);
+  else read_to<BF16>(c, slots, n, out, stride, s);
+  HIP_CHECK(hipGetLastError());
+}
+
+void launch_partition_scores(const PartitionArgs &a, hipStream_t s) {
+  if (a.c.type == F32) scores_from<F32>(a, s);
+  else if (a.c.type == F16) scores_from<F16>(a, s);
+  else scores_from<BF16>(a, s);
+  HIP_CHECK(hipGetLastError());
+}
+
+void launch_adjust_scores(const AdjustArgs &a, hipStream_t s) {
+  const uint32_t tiles = (a.n_columns + COLUMNS - 1) / COLUMNS;
+  const uint64_t work = (uint64_t)tiles * a.n_queries;
+  hipLaunchKernelGGL(adjust_scores_kernel, dim3(workgroups(work)), dim3(256), 0, s, a, tiles, work);
+  HIP_CHECK(hipGetLastError());
+}
+
+}  // namespace rsgpu
