@@ -8,7 +8,7 @@
 namespace rsgpu {
 
 // elements of a row in memory: every kernel works on whole units of 32
-inline uint32_t rows_padded(uint32_t dim) { return (dim + 31) / 32 * 32; }
+__host__ __device__ inline uint32_t rows_padded(uint32_t dim) { return (dim + 31) / 32 * 32; }
 
 struct RowCacheArgs {   // a checked RSGPU_RowCache
   uint8_t *codes;

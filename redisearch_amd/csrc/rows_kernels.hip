@@ -2,6 +2,8 @@
 // of ragged groups of queries with the paged rows of their partitions, and the rules on a batch's scores.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "rows.hpp"
 
 namespace rsgpu {
@@ -358,6 +360,22 @@ __device__ __forceinline__ f32x16 mfma(u4 a, u4 b, f32x16 c) {
   }
 }
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+template <int Q>
+__device__ __forceinline__ f32x4 mfma16(u4 a, u4 b, f32x4 c) {
+  if constexpr (Q == F16) {
+    half8 x, y;
+    __builtin_memcpy(&x, &a, 16);
+    __builtin_memcpy(&y, &b, 16);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0);
+  } else {
+    bf16x8 x, y;
+    __builtin_memcpy(&x, &a, 16);
+    __builtin_memcpy(&y, &b, 16);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0);
+  }
+}
+
 // x = hi + mid + lo, each a bf16 in the upper half of its dword.  An infinity or a NaN is hi alone.
 __device__ __forceinline__ void split3(uint32_t x, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
   hi = x & 0xffff0000u;
@@ -384,7 +402,18 @@ __device__ __forceinline__ void planes8(const float (&v)[8], u4 (&p)[3]) {
   }
 }
 
-// eight codes -> eight 16-bit floats
+// eight codes -> eight 16-bit floats (INT4 with bf16: sixteenths of the codes, CODE_UNIT)
+template <int FMT, int Q>
+constexpr float CODE_UNIT = FMT == INT4 && Q != F16 ? 16.0f : 1.0f;
+
+__device__ __forceinline__ uint32_t minus2(uint32_t x, float y) {
+  half2v h;
+  __builtin_memcpy(&h, &x, 4);
+  h -= half2v{(_Float16)y, (_Float16)y};
+  __builtin_memcpy(&x, &h, 4);
+  return x;
+}
+
 template <int FMT, int Q>
 __device__ __forceinline__ u4 widen8(uint32_t w0, uint32_t w1) {
   u4 r;
@@ -404,18 +433,26 @@ __device__ __forceinline__ u4 widen8(uint32_t w0, uint32_t w1) {
         r[i] = x;
       }
     }
+  } else if constexpr (Q == F16) {
+    // an fp16 number in [1024, 2048) has its integer in the low bits: 1024 + (code + bias), and the bias goes off exactly
+    if constexpr (FMT == INT8) {
+      const uint32_t a = w0 ^ 0x80808080u, b = w1 ^ 0x80808080u;
+      r = u4{minus2(__builtin_amdgcn_perm(0x64646464u, a, 0x04010400u), 1152.0f), minus2(__builtin_amdgcn_perm(0x64646464u, a, 0x04030402u), 1152.0f),
+             minus2(__builtin_amdgcn_perm(0x64646464u, b, 0x04010400u), 1152.0f), minus2(__builtin_amdgcn_perm(0x64646464u, b, 0x04030402u), 1152.0f)};
+    } else {
+      const uint32_t t = w0 ^ 0x88888888u, even = t & 0x0f0f0f0fu, odd = t >> 4 & 0x0f0f0f0fu;
+#pragma unroll
+      for (int i = 0; i < 4; i++) r[i] = minus2(__builtin_amdgcn_perm(odd, even, 0x0c040c00u + 0x00010001u * i) | 0x64006400u, 1032.0f);
+    }
   } else {
     float f[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
       if constexpr (FMT == INT8) f[i] = (float)(int8_t)((i < 4 ? w0 : w1) >> (8 * (i % 4)));
-      else f[i] = (float)((int32_t)(w0 << (28 - 4 * i)) >> 28);
+      else f[i] = __builtin_amdgcn_cvt_off_f32_i4((int)(w0 >> (4 * i)));   // the low four bits, two's complement, by 16
     }
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      if constexpr (Q == F16) r[i] = narrow2<F16>(f[2 * i], f[2 * i + 1]);
-      else r[i] = upper2(__float_as_uint(f[2 * i]), __float_as_uint(f[2 * i + 1]));
-    }
+    for (int i = 0; i < 4; i++) r[i] = upper2(__float_as_uint(f[2 * i]), __float_as_uint(f[2 * i + 1]));
   }
   return r;
 }
@@ -476,9 +513,383 @@ __device__ __noinline__ float plain_product(const float *row, const float *query
   return p;
 }
 
-// Each workgroup works through tiles of TQ = 32 QT queries x 128 rows, tile t of workgroup b being b, b + gridDim.x, ...  Which
-// partition a tile belongs to is found from the offsets and counts themselves (they are on the device): every workgroup sums the
-// partitions' tiles once, 256 threads a share each.
+// Which partition a tile belongs to is found from the offsets and counts themselves (they are on the device): every workgroup sums the
+// partitions' tiles once, a share of the partitions a thread; before[i] are the tiles before thread i's share.  Returns all tiles.
+template <int THREADS>
+__device__ __forceinline__ uint32_t count_tiles(const PartitionArgs &a, uint32_t tq, uint32_t tr, uint32_t per, uint32_t *before, uint32_t *waves) {
+  const uint32_t tid = threadIdx.x, lane = tid % 64;
+  uint32_t sum = 0;
+  for (uint32_t i = 0; i < per; i++) {
+    const uint32_t g = tid * per + i;
+    if (g >= a.n_partitions) break;
+    uint32_t lo, m, n;
+    partition(a, g, lo, m, n);
+    sum += (m + tq - 1) / tq * ((n + tr - 1) / tr);
+  }
+#pragma unroll
+  for (int k = 1; k < 64; k *= 2) {
+    const uint32_t v = __shfl_up(sum, k, 64);
+    if (lane >= (uint32_t)k) sum += v;
+  }
+  if (lane == 63) waves[tid / 64] = sum;
+  __syncthreads();
+  for (uint32_t w = 0; w < tid / 64; w++) sum += waves[w];
+  before[tid + 1] = sum;
+  if (tid == 0) before[0] = 0;
+  __syncthreads();
+  return before[THREADS];
+}
+
+// where tile t is: its partition, that partition's queries and rows, and the tile's number in it
+struct Place {
+  uint32_t g, lo, m, n, left;
+};
+template <int THREADS>
+__device__ __forceinline__ Place find_tile(const PartitionArgs &a, uint32_t tq, uint32_t tr, uint32_t per, const uint32_t *before, uint32_t t) {
+  uint32_t low = 0, high = THREADS;   // before[low] <= t < before[high]
+  while (high - low > 1) {
+    const uint32_t mid = (low + high) / 2;
+    if (before[mid] <= t) low = mid;
+    else high = mid;
+  }
+  Place p;
+  p.left = t - before[low];
+  for (p.g = low * per;; p.g++) {
+    partition(a, p.g, p.lo, p.m, p.n);
+    const uint32_t tiles = (p.m + tq - 1) / tq * ((p.n + tr - 1) / tr);
+    if (p.left < tiles) return p;
+    p.left -= tiles;
+  }
+}
+
+// eight elements of a query as 16-bit fragments (an fp32 query: three planes)
+template <int Q>
+__device__ __forceinline__ void stage8(const PartitionArgs &a, uint32_t query, uint32_t at, u4 (&w)[Q == F32 ? 3 : 1]) {
+  const uint8_t *src = static_cast<const uint8_t *>(a.queries) + (size_t)query * a.stride * elem_size<Q>;
+  if constexpr (Q == F32) {
+    float v[8];
+    load8<F32>(src, at, at < a.c.dim ? a.c.dim - at : 0, v);
+    planes8(v, w);
+  } else if (at + 8 <= a.c.dim) {
+    w[0] = *reinterpret_cast<const u4_any *>(src + at * 2);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      uint32_t x = 0;
+      if (at + 2 * i < a.c.dim) x = reinterpret_cast<const uint16_t *>(src)[at + 2 * i];
+      if (at + 2 * i + 1 < a.c.dim) x |= (uint32_t)reinterpret_cast<const uint16_t *>(src)[at + 2 * i + 1] << 16;
+      w[0][i] = x;
+    }
+  }
+}
+
+// the same where all lanes ask for one partition: scalar loads
+typedef const __attribute__((address_space(4))) int32_t *scalar_i32;
+__device__ __forceinline__ void partition_of_all(const PartitionArgs &a, uint32_t g, uint32_t &lo, uint32_t &m, uint32_t &n) {
+  const scalar_i32 offsets = (scalar_i32)(uintptr_t)a.query_offsets, counts = (scalar_i32)(uintptr_t)a.row_counts;
+  const int32_t from = cut(offsets[g], (int32_t)a.n_queries), to = cut(offsets[g + 1], (int32_t)a.n_queries);
+  lo = (uint32_t)from;
+  m = to > from ? (uint32_t)(to - from) : 0;
+  n = (uint32_t)cut(counts[g], (int32_t)a.most_rows);
+}
+
+// W neighbouring elements of a row, as a lane takes them from LDS
+template <int FMT, int Q, int W>
+struct Piece {
+  static constexpr int BYTES = FMT == NATIVE ? W * elem_size<Q> : FMT == INT4 ? W / 2 : W;
+  static constexpr int PLANES = FMT == NATIVE && Q == F32 ? 3 : 1;
+  uint32_t raw[BYTES / 4];
+
+  // elements 8 f .. 8 f + 7
+  __device__ __forceinline__ void fragment(int f, u4 (&out)[PLANES]) const {
+    if constexpr (FMT == NATIVE && Q == F32) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = __uint_as_float(raw[i]);
+      planes8(v, out);
+    } else if constexpr (FMT == NATIVE) {
+      out[0] = u4{raw[0], raw[1], raw[2], raw[3]};
+    } else if constexpr (FMT == INT4) {
+      out[0] = widen8<INT4, Q>(raw[f], 0);
+    } else {
+      out[0] = widen8<FMT, Q>(raw[2 * f], raw[2 * f + 1]);
+    }
+  }
+};
+
+// Few queries a partition: the rows' bytes are what it takes.  A workgroup has a run of tiles of 16 queries x 16 S rows a wavefront;
+// the queries of a partition are put into LDS once for all its tiles (in parts of KP stages if the rows are longer than that).
+// A wavefront takes its rows in stages of 4 KiB, 16 S rows x 256 / S bytes: four loads of 16 neighbouring bytes a lane, whole lines of
+// the rows, two stages in flight in registers and across tiles.  (Loads in the shape of the matrix instruction's operand touch 16
+// lines each and cost the same whatever they bring: 2.4 TB/s with 8 bytes a lane, 4.6 with 16.)  A stage passes through 4 KiB of LDS
+// that the wavefront has to itself, so nothing but the order of its own instructions guards it, and comes back as operands; the
+// sixteen-byte chunks of a row change places with its number, so that neither side meets a bank twice.
+template <int FMT, int Q, int W, int S, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionArgs a, FastDiv page) {
+  typedef Piece<FMT, Q, W> P;
+  constexpr int QP = Q == F32 ? 3 : 1, FR = W / 8, TQ = 16, WR = 16 * S, TR = WR * WAVES;
+  constexpr int CS = 16 / S;                                  // chunks of a row in a stage
+  constexpr int SP = CS * 16 / (4 * P::BYTES);                // steps of 4 W elements in a stage
+  constexpr int QS = FMT == NATIVE ? 0 : (SP + 3) / 4;        // scale loads a stage and row group: a lane's quarter has every fourth
+  constexpr int KP = (Q == F32 ? 24 : 32) / (SP * FR);        // stages of queries in LDS at a time: 72 or 32 KiB
+  static_assert(SP >= 1 && KP >= 1, "");
+  __shared__ u4 staged[KP * SP * FR * QP * 64];
+  __shared__ u4 passing[WAVES][256];
+  __shared__ uint32_t before[64 * WAVES + 1], wave_sums[WAVES];
+
+  const uint32_t tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), col = lane % 16, quarter = lane / 16;
+  const uint32_t per = (a.n_partitions + 64 * WAVES - 1) / (64 * WAVES);
+  const uint32_t total = count_tiles<64 * WAVES>(a, TQ, TR, per, before, wave_sums);
+  const uint32_t first = (uint32_t)((uint64_t)total * blockIdx.x / gridDim.x), last = (uint32_t)((uint64_t)total * (blockIdx.x + 1) / gridDim.x);
+  if (first == last) return;
+  const uint32_t chunks = a.c.row_bytes / 16, stages = (chunks + CS - 1) / CS;
+  // blocks are one step or two, or the row
+  const uint32_t block_shift = a.c.block >= a.c.dim ? 31 : a.c.block / (4 * W) >= 2 ? 1 : 0;
+  const float gone = a.form == RSGPU_SCORES_DISTANCE ? __builtin_inff() : -__builtin_inff();
+
+  struct Tile {
+    uint32_t g, query_tile, q0, q_end, n, j0;   // j0: the first row of this wavefront
+  };
+  Place start = find_tile<64 * WAVES>(a, TQ, TR, per, before, first);
+  start.g = __builtin_amdgcn_readfirstlane(start.g);
+  start.left = __builtin_amdgcn_readfirstlane(start.left);
+  partition_of_all(a, start.g, start.lo, start.m, start.n);
+  // the loads run ahead of the products, each with a place of their own
+  Place load_at = start, use_at = start;
+  const auto take = [&](Place &at) {
+    uint32_t row_tiles = (at.n + TR - 1) / TR;
+    while (at.left >= (at.m + TQ - 1) / TQ * row_tiles) {   // behind this partition's last tile
+      at.g++;
+      at.left = 0;
+      partition_of_all(a, at.g, at.lo, at.m, at.n);
+      row_tiles = (at.n + TR - 1) / TR;
+    }
+    const uint32_t query_tile = at.left / row_tiles;
+    const Tile t = {at.g, query_tile, at.lo + query_tile * TQ, at.lo + at.m, at.n, (at.left - query_tile * row_tiles) * TR + wave * WR};
+    at.left++;
+    return t;
+  };
+  // page of row j (of a row behind the partition's last: of its first, whose scores are not written)
+  const auto page_of = [&](const Tile &t, uint32_t j) { return a.pages[(size_t)t.g * a.max_pages + (j < t.n ? page.div(j) : 0)]; };
+  // slot of row j in it; one that is not there is read from slot 0 and not used
+  const auto slot_of = [&](uint32_t j, int32_t id, bool &there) {
+    const uint64_t slot = (uint64_t)(uint32_t)id * page.d + (j - page.div(j) * page.d);
+    there = id >= 0 && slot < a.c.capacity;
+    return there ? slot : 0;
+  };
+  // chunk i of a lane: row i * 64 / CS + lane / CS of the wavefront, its chunk number changed by the row's
+  const uint32_t my_row = lane / CS, turn = CS == 4 ? (lane / CS >> 1) & 3 : (lane / CS) & (CS - 1);
+  constexpr uint32_t ROWS_A_LOAD = 64 / CS;
+
+  // ---- loads: the tile they are at, the pages of the next one
+  struct Next {
+    int32_t id[4], scale_id[S];
+  } ids;
+  const auto look_up = [&](const Tile &t) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) ids.id[i] = page_of(t, t.j0 + i * ROWS_A_LOAD + my_row);
+    if (FMT != NATIVE) {
+#pragma unroll
+      for (int k = 0; k < S; k++) ids.scale_id[k] = page_of(t, t.j0 + k * 16 + col);
+    }
+  };
+  const uint8_t *source[4];
+  const float *scale_source[S];
+  const auto rows_of = [&](const Tile &t) {
+    bool there;
+#pragma unroll
+    for (int i = 0; i < 4; i++) source[i] = a.c.codes + slot_of(t.j0 + i * ROWS_A_LOAD + my_row, ids.id[i], there) * a.c.row_bytes;
+    if (FMT != NATIVE) {
+#pragma unroll
+      for (int k = 0; k < S; k++) scale_source[k] = a.c.scales + slot_of(t.j0 + k * 16 + col, ids.scale_id[k], there) * a.c.nb;
+    }
+  };
+  u4 held[2][4];
+  float held_scales[2][S][QS ? QS : 1];
+  uint32_t load_stage = 0, load_tile = first;
+  Tile loading = take(load_at), coming = loading;
+  const auto load_next = [&](u4 (&h)[4], float (&sc)[S][QS ? QS : 1]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t c = load_stage * CS + ((lane % CS) ^ ((CS == 4 ? turn : (i * ROWS_A_LOAD + my_row) & (CS - 1))));
+      h[i] = *reinterpret_cast<const u4 *>(source[i] + (c < chunks ? c : chunks - 1) * 16);
+    }
+#pragma unroll
+    for (int k = 0; k < S; k++)
+#pragma unroll
+      for (int q = 0; q < QS; q++) {
+        const uint32_t b = ((load_stage * SP) >> block_shift) + q * 4 + quarter;
+        sc[k][q] = scale_source[k][b < a.c.nb ? b : a.c.nb - 1];
+      }
+    if (++load_stage == stages) {   // on to the next tile, the last one's again behind the run's end
+      load_stage = 0;
+      if (load_tile + 1 < last) load_tile++;
+      loading = coming;
+      rows_of(loading);
+      if (load_tile + 1 < last) coming = take(load_at);
+      look_up(coming);
+    }
+  };
+
+  // stages p0 .. p0 + np - 1 of a tile's queries into LDS
+  const auto stage = [&](const Tile &t, uint32_t p0, uint32_t np) {
+    const uint32_t asked = t.q_end - t.q0 < TQ ? t.q_end - t.q0 : TQ;   // what is in LDS behind them is multiplied and not used
+    const uint32_t shift = asked > 8 ? 4 : asked > 4 ? 3 : asked > 2 ? 2 : asked > 1 ? 1 : 0;
+    for (uint32_t i = tid; i < np * (SP * FR * 4) << shift; i += 64 * WAVES) {
+      const uint32_t q = i & ((1u << shift) - 1), chunk = i >> shift, f = chunk % FR, h = chunk / FR % 4, st = chunk / (4 * FR);
+      if (q >= asked) continue;
+      u4 w[QP];
+      stage8<Q>(a, t.q0 + q, (p0 * SP + st) * (4 * W) + h * W + f * 8, w);
+#pragma unroll
+      for (int p = 0; p < QP; p++) staged[((st * FR + f) * QP + p) * 64 + h * 16 + q] = w[p];
+    }
+    __syncthreads();
+  };
+
+  look_up(loading);
+  Tile now = take(use_at);
+  stage(now, 0, stages < KP ? stages : KP);
+  uint32_t held_g = now.g, held_q = now.query_tile, held_p = 0;   // whose queries are in LDS, from which stage on
+  rows_of(loading);
+  if (load_tile + 1 < last) coming = take(load_at);
+  look_up(coming);
+  load_next(held[0], held_scales[0]);
+  load_next(held[1], held_scales[1]);
+
+  uint32_t use_stage = 0, use_tile = first;
+  f32x4 acc[S], part[S];
+#pragma unroll
+  for (int k = 0; k < S; k++) acc[k] = part[k] = f32x4{0, 0, 0, 0};
+  u4 *const mine = passing[wave];
+
+  const auto use = [&](u4 (&h)[4], float (&sc)[S][QS ? QS : 1]) {
+    const uint32_t p0 = use_stage / KP * KP;
+    if (held_p != p0 || held_g != now.g || held_q != now.query_tile) {
+      __syncthreads();
+      stage(now, p0, stages - p0 < KP ? stages - p0 : KP);
+      held_g = now.g;
+      held_q = now.query_tile;
+      held_p = p0;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) mine[i * 64 + lane] = h[i];
+    float scale[S][QS ? QS : 1];
+#pragma unroll
+    for (int k = 0; k < S; k++)
+#pragma unroll
+      for (int q = 0; q < QS; q++) scale[k][q] = sc[k][q];
+    load_next(h, sc);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const u4 *queries = staged + (use_stage - p0) * (SP * FR * QP * 64) + lane;
+    const bool last_stage = use_stage + 1 == stages;
+    const uint32_t first_block = (use_stage * SP) >> block_shift;
+#pragma unroll
+    for (int st = 0; st < SP; st++) {
+      P piece[S];
+#pragma unroll
+      for (int k = 0; k < S; k++) {
+        const uint32_t row = k * 16 + col, at = st * 4 * P::BYTES + quarter * P::BYTES;
+        const uint32_t t = CS == 4 ? (row >> 1) & 3 : row & (CS - 1);
+#pragma unroll
+        for (int e = 0; e < (P::BYTES + 15) / 16; e++) {
+          const uint8_t *p = reinterpret_cast<const uint8_t *>(mine + row * CS + ((at / 16 + e) ^ t)) + at % 16;
+          if constexpr (P::BYTES == 4) {
+            piece[k].raw[0] = *reinterpret_cast<const uint32_t *>(p);
+          } else if constexpr (P::BYTES == 8) {
+            const u2 w = *reinterpret_cast<const u2 *>(p);
+            piece[k].raw[0] = w[0];
+            piece[k].raw[1] = w[1];
+          } else {
+            const u4 w = *reinterpret_cast<const u4 *>(p);
+#pragma unroll
+            for (int i = 0; i < 4; i++) piece[k].raw[4 * e + i] = w[i];
+          }
+        }
+      }
+#pragma unroll
+      for (int f = 0; f < FR; f++) {
+        u4 q[QP];
+#pragma unroll
+        for (int p = 0; p < QP; p++) q[p] = queries[((st * FR + f) * QP + p) * 64];
+#pragma unroll
+        for (int k = 0; k < S; k++) {
+          u4 b[P::PLANES];
+          piece[k].fragment(f, b);
+          if (FMT == NATIVE) {   // behind the row's end its last chunk comes again: an infinity there would meet a zero
+            const bool in = (use_stage * SP + st) * 4 * W + quarter * W < a.c.row_bytes / elem_size<Q>;
+#pragma unroll
+            for (int c = 0; c < P::PLANES; c++)
+#pragma unroll
+              for (int e = 0; e < 4; e++) b[c][e] = in ? b[c][e] : 0;
+          }
+#pragma unroll
+          for (int p = 0; p < QP; p++)
+#pragma unroll
+            for (int c = 0; c < P::PLANES; c++)
+              if (p + c < 3) part[k] = mfma16<Q>(q[p], b[c], part[k]);   // the planes left out are below 2^-24 of the product
+        }
+      }
+      if (FMT != NATIVE) {
+        const uint32_t step = use_stage * SP + st;
+        if (((step + 1) & ((1u << block_shift) - 1)) == 0 || (last_stage && st == SP - 1)) {
+          const uint32_t b = (step >> block_shift) - first_block;
+#pragma unroll
+          for (int k = 0; k < S; k++) {
+            float v = scale[k][0];
+#pragma unroll
+            for (int q = 1; q < QS; q++) v = b / 4 == (uint32_t)q ? scale[k][q] : v;
+            v = __uint_as_float(__builtin_amdgcn_ds_bpermute((b % 4 * 16 + col) * 4, __float_as_uint(v)));
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+              acc[k][r] = __builtin_fmaf(v, part[k][r], acc[k][r]);
+              part[k][r] = 0.0f;
+            }
+          }
+        }
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (!last_stage) {
+      use_stage++;
+      return;
+    }
+
+#pragma unroll
+    for (int k = 0; k < S; k++) {
+      const uint32_t j = now.j0 + k * 16 + col;
+      if (j < now.n && quarter * 4 < now.q_end - now.q0) {
+        bool there;
+        const uint64_t slot = slot_of(j, page_of(now, j), there);
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const uint32_t q = now.q0 + quarter * 4 + r;
+          if (q < now.q_end) {
+            float p = FMT == NATIVE ? part[k][r] : acc[k][r] * CODE_UNIT<FMT, Q>;
+            if constexpr (FMT == NATIVE && Q == F32) {
+              // an infinity meets the other side's planes, some of them 0: the sum is taken again, element by element
+              if (p != p && there)
+                p = plain_product(reinterpret_cast<const float *>(a.c.codes + slot * a.c.row_bytes), static_cast<const float *>(a.queries) + q * a.stride, a.c.dim);
+            }
+            if (a.form == RSGPU_SCORES_DISTANCE) p = 1.0f - p;
+            a.scores[(size_t)q * a.ld + j] = there ? p : gone;
+          }
+        }
+      }
+      acc[k] = part[k] = f32x4{0, 0, 0, 0};
+    }
+    use_stage = 0;
+    if (++use_tile < last) now = take(use_at);
+  };
+  for (;;) {
+    use(held[0], held_scales[0]);
+    if (use_tile == last) break;
+    use(held[1], held_scales[1]);
+    if (use_tile == last) break;
+  }
+}
+
 template <int FMT, int Q, int QT>
 __global__ __launch_bounds__(256) void partition_scores_kernel(PartitionArgs a, FastDiv page) {
   constexpr int TQ = 32 * QT;
@@ -486,50 +897,19 @@ __global__ __launch_bounds__(256) void partition_scores_kernel(PartitionArgs a, 
   constexpr int KU = (QT == 1 ? 48 : 64) * 1024 / (2048 * QP * QT);   // units of 32 elements staged at a time: 48 / 64 KiB
   typedef Unit<FMT, Q> U;
   __shared__ u4 staged[KU * 2 * QP * QT * 64];
-  __shared__ uint32_t before[257];
+  __shared__ uint32_t before[257], wave_sums[4];
 
   const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
   const uint32_t per = (a.n_partitions + 255) / 256;
-  {
-    uint32_t sum = 0;
-    for (uint32_t i = 0; i < per; i++) {
-      const uint32_t g = tid * per + i;
-      if (g >= a.n_partitions) break;
-      uint32_t lo, m, n;
-      partition(a, g, lo, m, n);
-      sum += (m + TQ - 1) / TQ * ((n + ROW_TILE - 1) / ROW_TILE);
-    }
-    before[tid + 1] = sum;
-    if (tid == 0) before[0] = 0;
-    __syncthreads();
-    for (uint32_t k = 1; k < 256; k *= 2) {
-      const uint32_t v = tid >= k ? before[tid + 1 - k] : 0;
-      __syncthreads();
-      before[tid + 1] += v;
-      __syncthreads();
-    }
-  }
-  const uint32_t total = before[256];
+  const uint32_t total = count_tiles<256>(a, TQ, ROW_TILE, per, before, wave_sums);
   const uint32_t units = (a.c.dim + 31) / 32;
   const uint32_t block_units = FMT == NATIVE || a.c.block >= a.c.dim ? units : a.c.block / 32;
   const float gone = a.form == RSGPU_SCORES_DISTANCE ? __builtin_inff() : -__builtin_inff();
 
   for (uint32_t t = blockIdx.x; t < total; t += gridDim.x) {
-    uint32_t low = 0, high = 256;                               // before[low] <= t < before[high]
-    while (high - low > 1) {
-      const uint32_t mid = (low + high) / 2;
-      if (before[mid] <= t) low = mid;
-      else high = mid;
-    }
-    uint32_t left = t - before[low], g = low * per, lo, m, n, qt;
-    for (;; g++) {
-      partition(a, g, lo, m, n);
-      qt = (m + TQ - 1) / TQ;
-      const uint32_t tiles = qt * ((n + ROW_TILE - 1) / ROW_TILE);
-      if (left < tiles) break;
-      left -= tiles;
-    }
-    const uint32_t row_tile = left / qt, q0 = lo + (left - row_tile * qt) * TQ, q_end = lo + m;
+    const Place at = find_tile<256>(a, TQ, ROW_TILE, per, before, t);
+    const uint32_t g = at.g, n = at.n, qt = (at.m + TQ - 1) / TQ;
+    const uint32_t row_tile = at.left / qt, q0 = at.lo + (at.left - row_tile * qt) * TQ, q_end = at.lo + at.m;
     const uint32_t j = row_tile * ROW_TILE + wave * 32 + lane % 32, half = lane / 32;
 
     // the row of this lane; one that is not there is read from slot 0 and not used
@@ -557,30 +937,10 @@ __global__ __launch_bounds__(256) void partition_scores_kernel(PartitionArgs a, 
       const uint32_t nu = units - u0 < KU ? units - u0 : KU;
       __syncthreads();
       for (uint32_t i = tid; i < nu * 4 * TQ; i += 256) {
-        const uint32_t q = i % TQ, chunk = i / TQ, at = u0 * 32 + chunk * 8;   // chunk: unit, half, fragment
-        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        const uint32_t q = i % TQ, chunk = i / TQ;   // chunk: unit, half, fragment
         u4 w[QP];
-        const bool some = q0 + q < q_end && at < a.c.dim;
-        const uint8_t *src = static_cast<const uint8_t *>(a.queries) + (size_t)(q0 + q) * a.stride * elem_size<Q>;
-        if constexpr (Q == F32) {
-          if (some) load8<F32>(src, at, a.c.dim - at, v);
-          planes8(v, w);
-        } else {
-          w[0] = u4{0, 0, 0, 0};
-          if (some) {
-            if (at + 8 <= a.c.dim) {
-              w[0] = *reinterpret_cast<const u4_any *>(src + at * 2);
-            } else {
-              for (uint32_t k = 0; at + k < a.c.dim; k++) {
-                const uint32_t x = (uint32_t)reinterpret_cast<const uint16_t *>(src)[at + k] << (16 * (k % 2));
-                if (k / 2 == 0) w[0][0] |= x;
-                else if (k / 2 == 1) w[0][1] |= x;
-                else if (k / 2 == 2) w[0][2] |= x;
-                else w[0][3] |= x;
-              }
-            }
-          }
-        }
+        if (q0 + q < q_end) stage8<Q>(a, q0 + q, u0 * 32 + chunk * 8, w);
+        else continue;   // what is in LDS for a query that is not there is multiplied and not used
         const uint32_t u = chunk / 4, h = chunk / 2 % 2, f = chunk % 2;
 #pragma unroll
         for (int p = 0; p < QP; p++) staged[(((u * 2 + f) * QP + p) * QT + q / 32) * 64 + h * 32 + q % 32] = w[p];
@@ -604,7 +964,7 @@ __global__ __launch_bounds__(256) void partition_scores_kernel(PartitionArgs a, 
             }
         }
         if ((u0 + u + 1) % block_units == 0 || u0 + u + 1 == units) {
-          const float s = FMT == NATIVE ? 1.0f : scale[(u0 + u) / block_units];
+          const float s = FMT == NATIVE ? 1.0f : scale[(u0 + u) / block_units] * CODE_UNIT<FMT, Q>;
 #pragma unroll
           for (int i = 0; i < QT; i++)
 #pragma unroll
@@ -758,15 +1118,49 @@ void read_to(const RowCacheArgs &c, const int64_t *slots, uint32_t n, void *out,
   }
 }
 
+// workgroups of a kernel that the device holds at once: kernels that go round give each of them the same share
+uint32_t resident(const void *kernel, uint32_t threads) {
+  int device = 0, units = 0, each = 0;
+  HIP_CHECK(hipGetDevice(&device));
+  HIP_CHECK(hipDeviceGetAttribute(&units, hipDeviceAttributeMultiprocessorCount, device));
+  HIP_CHECK(hipOccupancyMaxActiveBlocksPerMultiprocessor(&each, kernel, (int)threads, 0));
+  return (uint32_t)(units > 0 && each > 0 ? units * each : 256);
+}
+
 template <int FMT, int Q>
 void scores_as(const PartitionArgs &a, hipStream_t s) {
   const FastDiv page(a.page_rows);
-  const bool many = a.n_queries / a.n_partitions >= 48;
-  const uint64_t tq = many ? 128 : 32, asked = a.n_partitions < a.n_queries ? a.n_partitions : a.n_queries;
-  const uint64_t most = (a.n_queries / tq + asked) * ((a.most_rows + ROW_TILE - 1) / ROW_TILE);
-  const dim3 grid((uint32_t)(most < 2048 ? most : 2048));
-  if (many) hipLaunchKernelGGL((partition_scores_kernel<FMT, Q, 4>), grid, dim3(256), 0, s, a, page);
-  else hipLaunchKernelGGL((partition_scores_kernel<FMT, Q, 1>), grid, dim3(256), 0, s, a, page);
+  const uint32_t asked = a.n_partitions < a.n_queries ? a.n_partitions : a.n_queries;   // partitions with queries, at most
+  const uint32_t each = a.n_queries / a.n_partitions;
+  // no more workgroups than there can be tiles, and no more than are resident at once
+  const auto grid = [&](uint32_t tq, uint32_t tr, uint64_t resident) {
+    const uint64_t tiles = ((uint64_t)a.n_queries / tq + asked) * ((a.most_rows + tr - 1) / tr);
+    return dim3((uint32_t)(tiles < resident ? tiles : resident));
+  };
+  if (each >= 48) {
+    hipLaunchKernelGGL((partition_scores_kernel<FMT, Q, 4>), grid(128, ROW_TILE, 2048), dim3(256), 0, s, a, page);
+    return;
+  }
+  // the rows' chunks of a stage: the number that leaves the fewest places empty, the largest of those
+  const uint32_t chunks = a.c.row_bytes / 16;
+  uint32_t cs = 16;
+  constexpr bool widest = FMT == NATIVE && Q == F32;   // whose step is eight chunks
+  for (uint32_t c : {8u, 4u})
+    if (!(widest && c == 4) && (chunks + c - 1) / c * c < (chunks + cs - 1) / cs * cs) cs = c;
+  const auto few = [&](auto w) {
+    constexpr int W = decltype(w)::value, WAVES = Q == F32 ? 16 : 8;
+    const auto launch = [&](auto kernel, uint32_t tr) {
+      hipLaunchKernelGGL(kernel, grid(16, tr, resident(reinterpret_cast<const void *>(kernel), 64 * WAVES)), dim3(64 * WAVES), 0, s, a, page);
+    };
+    if (cs == 16) launch(partition_few_kernel<FMT, Q, W, 1, WAVES>, 16 * WAVES);
+    else if (cs == 8) launch(partition_few_kernel<FMT, Q, W, 2, WAVES>, 32 * WAVES);
+    else if constexpr (!widest) launch(partition_few_kernel<FMT, Q, W, 4, WAVES>, 64 * WAVES);
+  };
+  // a lane's piece of a row: as wide as four of them fit into a block
+  if constexpr (FMT != NATIVE) {
+    if (a.c.block != 32) return few(std::integral_constant<int, 16>());
+  }
+  few(std::integral_constant<int, 8>());
 }
 
 template <int Q>
