@@ -13,6 +13,7 @@ typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 // the caller's rows may begin at any element: gfx950 loads 16 bytes from any address its element type allows
 typedef u4 u4_any __attribute__((aligned(2)));
+typedef u4 u4_any4 __attribute__((aligned(4)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -50,7 +51,7 @@ template <int T>
 __device__ __forceinline__ void load8(const void *row, uint32_t at, uint32_t valid, float (&v)[8]) {
   if (valid >= 8) {
     if constexpr (T == F32) {
-      const u4_any *p = reinterpret_cast<const u4_any *>(static_cast<const float *>(row) + at);
+      const u4_any4 *p = reinterpret_cast<const u4_any4 *>(static_cast<const float *>(row) + at);
       const u4 a = p[0], b = p[1];
 #pragma unroll
       for (int i = 0; i < 4; i++) {
@@ -378,13 +379,9 @@ __device__ __forceinline__ f32x4 mfma16(u4 a, u4 b, f32x4 c) {
 
 // x = hi + mid + lo, each a bf16 in the upper half of its dword.  An infinity or a NaN is hi alone.
 __device__ __forceinline__ void split3(uint32_t x, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
-  hi = x & 0xffff0000u;
-  if ((x & 0x7f800000u) == 0x7f800000u) {
-    if (x & 0xffffu) hi |= 0x400000u;   // a NaN whose payload sits in the bits cut off
-    mid = lo = 0;
-    return;
-  }
-  const float r = __uint_as_float(x) - __uint_as_float(hi);
+  const bool special = (x & 0x7f800000u) == 0x7f800000u;
+  hi = (x & 0xffff0000u) | (special && (x & 0xffffu) ? 0x400000u : 0);   // a NaN whose payload sits in the bits cut off stays one
+  const float r = special ? 0.0f : __uint_as_float(x) - __uint_as_float(hi);
   mid = __float_as_uint(r) & 0xffff0000u;
   lo = __float_as_uint(r - __uint_as_float(mid));
 }
@@ -513,53 +510,68 @@ __device__ __noinline__ float plain_product(const float *row, const float *query
   return p;
 }
 
-// Which partition a tile belongs to is found from the offsets and counts themselves (they are on the device): every workgroup sums the
-// partitions' tiles once, a share of the partitions a thread; before[i] are the tiles before thread i's share.  Returns all tiles.
+// A workgroup's run of tiles, and where its first one is: the partition, that partition's queries and rows, the tile's number in it
+struct Place {
+  uint32_t g, lo, m, n, left;
+};
+struct Run {
+  uint32_t first, last;
+  Place at;
+};
+struct RunShared {
+  uint32_t wave_sums[16];
+  Place at;
+};
+// The offsets and counts are on the device, so every workgroup sums the partitions' tiles itself, a share of the partitions a
+// thread, takes its even part of them, and the thread in whose share that begins says where.
 template <int THREADS>
-__device__ __forceinline__ uint32_t count_tiles(const PartitionArgs &a, uint32_t tq, uint32_t tr, uint32_t per, uint32_t *before, uint32_t *waves) {
-  const uint32_t tid = threadIdx.x, lane = tid % 64;
-  uint32_t sum = 0;
+__device__ __forceinline__ Run find_run(const PartitionArgs &a, uint32_t tq, uint32_t tr, RunShared &shared) {
+  const uint32_t tid = threadIdx.x, lane = tid % 64, per = (a.n_partitions + THREADS - 1) / THREADS;
+  uint32_t own = 0;
   for (uint32_t i = 0; i < per; i++) {
     const uint32_t g = tid * per + i;
     if (g >= a.n_partitions) break;
     uint32_t lo, m, n;
     partition(a, g, lo, m, n);
-    sum += (m + tq - 1) / tq * ((n + tr - 1) / tr);
+    own += (m + tq - 1) / tq * ((n + tr - 1) / tr);
   }
+  uint32_t sum = own;
 #pragma unroll
   for (int k = 1; k < 64; k *= 2) {
     const uint32_t v = __shfl_up(sum, k, 64);
     if (lane >= (uint32_t)k) sum += v;
   }
-  if (lane == 63) waves[tid / 64] = sum;
+  if (lane == 63) shared.wave_sums[tid / 64] = sum;
   __syncthreads();
-  for (uint32_t w = 0; w < tid / 64; w++) sum += waves[w];
-  before[tid + 1] = sum;
-  if (tid == 0) before[0] = 0;
+  uint32_t total = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < THREADS / 64; w++) {
+    const uint32_t v = shared.wave_sums[w];
+    if (w < tid / 64) sum += v;
+    total += v;
+  }
+  Run run;
+  run.first = (uint32_t)((uint64_t)total * blockIdx.x / gridDim.x);
+  run.last = (uint32_t)((uint64_t)total * (blockIdx.x + 1) / gridDim.x);
+  if (run.first == run.last) return run;
+  if (sum - own <= run.first && run.first < sum) {
+    Place p;
+    p.left = run.first - (sum - own);
+    for (p.g = tid * per;; p.g++) {
+      partition(a, p.g, p.lo, p.m, p.n);
+      const uint32_t tiles = (p.m + tq - 1) / tq * ((p.n + tr - 1) / tr);
+      if (p.left < tiles) break;
+      p.left -= tiles;
+    }
+    shared.at = p;
+  }
   __syncthreads();
-  return before[THREADS];
-}
-
-// where tile t is: its partition, that partition's queries and rows, and the tile's number in it
-struct Place {
-  uint32_t g, lo, m, n, left;
-};
-template <int THREADS>
-__device__ __forceinline__ Place find_tile(const PartitionArgs &a, uint32_t tq, uint32_t tr, uint32_t per, const uint32_t *before, uint32_t t) {
-  uint32_t low = 0, high = THREADS;   // before[low] <= t < before[high]
-  while (high - low > 1) {
-    const uint32_t mid = (low + high) / 2;
-    if (before[mid] <= t) low = mid;
-    else high = mid;
-  }
-  Place p;
-  p.left = t - before[low];
-  for (p.g = low * per;; p.g++) {
-    partition(a, p.g, p.lo, p.m, p.n);
-    const uint32_t tiles = (p.m + tq - 1) / tq * ((p.n + tr - 1) / tr);
-    if (p.left < tiles) return p;
-    p.left -= tiles;
-  }
+  run.at.g = __builtin_amdgcn_readfirstlane(shared.at.g);
+  run.at.lo = __builtin_amdgcn_readfirstlane(shared.at.lo);
+  run.at.m = __builtin_amdgcn_readfirstlane(shared.at.m);
+  run.at.n = __builtin_amdgcn_readfirstlane(shared.at.n);
+  run.at.left = __builtin_amdgcn_readfirstlane(shared.at.left);
+  return run;
 }
 
 // eight elements of a query as 16-bit fragments (an fp32 query: three planes)
@@ -620,10 +632,11 @@ struct Piece {
 // Few queries a partition: the rows' bytes are what it takes.  A workgroup has a run of tiles of 16 queries x 16 S rows a wavefront;
 // the queries of a partition are put into LDS once for all its tiles (in parts of KP stages if the rows are longer than that).
 // A wavefront takes its rows in stages of 4 KiB, 16 S rows x 256 / S bytes: four loads of 16 neighbouring bytes a lane, whole lines of
-// the rows, two stages in flight in registers and across tiles.  (Loads in the shape of the matrix instruction's operand touch 16
-// lines each and cost the same whatever they bring: 2.4 TB/s with 8 bytes a lane, 4.6 with 16.)  A stage passes through 4 KiB of LDS
-// that the wavefront has to itself, so nothing but the order of its own instructions guards it, and comes back as operands; the
-// sixteen-byte chunks of a row change places with its number, so that neither side meets a bank twice.
+// the rows, one stage in registers under way (across tiles too) while the one before is multiplied.  (Loads in the shape of the matrix
+// instruction's operand touch 16 lines each and cost the same whatever they bring: 2.4 TB/s with 8 bytes a lane, 4.6 with 16.)  A stage
+// passes through 4 KiB of LDS that the wavefront has to itself, so nothing but the order of its own instructions guards it, and comes
+// back as operands; the sixteen-byte chunks of a row change places with its number, so that neither side meets a bank twice.
+// Every part of the loop is in the code once: a small call is mostly the first pass of its instructions through the caches.
 template <int FMT, int Q, int W, int S, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionArgs a, FastDiv page) {
   typedef Piece<FMT, Q, W> P;
@@ -635,13 +648,13 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
   static_assert(SP >= 1 && KP >= 1, "");
   __shared__ u4 staged[KP * SP * FR * QP * 64];
   __shared__ u4 passing[WAVES][256];
-  __shared__ uint32_t before[64 * WAVES + 1], wave_sums[WAVES];
+  __shared__ RunShared run_shared;
 
   const uint32_t tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), col = lane % 16, quarter = lane / 16;
-  const uint32_t per = (a.n_partitions + 64 * WAVES - 1) / (64 * WAVES);
-  const uint32_t total = count_tiles<64 * WAVES>(a, TQ, TR, per, before, wave_sums);
-  const uint32_t first = (uint32_t)((uint64_t)total * blockIdx.x / gridDim.x), last = (uint32_t)((uint64_t)total * (blockIdx.x + 1) / gridDim.x);
+  const Run run = find_run<64 * WAVES>(a, TQ, TR, run_shared);
+  const uint32_t first = run.first, last = run.last;
   if (first == last) return;
+  Place at = run.at;
   const uint32_t chunks = a.c.row_bytes / 16, stages = (chunks + CS - 1) / CS;
   // blocks are one step or two, or the row
   const uint32_t block_shift = a.c.block >= a.c.dim ? 31 : a.c.block / (4 * W) >= 2 ? 1 : 0;
@@ -650,243 +663,236 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
   struct Tile {
     uint32_t g, query_tile, q0, q_end, n, j0;   // j0: the first row of this wavefront
   };
-  Place start = find_tile<64 * WAVES>(a, TQ, TR, per, before, first);
-  start.g = __builtin_amdgcn_readfirstlane(start.g);
-  start.left = __builtin_amdgcn_readfirstlane(start.left);
-  partition_of_all(a, start.g, start.lo, start.m, start.n);
-  // the loads run ahead of the products, each with a place of their own
-  Place load_at = start, use_at = start;
-  const auto take = [&](Place &at) {
-    uint32_t row_tiles = (at.n + TR - 1) / TR;
-    while (at.left >= (at.m + TQ - 1) / TQ * row_tiles) {   // behind this partition's last tile
-      at.g++;
-      at.left = 0;
-      partition_of_all(a, at.g, at.lo, at.m, at.n);
-      row_tiles = (at.n + TR - 1) / TR;
-    }
-    const uint32_t query_tile = at.left / row_tiles;
-    const Tile t = {at.g, query_tile, at.lo + query_tile * TQ, at.lo + at.m, at.n, (at.left - query_tile * row_tiles) * TR + wave * WR};
-    at.left++;
-    return t;
-  };
-  // page of row j (of a row behind the partition's last: of its first, whose scores are not written)
-  const auto page_of = [&](const Tile &t, uint32_t j) { return a.pages[(size_t)t.g * a.max_pages + (j < t.n ? page.div(j) : 0)]; };
-  // slot of row j in it; one that is not there is read from slot 0 and not used
+  // slot of row j in page `id`; one that is not there is read from slot 0 and not used
   const auto slot_of = [&](uint32_t j, int32_t id, bool &there) {
     const uint64_t slot = (uint64_t)(uint32_t)id * page.d + (j - page.div(j) * page.d);
     there = id >= 0 && slot < a.c.capacity;
     return there ? slot : 0;
   };
-  // chunk i of a lane: row i * 64 / CS + lane / CS of the wavefront, its chunk number changed by the row's
-  const uint32_t my_row = lane / CS, turn = CS == 4 ? (lane / CS >> 1) & 3 : (lane / CS) & (CS - 1);
-  constexpr uint32_t ROWS_A_LOAD = 64 / CS;
 
-  // ---- loads: the tile they are at, the pages of the next one
-  struct Next {
-    int32_t id[4], scale_id[S];
-  } ids;
-  const auto look_up = [&](const Tile &t) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) ids.id[i] = page_of(t, t.j0 + i * ROWS_A_LOAD + my_row);
-    if (FMT != NATIVE) {
-#pragma unroll
-      for (int k = 0; k < S; k++) ids.scale_id[k] = page_of(t, t.j0 + k * 16 + col);
-    }
-  };
+  // Three tiles: `now` is multiplied, `held` is in registers or LDS (its rows in `source`), the pages of `coming` are looked up.
+  // Chunk i of a lane is of row i * 64 / CS + lane / CS of the wavefront.
+  constexpr uint32_t ROWS_A_LOAD = 64 / CS;
+  const uint32_t my_row = lane / CS;
+  Tile now = {}, held = {}, coming = {};
+  uint32_t there = 0, held_there = 0;             // which of the rows 16 k + col are there
+  int32_t id[4], col_id[S];
   const uint8_t *source[4];
   const float *scale_source[S];
-  const auto rows_of = [&](const Tile &t) {
-    bool there;
+  u4 chunk[4];
+  float next_scale[S][QS ? QS : 1], scale[S][QS ? QS : 1];
+  u4 *const mine = passing[wave];
+  f32x4 acc[S];
 #pragma unroll
-    for (int i = 0; i < 4; i++) source[i] = a.c.codes + slot_of(t.j0 + i * ROWS_A_LOAD + my_row, ids.id[i], there) * a.c.row_bytes;
-    if (FMT != NATIVE) {
+  for (int k = 0; k < S; k++) acc[k] = f32x4{0, 0, 0, 0};
+  uint32_t staged_g = ~0u, staged_q = 0, staged_p = 0;   // whose queries are in LDS, from which stage on
+  uint32_t taken = first;
+  uint32_t use_stage = 0, load_stage = stages;           // stages: on to the next tile before the next load
+  const int64_t rounds = (int64_t)(last - first) * stages;
+
+  for (int64_t round = -2; round < rounds; round++) {
+    if (load_stage == stages) {
+      // the tile whose pages are known is loaded from now on (behind the run's last tile: that one again)
+      load_stage = 0;
+      held = coming;
+      held_there = 0;
 #pragma unroll
-      for (int k = 0; k < S; k++) scale_source[k] = a.c.scales + slot_of(t.j0 + k * 16 + col, ids.scale_id[k], there) * a.c.nb;
+      for (int i = 0; i < 4; i++) {
+        bool is;
+        const uint64_t slot = slot_of(held.j0 + i * ROWS_A_LOAD + my_row, round == -2 ? -1 : id[i], is);
+        source[i] = a.c.codes + slot * a.c.row_bytes;
+      }
+#pragma unroll
+      for (int k = 0; k < S; k++) {
+        bool is;
+        const uint64_t slot = slot_of(held.j0 + k * 16 + col, round == -2 ? -1 : col_id[k], is);
+        held_there |= is ? 1u << k : 0;
+        scale_source[k] = a.c.scales + slot * a.c.nb;
+      }
+      if (taken < last) {
+        uint32_t row_tiles = (at.n + TR - 1) / TR;
+        while (at.left >= (at.m + TQ - 1) / TQ * row_tiles) {   // behind this partition's last tile
+          at.g++;
+          at.left = 0;
+          partition_of_all(a, at.g, at.lo, at.m, at.n);
+          row_tiles = (at.n + TR - 1) / TR;
+        }
+        const uint32_t query_tile = at.left / row_tiles;
+        coming = Tile{at.g, query_tile, at.lo + query_tile * TQ, at.lo + at.m, at.n, (at.left - query_tile * row_tiles) * TR + wave * WR};
+        at.left++;
+        taken++;
+      }
+      // page of row j (of a row behind the partition's last: of its first, whose scores are not written)
+      const int32_t *pages = a.pages + (size_t)coming.g * a.max_pages;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const uint32_t j = coming.j0 + i * ROWS_A_LOAD + my_row;
+        id[i] = pages[j < coming.n ? page.div(j) : 0];
+      }
+#pragma unroll
+      for (int k = 0; k < S; k++) {
+        const uint32_t j = coming.j0 + k * 16 + col;
+        col_id[k] = pages[j < coming.n ? page.div(j) : 0];
+      }
+      if (round == -2) {
+        load_stage = stages;
+        continue;
+      }
     }
-  };
-  u4 held[2][4];
-  float held_scales[2][S][QS ? QS : 1];
-  uint32_t load_stage = 0, load_tile = first;
-  Tile loading = take(load_at), coming = loading;
-  const auto load_next = [&](u4 (&h)[4], float (&sc)[S][QS ? QS : 1]) {
+
+    // a stage under way
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const uint32_t c = load_stage * CS + ((lane % CS) ^ ((CS == 4 ? turn : (i * ROWS_A_LOAD + my_row) & (CS - 1))));
-      h[i] = *reinterpret_cast<const u4 *>(source[i] + (c < chunks ? c : chunks - 1) * 16);
+      const uint32_t row = i * ROWS_A_LOAD + my_row, c = load_stage * CS + (lane % CS ^ (CS == 4 ? row >> 1 & 3 : row & (CS - 1)));
+      chunk[i] = *reinterpret_cast<const u4 *>(source[i] + (c < chunks ? c : chunks - 1) * 16);
     }
 #pragma unroll
     for (int k = 0; k < S; k++)
 #pragma unroll
       for (int q = 0; q < QS; q++) {
         const uint32_t b = ((load_stage * SP) >> block_shift) + q * 4 + quarter;
-        sc[k][q] = scale_source[k][b < a.c.nb ? b : a.c.nb - 1];
+        next_scale[k][q] = scale_source[k][b < a.c.nb ? b : a.c.nb - 1];
       }
-    if (++load_stage == stages) {   // on to the next tile, the last one's again behind the run's end
-      load_stage = 0;
-      if (load_tile + 1 < last) load_tile++;
-      loading = coming;
-      rows_of(loading);
-      if (load_tile + 1 < last) coming = take(load_at);
-      look_up(coming);
-    }
-  };
+    load_stage++;
 
-  // stages p0 .. p0 + np - 1 of a tile's queries into LDS
-  const auto stage = [&](const Tile &t, uint32_t p0, uint32_t np) {
-    const uint32_t asked = t.q_end - t.q0 < TQ ? t.q_end - t.q0 : TQ;   // what is in LDS behind them is multiplied and not used
-    const uint32_t shift = asked > 8 ? 4 : asked > 4 ? 3 : asked > 2 ? 2 : asked > 1 ? 1 : 0;
-    for (uint32_t i = tid; i < np * (SP * FR * 4) << shift; i += 64 * WAVES) {
-      const uint32_t q = i & ((1u << shift) - 1), chunk = i >> shift, f = chunk % FR, h = chunk / FR % 4, st = chunk / (4 * FR);
-      if (q >= asked) continue;
-      u4 w[QP];
-      stage8<Q>(a, t.q0 + q, (p0 * SP + st) * (4 * W) + h * W + f * 8, w);
+    if (round >= 0) {
+      // the one in LDS multiplied
+      const u4 *queries = staged + use_stage % KP * (SP * FR * QP * 64) + lane;
+      const uint32_t first_block = (use_stage * SP) >> block_shift;
+      P piece[SP][S];
 #pragma unroll
-      for (int p = 0; p < QP; p++) staged[((st * FR + f) * QP + p) * 64 + h * 16 + q] = w[p];
-    }
-    __syncthreads();
-  };
-
-  look_up(loading);
-  Tile now = take(use_at);
-  stage(now, 0, stages < KP ? stages : KP);
-  uint32_t held_g = now.g, held_q = now.query_tile, held_p = 0;   // whose queries are in LDS, from which stage on
-  rows_of(loading);
-  if (load_tile + 1 < last) coming = take(load_at);
-  look_up(coming);
-  load_next(held[0], held_scales[0]);
-  load_next(held[1], held_scales[1]);
-
-  uint32_t use_stage = 0, use_tile = first;
-  f32x4 acc[S], part[S];
+      for (int st = 0; st < SP; st++)
 #pragma unroll
-  for (int k = 0; k < S; k++) acc[k] = part[k] = f32x4{0, 0, 0, 0};
-  u4 *const mine = passing[wave];
+        for (int k = 0; k < S; k++) {
+          const uint32_t row = k * 16 + col, bytes = st * 4 * P::BYTES + quarter * P::BYTES, turn = CS == 4 ? row >> 1 & 3 : row & (CS - 1);
+#pragma unroll
+          for (int e = 0; e < (P::BYTES + 15) / 16; e++) {
+            const uint8_t *p = reinterpret_cast<const uint8_t *>(mine + row * CS + ((bytes / 16 + e) ^ turn)) + bytes % 16;
+            if constexpr (P::BYTES == 4) {
+              piece[st][k].raw[0] = *reinterpret_cast<const uint32_t *>(p);
+            } else if constexpr (P::BYTES == 8) {
+              const u2 w = *reinterpret_cast<const u2 *>(p);
+              piece[st][k].raw[0] = w[0];
+              piece[st][k].raw[1] = w[1];
+            } else {
+              const u4 w = *reinterpret_cast<const u4 *>(p);
+#pragma unroll
+              for (int i = 0; i < 4; i++) piece[st][k].raw[4 * e + i] = w[i];
+            }
+          }
+        }
+#pragma unroll
+      for (int st = 0; st < SP; st++) {
+        f32x4 part[S];
+#pragma unroll
+        for (int k = 0; k < S; k++) part[k] = FMT == NATIVE ? acc[k] : f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int f = 0; f < FR; f++) {
+          u4 q[QP];
+#pragma unroll
+          for (int p = 0; p < QP; p++) q[p] = queries[((st * FR + f) * QP + p) * 64];
+#pragma unroll
+          for (int k = 0; k < S; k++) {
+            u4 b[P::PLANES];
+            piece[st][k].fragment(f, b);
+            if (FMT == NATIVE) {   // behind the row's end its last chunk comes again: an infinity there would meet a zero
+              const bool in = (use_stage * SP + st) * 4 * W + quarter * W < a.c.row_bytes / elem_size<Q>;
+#pragma unroll
+              for (int c = 0; c < P::PLANES; c++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) b[c][e] = in ? b[c][e] : 0;
+            }
+#pragma unroll
+            for (int p = QP - 1; p >= 0; p--)   // the smallest first
+#pragma unroll
+              for (int c = P::PLANES - 1; c >= 0; c--)
+                if (p + c < 3) part[k] = mfma16<Q>(q[p], b[c], part[k]);   // the planes left out are below 2^-24 of the product
+          }
+        }
+        // a step's sum, times the scale of the block that it is in (no branch for the block's end: the steps overlap)
+        const uint32_t block = ((use_stage * SP + st) >> block_shift) - first_block;
+#pragma unroll
+        for (int k = 0; k < S; k++) {
+          if (FMT == NATIVE) {
+            acc[k] = part[k];
+          } else {
+            float v = scale[k][0];
+#pragma unroll
+            for (int q = 1; q < QS; q++) v = block / 4 == (uint32_t)q ? scale[k][q] : v;
+            v = __uint_as_float(__builtin_amdgcn_ds_bpermute((block % 4 * 16 + col) * 4, __float_as_uint(v)));
+#pragma unroll
+            for (int r = 0; r < 4; r++) acc[k][r] = __builtin_fmaf(v, part[k][r], acc[k][r]);
+          }
+        }
+      }
+      use_stage++;
+    }
 
-  const auto use = [&](u4 (&h)[4], float (&sc)[S][QS ? QS : 1]) {
-    const uint32_t p0 = use_stage / KP * KP;
-    if (held_p != p0 || held_g != now.g || held_q != now.query_tile) {
+    // the queries that the next stage meets, if they are not in LDS yet; they and the stage under way come together
+    const bool turned = round < 0 || use_stage == stages;
+    const uint32_t meets_g = turned ? held.g : now.g, meets_q = turned ? held.query_tile : now.query_tile, p0 = turned ? 0 : use_stage / KP * KP;
+    if ((staged_g != meets_g || staged_q != meets_q || staged_p != p0) && round + 1 < rounds) {
+      const uint32_t q0 = turned ? held.q0 : now.q0, q_end = turned ? held.q_end : now.q_end;
       __syncthreads();
-      stage(now, p0, stages - p0 < KP ? stages - p0 : KP);
-      held_g = now.g;
-      held_q = now.query_tile;
-      held_p = p0;
-    }
+      const uint32_t np = stages - p0 < KP ? stages - p0 : KP, asked = q_end - q0 < TQ ? q_end - q0 : TQ;
+      const uint32_t shift = asked > 8 ? 4 : asked > 4 ? 3 : asked > 2 ? 2 : asked > 1 ? 1 : 0;
+      for (uint32_t i = tid; i < np * (SP * FR * 4) << shift; i += 64 * WAVES) {
+        const uint32_t q = i & ((1u << shift) - 1), e = i >> shift, f = e % FR, h = e / FR % 4, st = e / (4 * FR);
+        if (q >= asked) continue;   // what is in LDS behind them is multiplied and not used
+        u4 w[QP];
+        stage8<Q>(a, q0 + q, (p0 * SP + st) * (4 * W) + h * W + f * 8, w);
 #pragma unroll
-    for (int i = 0; i < 4; i++) mine[i * 64 + lane] = h[i];
-    float scale[S][QS ? QS : 1];
+        for (int p = 0; p < QP; p++) staged[((st * FR + f) * QP + p) * 64 + h * 16 + q] = w[p];
+      }
+      __syncthreads();
+      staged_g = meets_g;
+      staged_q = meets_q;
+      staged_p = p0;
+    }
+
+    // the stage under way into LDS, behind the reads of the one before it
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < 4; i++) mine[i * 64 + lane] = chunk[i];
 #pragma unroll
     for (int k = 0; k < S; k++)
 #pragma unroll
-      for (int q = 0; q < QS; q++) scale[k][q] = sc[k][q];
-    load_next(h, sc);
+      for (int q = 0; q < QS; q++) scale[k][q] = next_scale[k][q];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    const u4 *queries = staged + (use_stage - p0) * (SP * FR * QP * 64) + lane;
-    const bool last_stage = use_stage + 1 == stages;
-    const uint32_t first_block = (use_stage * SP) >> block_shift;
-#pragma unroll
-    for (int st = 0; st < SP; st++) {
-      P piece[S];
+
+    if (use_stage == stages) {
 #pragma unroll
       for (int k = 0; k < S; k++) {
-        const uint32_t row = k * 16 + col, at = st * 4 * P::BYTES + quarter * P::BYTES;
-        const uint32_t t = CS == 4 ? (row >> 1) & 3 : row & (CS - 1);
+        const uint32_t j = now.j0 + k * 16 + col;
+        if (j < now.n) {
 #pragma unroll
-        for (int e = 0; e < (P::BYTES + 15) / 16; e++) {
-          const uint8_t *p = reinterpret_cast<const uint8_t *>(mine + row * CS + ((at / 16 + e) ^ t)) + at % 16;
-          if constexpr (P::BYTES == 4) {
-            piece[k].raw[0] = *reinterpret_cast<const uint32_t *>(p);
-          } else if constexpr (P::BYTES == 8) {
-            const u2 w = *reinterpret_cast<const u2 *>(p);
-            piece[k].raw[0] = w[0];
-            piece[k].raw[1] = w[1];
-          } else {
-            const u4 w = *reinterpret_cast<const u4 *>(p);
-#pragma unroll
-            for (int i = 0; i < 4; i++) piece[k].raw[4 * e + i] = w[i];
-          }
-        }
-      }
-#pragma unroll
-      for (int f = 0; f < FR; f++) {
-        u4 q[QP];
-#pragma unroll
-        for (int p = 0; p < QP; p++) q[p] = queries[((st * FR + f) * QP + p) * 64];
-#pragma unroll
-        for (int k = 0; k < S; k++) {
-          u4 b[P::PLANES];
-          piece[k].fragment(f, b);
-          if (FMT == NATIVE) {   // behind the row's end its last chunk comes again: an infinity there would meet a zero
-            const bool in = (use_stage * SP + st) * 4 * W + quarter * W < a.c.row_bytes / elem_size<Q>;
-#pragma unroll
-            for (int c = 0; c < P::PLANES; c++)
-#pragma unroll
-              for (int e = 0; e < 4; e++) b[c][e] = in ? b[c][e] : 0;
-          }
-#pragma unroll
-          for (int p = 0; p < QP; p++)
-#pragma unroll
-            for (int c = 0; c < P::PLANES; c++)
-              if (p + c < 3) part[k] = mfma16<Q>(q[p], b[c], part[k]);   // the planes left out are below 2^-24 of the product
-        }
-      }
-      if (FMT != NATIVE) {
-        const uint32_t step = use_stage * SP + st;
-        if (((step + 1) & ((1u << block_shift) - 1)) == 0 || (last_stage && st == SP - 1)) {
-          const uint32_t b = (step >> block_shift) - first_block;
-#pragma unroll
-          for (int k = 0; k < S; k++) {
-            float v = scale[k][0];
-#pragma unroll
-            for (int q = 1; q < QS; q++) v = b / 4 == (uint32_t)q ? scale[k][q] : v;
-            v = __uint_as_float(__builtin_amdgcn_ds_bpermute((b % 4 * 16 + col) * 4, __float_as_uint(v)));
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-              acc[k][r] = __builtin_fmaf(v, part[k][r], acc[k][r]);
-              part[k][r] = 0.0f;
+          for (int r = 0; r < 4; r++) {
+            const uint32_t q = now.q0 + quarter * 4 + r;
+            if (q < now.q_end) {
+              float p = acc[k][r] * CODE_UNIT<FMT, Q>;
+              if constexpr (FMT == NATIVE && Q == F32) {
+                // an infinity meets the other side's planes, some of them 0: the sum is taken again, element by element
+                if (p != p && (there >> k & 1)) {
+                  bool is;
+                  const uint64_t slot = slot_of(j, a.pages[(size_t)now.g * a.max_pages + page.div(j)], is);
+                  p = plain_product(reinterpret_cast<const float *>(a.c.codes + slot * a.c.row_bytes), static_cast<const float *>(a.queries) + q * a.stride, a.c.dim);
+                }
+              }
+              if (a.form == RSGPU_SCORES_DISTANCE) p = 1.0f - p;
+              a.scores[(size_t)q * a.ld + j] = there >> k & 1 ? p : gone;
             }
           }
         }
+        acc[k] = f32x4{0, 0, 0, 0};
       }
+      use_stage = 0;
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    if (!last_stage) {
-      use_stage++;
-      return;
+    if (use_stage == 0) {
+      now = held;
+      there = held_there;
     }
-
-#pragma unroll
-    for (int k = 0; k < S; k++) {
-      const uint32_t j = now.j0 + k * 16 + col;
-      if (j < now.n && quarter * 4 < now.q_end - now.q0) {
-        bool there;
-        const uint64_t slot = slot_of(j, page_of(now, j), there);
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const uint32_t q = now.q0 + quarter * 4 + r;
-          if (q < now.q_end) {
-            float p = FMT == NATIVE ? part[k][r] : acc[k][r] * CODE_UNIT<FMT, Q>;
-            if constexpr (FMT == NATIVE && Q == F32) {
-              // an infinity meets the other side's planes, some of them 0: the sum is taken again, element by element
-              if (p != p && there)
-                p = plain_product(reinterpret_cast<const float *>(a.c.codes + slot * a.c.row_bytes), static_cast<const float *>(a.queries) + q * a.stride, a.c.dim);
-            }
-            if (a.form == RSGPU_SCORES_DISTANCE) p = 1.0f - p;
-            a.scores[(size_t)q * a.ld + j] = there ? p : gone;
-          }
-        }
-      }
-      acc[k] = part[k] = f32x4{0, 0, 0, 0};
-    }
-    use_stage = 0;
-    if (++use_tile < last) now = take(use_at);
-  };
-  for (;;) {
-    use(held[0], held_scales[0]);
-    if (use_tile == last) break;
-    use(held[1], held_scales[1]);
-    if (use_tile == last) break;
   }
 }
 
@@ -897,19 +903,24 @@ __global__ __launch_bounds__(256) void partition_scores_kernel(PartitionArgs a, 
   constexpr int KU = (QT == 1 ? 48 : 64) * 1024 / (2048 * QP * QT);   // units of 32 elements staged at a time: 48 / 64 KiB
   typedef Unit<FMT, Q> U;
   __shared__ u4 staged[KU * 2 * QP * QT * 64];
-  __shared__ uint32_t before[257], wave_sums[4];
+  __shared__ RunShared run_shared;
 
   const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
-  const uint32_t per = (a.n_partitions + 255) / 256;
-  const uint32_t total = count_tiles<256>(a, TQ, ROW_TILE, per, before, wave_sums);
+  const Run run = find_run<256>(a, TQ, ROW_TILE, run_shared);
+  Place at = run.at;
   const uint32_t units = (a.c.dim + 31) / 32;
   const uint32_t block_units = FMT == NATIVE || a.c.block >= a.c.dim ? units : a.c.block / 32;
   const float gone = a.form == RSGPU_SCORES_DISTANCE ? __builtin_inff() : -__builtin_inff();
 
-  for (uint32_t t = blockIdx.x; t < total; t += gridDim.x) {
-    const Place at = find_tile<256>(a, TQ, ROW_TILE, per, before, t);
+  for (uint32_t t = run.first; t < run.last; t++) {
+    while (at.left >= (at.m + TQ - 1) / TQ * ((at.n + ROW_TILE - 1) / ROW_TILE)) {   // behind this partition's last tile
+      at.g++;
+      at.left = 0;
+      partition_of_all(a, at.g, at.lo, at.m, at.n);
+    }
     const uint32_t g = at.g, n = at.n, qt = (at.m + TQ - 1) / TQ;
     const uint32_t row_tile = at.left / qt, q0 = at.lo + (at.left - row_tile * qt) * TQ, q_end = at.lo + at.m;
+    at.left++;
     const uint32_t j = row_tile * ROW_TILE + wave * 32 + lane % 32, half = lane / 32;
 
     // the row of this lane; one that is not there is read from slot 0 and not used
@@ -1144,7 +1155,7 @@ void scores_as(const PartitionArgs &a, hipStream_t s) {
   // the rows' chunks of a stage: the number that leaves the fewest places empty, the largest of those
   const uint32_t chunks = a.c.row_bytes / 16;
   uint32_t cs = 16;
-  constexpr bool widest = FMT == NATIVE && Q == F32;   // whose step is eight chunks
+  constexpr bool widest = Q == F32;   // an fp32 step is eight chunks, and 64 rows of three planes do not fit into 128 registers
   for (uint32_t c : {8u, 4u})
     if (!(widest && c == 4) && (chunks + c - 1) / c * c < (chunks + cs - 1) / cs * cs) cs = c;
   const auto few = [&](auto w) {
