@@ -454,46 +454,6 @@ __device__ __forceinline__ u4 widen8(uint32_t w0, uint32_t w1) {
   return r;
 }
 
-constexpr int ROW_TILE = 128;   // rows of a workgroup: 32 for each of its four wavefronts
-
-// what a lane holds of one row and one unit of 32 elements: the 16 elements of its half, as two fragments (in up to three planes)
-template <int FMT, int Q>
-struct Unit {
-  static constexpr int BYTES = FMT == NATIVE ? 32 * elem_size<Q> : FMT == INT4 ? 16 : 32;
-  static constexpr int PLANES = FMT == NATIVE && Q == F32 ? 3 : 1;
-  uint32_t raw[BYTES / 8];
-
-  __device__ __forceinline__ void load(const uint8_t *row, uint32_t unit, uint32_t half) {
-    const uint8_t *p = row + unit * BYTES + half * (BYTES / 2);
-    if constexpr (BYTES == 16) {
-      const u2 w = *reinterpret_cast<const u2 *>(p);
-      raw[0] = w[0];
-      raw[1] = w[1];
-    } else {
-#pragma unroll
-      for (int i = 0; i < BYTES / 32; i++) {
-        const u4 w = reinterpret_cast<const u4 *>(p)[i];
-#pragma unroll
-        for (int k = 0; k < 4; k++) raw[4 * i + k] = w[k];
-      }
-    }
-  }
-  __device__ __forceinline__ void fragment(int f, u4 (&out)[PLANES]) const {
-    if constexpr (FMT == NATIVE && Q == F32) {
-      float v[8];
-#pragma unroll
-      for (int i = 0; i < 8; i++) v[i] = __uint_as_float(raw[8 * f + i]);
-      planes8(v, out);
-    } else if constexpr (FMT == NATIVE) {
-      out[0] = u4{raw[4 * f], raw[4 * f + 1], raw[4 * f + 2], raw[4 * f + 3]};
-    } else if constexpr (FMT == INT4) {
-      out[0] = widen8<INT4, Q>(raw[f], 0);
-    } else {
-      out[0] = widen8<FMT, Q>(raw[2 * f], raw[2 * f + 1]);
-    }
-  }
-};
-
 __device__ __forceinline__ int32_t cut(int32_t x, int32_t most) { return x < 0 ? 0 : x > most ? most : x; }
 
 // queries [lo, lo + m) and rows of partition g
@@ -896,113 +856,267 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
   }
 }
 
-template <int FMT, int Q, int QT>
-__global__ __launch_bounds__(256) void partition_scores_kernel(PartitionArgs a, FastDiv page) {
-  constexpr int TQ = 32 * QT;
-  constexpr int QP = Q == F32 ? 3 : 1;                          // planes of a query
-  constexpr int KU = (QT == 1 ? 48 : 64) * 1024 / (2048 * QP * QT);   // units of 32 elements staged at a time: 48 / 64 KiB
-  typedef Unit<FMT, Q> U;
-  __shared__ u4 staged[KU * 2 * QP * QT * 64];
+// Many queries a partition: the matrix cores' work.  A workgroup has a run of tiles of 128 queries x 128 rows, a wavefront 64 x 64 of
+// each; both sides go through LDS in stages of KC elements as operands of the 32 x 32 x 16 product, the rows' codes widened once on
+// the way there.  One stage is multiplied while the next one, of this tile or the next, is on its way in registers.  In LDS an
+// operand's 32 rows change places with the number of its eight elements, so that neither side meets a bank twice.  A block's
+// products are summed by themselves and multiplied by the row's scale at every FLUSH elements.
+template <int FMT, int Q, int FLUSH>
+__global__ __launch_bounds__(256, FMT == NATIVE && Q == F32 ? 1 : 2) void partition_many_kernel(PartitionArgs a, FastDiv page) {
+  constexpr int T = 128, KC = Q == F32 ? 32 : 64, QP = Q == F32 ? 3 : 1, RP = FMT == NATIVE && Q == F32 ? 3 : 1;
+  constexpr int C8 = KC / 8;                                                 // eights of a stage
+  constexpr int PIECE = FMT == NATIVE ? 8 : FMT == INT4 ? 32 : 16;           // elements of a row that a thread loads together
+  constexpr int PIECE_BYTES = FMT == NATIVE ? 8 * elem_size<Q> : 16, PU = PIECE_BYTES / 16;
+  constexpr int NP = KC / PIECE, RT = (T * NP + 255) / 256;                  // pieces of a row in a stage, of a thread
+  constexpr int QU = Q == F32 ? 2 : 1, QN = T * C8 / 256;                    // 16 bytes of eight elements of a query, eights of a thread
+  static_assert(FLUSH == 32 || FLUSH == KC, "");
+  typedef Piece<FMT, Q, PIECE> P;
+  __shared__ u4 q_lds[2][KC / 16 * QP * 4 * 64], r_lds[2][KC / 16 * RP * 4 * 64];
+  __shared__ float s_lds[2][2][T];
   __shared__ RunShared run_shared;
 
-  const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
-  const Run run = find_run<256>(a, TQ, ROW_TILE, run_shared);
+  const uint32_t tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), col = lane % 32, half = lane / 32;
+  const Run run = find_run<256>(a, T, T, run_shared);
+  const uint32_t first = run.first, last = run.last;
+  if (first == last) return;
   Place at = run.at;
-  const uint32_t units = (a.c.dim + 31) / 32;
-  const uint32_t block_units = FMT == NATIVE || a.c.block >= a.c.dim ? units : a.c.block / 32;
+  const uint32_t padded = rows_padded(a.c.dim), stages = (padded + KC - 1) / KC;
+  const bool even = a.c.dim % 8 == 0;   // no eight of a query is cut by its end
   const float gone = a.form == RSGPU_SCORES_DISTANCE ? __builtin_inff() : -__builtin_inff();
+  const auto slot_of = [&](uint32_t j, int32_t id, bool &there) {
+    const uint64_t slot = (uint64_t)(uint32_t)id * page.d + (j - page.div(j) * page.d);
+    there = id >= 0 && slot < a.c.capacity;
+    return there ? slot : 0;   // one that is not there is read from slot 0 and not used
+  };
+  // the place of eight elements (number c of the stage) of row r in an operand of plane p
+  const auto place = [](uint32_t c, uint32_t planes, uint32_t p, uint32_t r) {
+    return ((c / 2 * planes + p) * 4 + r / 32) * 64 + c % 2 * 32 + (r % 32 ^ c * (8 / C8));
+  };
 
-  for (uint32_t t = run.first; t < run.last; t++) {
-    while (at.left >= (at.m + TQ - 1) / TQ * ((at.n + ROW_TILE - 1) / ROW_TILE)) {   // behind this partition's last tile
-      at.g++;
-      at.left = 0;
-      partition_of_all(a, at.g, at.lo, at.m, at.n);
-    }
-    const uint32_t g = at.g, n = at.n, qt = (at.m + TQ - 1) / TQ;
-    const uint32_t row_tile = at.left / qt, q0 = at.lo + (at.left - row_tile * qt) * TQ, q_end = at.lo + at.m;
-    at.left++;
-    const uint32_t j = row_tile * ROW_TILE + wave * 32 + lane % 32, half = lane / 32;
+  struct Tile {
+    uint32_t g, q0, q_end, n, j0;
+  };
+  Tile now = {}, held = {}, coming = {};
+  uint32_t there = 0, held_there = 0;
+  // thread: piece i is of row (i * 256 + tid) / NP, eight i of query (i * 256 + tid) / C8; its scale is row tid % 128's
+  int32_t id[RT], col_id[2], scale_id;
+  const uint8_t *source[RT], *queries[QN];
+  const float *scale_source;
+  u4 row_held[RT][PU], query_held[QN][QU];
+  float scale_held;
+  uint32_t taken = first, load_stage = stages, use_stage = 0;
+  const int64_t rounds = (int64_t)(last - first) * stages;
+  const uint32_t wave_q = wave / 2 * 64, wave_r = wave % 2 * 64;
+  f32x16 acc[2][2];
+#pragma unroll
+  for (int x = 0; x < 2; x++)
+#pragma unroll
+    for (int y = 0; y < 2; y++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[x][y][r] = 0.0f;
 
-    // the row of this lane; one that is not there is read from slot 0 and not used
-    const uint8_t *row = a.c.codes;
-    const float *scale = a.c.scales;
-    bool there = false;
-    if (j < n) {
-      const uint32_t p = page.div(j);
-      const int32_t id = a.pages[(size_t)g * a.max_pages + p];
-      const uint64_t slot = (uint64_t)(uint32_t)id * page.d + (j - p * page.d);
-      if (id >= 0 && slot < a.c.capacity) {
-        there = true;
-        row += slot * a.c.row_bytes;
-        scale += slot * a.c.nb;
+  for (int64_t round = -2; round < rounds; round++) {
+    if (load_stage == stages) {
+      // the tile whose pages are known is loaded from now on (behind the run's last tile: that one again)
+      load_stage = 0;
+      held = coming;
+      held_there = 0;
+      bool is;
+#pragma unroll
+      for (int i = 0; i < RT; i++) source[i] = a.c.codes + slot_of(held.j0 + (i * 256 + tid) / NP % T, round == -2 ? -1 : id[i], is) * a.c.row_bytes;
+#pragma unroll
+      for (int y = 0; y < 2; y++) {
+        slot_of(held.j0 + wave_r + y * 32 + col, round == -2 ? -1 : col_id[y], is);
+        held_there |= is ? 1u << y : 0;
       }
-    }
-
-    f32x16 acc[QT], part[QT];
+      if (FMT != NATIVE) scale_source = a.c.scales + slot_of(held.j0 + tid % T, round == -2 ? -1 : scale_id, is) * a.c.nb;
 #pragma unroll
-    for (int i = 0; i < QT; i++)
-#pragma unroll
-      for (int r = 0; r < 16; r++) acc[i][r] = part[i][r] = 0.0f;
-
-    for (uint32_t u0 = 0; u0 < units; u0 += KU) {
-      const uint32_t nu = units - u0 < KU ? units - u0 : KU;
-      __syncthreads();
-      for (uint32_t i = tid; i < nu * 4 * TQ; i += 256) {
-        const uint32_t q = i % TQ, chunk = i / TQ;   // chunk: unit, half, fragment
-        u4 w[QP];
-        if (q0 + q < q_end) stage8<Q>(a, q0 + q, u0 * 32 + chunk * 8, w);
-        else continue;   // what is in LDS for a query that is not there is multiplied and not used
-        const uint32_t u = chunk / 4, h = chunk / 2 % 2, f = chunk % 2;
-#pragma unroll
-        for (int p = 0; p < QP; p++) staged[(((u * 2 + f) * QP + p) * QT + q / 32) * 64 + h * 32 + q % 32] = w[p];
+      for (int i = 0; i < QN; i++) {
+        const uint32_t q = held.q0 + (i * 256 + tid) / C8;   // of a query behind the partition's last: the last's, not used
+        queries[i] = static_cast<const uint8_t *>(a.queries) + (size_t)(q < held.q_end ? q : held.q_end ? held.q_end - 1 : 0) * a.stride * elem_size<Q>;
       }
-      __syncthreads();
-      for (uint32_t u = 0; u < nu; u++) {
-        U x;
-        x.load(row, u0 + u, half);
-#pragma unroll
-        for (int f = 0; f < 2; f++) {
-          u4 b[U::PLANES];
-          x.fragment(f, b);
-#pragma unroll
-          for (int i = 0; i < QT; i++)
-#pragma unroll
-            for (int p = 0; p < QP; p++) {
-              const u4 q = staged[(((u * 2 + f) * QP + p) * QT + i) * 64 + lane];
-#pragma unroll
-              for (int k = 0; k < U::PLANES; k++)
-                if (p + k < 3) part[i] = mfma<Q>(q, b[k], part[i]);   // the planes left out are below 2^-24 of the product
-            }
+      if (taken < last) {
+        uint32_t query_tiles = (at.m + T - 1) / T;
+        while (at.left >= query_tiles * ((at.n + T - 1) / T)) {   // behind this partition's last tile
+          at.g++;
+          at.left = 0;
+          partition_of_all(a, at.g, at.lo, at.m, at.n);
+          query_tiles = (at.m + T - 1) / T;
         }
-        if ((u0 + u + 1) % block_units == 0 || u0 + u + 1 == units) {
-          const float s = FMT == NATIVE ? 1.0f : scale[(u0 + u) / block_units] * CODE_UNIT<FMT, Q>;
+        const uint32_t row_tile = at.left / query_tiles;
+        coming = Tile{at.g, at.lo + (at.left - row_tile * query_tiles) * T, at.lo + at.m, at.n, row_tile * T};
+        at.left++;
+        taken++;
+      }
+      // page of row j (of a row behind the partition's last: of its first, whose scores are not written)
+      const int32_t *pages = a.pages + (size_t)coming.g * a.max_pages;
+      const auto page_of = [&](uint32_t j) { return pages[j < coming.n ? page.div(j) : 0]; };
 #pragma unroll
-          for (int i = 0; i < QT; i++)
+      for (int i = 0; i < RT; i++) id[i] = page_of(coming.j0 + (i * 256 + tid) / NP % T);
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-              acc[i][r] = __builtin_fmaf(s, part[i][r], acc[i][r]);
-              part[i][r] = 0.0f;
-            }
-        }
+      for (int y = 0; y < 2; y++) col_id[y] = page_of(coming.j0 + wave_r + y * 32 + col);
+      if (FMT != NATIVE) scale_id = page_of(coming.j0 + tid % T);
+      if (round == -2) {
+        load_stage = stages;
+        continue;
       }
     }
 
-    if (j < n) {
+    // a stage under way
+    const uint32_t base = load_stage * KC;
 #pragma unroll
-      for (int i = 0; i < QT; i++)
+    for (int i = 0; i < RT; i++) {
+      const uint32_t e = base + tid % NP * PIECE;
+      const u4 *p = reinterpret_cast<const u4 *>(source[i] + (e < padded ? e : 0) / PIECE * PIECE_BYTES);
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-          const uint32_t q = q0 + i * 32 + 8 * (r / 4) + 4 * half + r % 4;
-          if (q < q_end) {
-            float p = acc[i][r];
-            if constexpr (FMT == NATIVE && Q == F32) {
-              // an infinity meets the other side's planes, some of them 0: the sum is taken again, element by element
-              if (p != p && there) p = plain_product(reinterpret_cast<const float *>(row), static_cast<const float *>(a.queries) + q * a.stride, a.c.dim);
-            }
-            if (a.form == RSGPU_SCORES_DISTANCE) p = 1.0f - p;
-            a.scores[(size_t)q * a.ld + j] = there ? p : gone;
+      for (int u = 0; u < PU; u++) row_held[i][u] = p[u];
+    }
+    if (FMT != NATIVE) {
+      const uint32_t b = (base + (FLUSH == KC ? 0 : tid / T * 32)) / a.c.block;
+      scale_held = scale_source[b < a.c.nb ? b : a.c.nb - 1];
+    }
+    const uint32_t query_at = base + tid % C8 * 8;
+    if (even) {
+#pragma unroll
+      for (int i = 0; i < QN; i++) {
+        const uint8_t *p = queries[i] + (query_at < a.c.dim ? query_at : 0) * elem_size<Q>;
+        if constexpr (Q == F32) {
+          query_held[i][0] = reinterpret_cast<const u4_any4 *>(p)[0];
+          query_held[i][1] = reinterpret_cast<const u4_any4 *>(p)[1];
+        } else {
+          query_held[i][0] = *reinterpret_cast<const u4_any *>(p);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < QN; i++) {
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+          const bool in = query_at + k < a.c.dim;
+          if constexpr (Q == F32) {
+            query_held[i][k / 4][k % 4] = reinterpret_cast<const uint32_t *>(queries[i])[in ? query_at + k : 0];
+          } else {
+            const uint32_t x = reinterpret_cast<const uint16_t *>(queries[i])[in ? query_at + k : 0];
+            query_held[i][0][k / 2] = k % 2 ? query_held[i][0][k / 2] | x << 16 : x;
           }
         }
+      }
+    }
+    load_stage++;
+
+    if (round >= 0) {
+      const u4 *q_at = q_lds[round & 1], *r_at = r_lds[round & 1];
+#pragma unroll
+      for (int k0 = 0; k0 < KC / 16; k0 += FLUSH / 16) {
+        f32x16 part[2][2];
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+          for (int y = 0; y < 2; y++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) part[x][y][r] = FMT == NATIVE ? acc[x][y][r] : 0.0f;
+#pragma unroll
+        for (int k = k0; k < k0 + FLUSH / 16; k++) {
+          u4 q[2][QP], r[2][RP];
+#pragma unroll
+          for (int x = 0; x < 2; x++) {
+#pragma unroll
+            for (int p = 0; p < QP; p++) q[x][p] = q_at[place(2 * k + half, QP, p, wave_q + x * 32 + col)];
+#pragma unroll
+            for (int p = 0; p < RP; p++) r[x][p] = r_at[place(2 * k + half, RP, p, wave_r + x * 32 + col)];
+          }
+#pragma unroll
+          for (int p = QP - 1; p >= 0; p--)   // the smallest first
+#pragma unroll
+            for (int c = RP - 1; c >= 0; c--)
+              if (p + c < 3) {   // the planes left out are below 2^-24 of the product
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+#pragma unroll
+                  for (int y = 0; y < 2; y++) part[x][y] = mfma<Q>(q[x][p], r[y][c], part[x][y]);
+              }
+        }
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+          const float scale = FMT == NATIVE ? 1.0f : s_lds[round & 1][FLUSH == KC ? 0 : k0 / 2][wave_r + y * 32 + col];
+#pragma unroll
+          for (int x = 0; x < 2; x++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) acc[x][y][r] = FMT == NATIVE ? part[x][y][r] : __builtin_fmaf(scale, part[x][y][r], acc[x][y][r]);
+        }
+      }
+      use_stage++;
+    }
+
+    // the stage under way into the other half of LDS, which nobody has read since the last barrier
+    u4 *q_to = q_lds[(round + 1) & 1], *r_to = r_lds[(round + 1) & 1];
+#pragma unroll
+    for (int i = 0; i < QN; i++) {
+      u4 w[QP];
+      if constexpr (Q == F32) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = query_at + (even ? 0 : k) < a.c.dim ? __uint_as_float(query_held[i][k / 4][k % 4]) : 0.0f;
+        planes8(v, w);
+      } else {
+        w[0] = query_held[i][0];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          if (even) w[0][k] = query_at < a.c.dim ? w[0][k] : 0;
+          else w[0][k] = (query_at + 2 * k < a.c.dim ? w[0][k] & 0xffffu : 0) | (query_at + 2 * k + 1 < a.c.dim ? w[0][k] & 0xffff0000u : 0);
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < QP; p++) q_to[place(tid % C8, QP, p, (i * 256 + tid) / C8)] = w[p];
+    }
+#pragma unroll
+    for (int i = 0; i < RT; i++) {
+      if (T * NP < 256 && tid >= (uint32_t)(T * NP)) break;
+      P piece;
+      const bool in = base + tid % NP * PIECE < padded;
+#pragma unroll
+      for (int k = 0; k < PIECE_BYTES / 4; k++) piece.raw[k] = FMT != NATIVE || in ? row_held[i][k / 4][k % 4] : 0;
+#pragma unroll
+      for (int f = 0; f < PIECE / 8; f++) {
+        u4 w[RP];
+        piece.fragment(f, w);
+#pragma unroll
+        for (int p = 0; p < RP; p++) r_to[place(tid % NP * (PIECE / 8) + f, RP, p, (i * 256 + tid) / NP)] = w[p];
+      }
+    }
+    if (FMT != NATIVE) s_lds[(round + 1) & 1][tid / T][tid % T] = scale_held;
+    __syncthreads();
+
+    if (use_stage == stages) {
+#pragma unroll
+      for (int y = 0; y < 2; y++) {
+        const uint32_t j = now.j0 + wave_r + y * 32 + col;
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            const uint32_t q = now.q0 + wave_q + x * 32 + 8 * (r / 4) + 4 * half + r % 4;
+            float p = acc[x][y][r] * CODE_UNIT<FMT, Q>;
+            acc[x][y][r] = 0.0f;
+            if (j < now.n && q < now.q_end) {
+              if constexpr (FMT == NATIVE && Q == F32) {
+                // an infinity meets the other side's planes, some of them 0: the sum is taken again, element by element
+                if (p != p && (there >> y & 1)) {
+                  bool is;
+                  const uint64_t slot = slot_of(j, a.pages[(size_t)now.g * a.max_pages + page.div(j)], is);
+                  p = plain_product(reinterpret_cast<const float *>(a.c.codes + slot * a.c.row_bytes), static_cast<const float *>(a.queries) + q * a.stride, a.c.dim);
+                }
+              }
+              if (a.form == RSGPU_SCORES_DISTANCE) p = 1.0f - p;
+              a.scores[(size_t)q * a.ld + j] = there >> y & 1 ? p : gone;
+            }
+          }
+      }
+      use_stage = 0;
+    }
+    if (use_stage == 0) {
+      now = held;
+      there = held_there;
     }
   }
 }
@@ -1149,7 +1263,12 @@ void scores_as(const PartitionArgs &a, hipStream_t s) {
     return dim3((uint32_t)(tiles < resident ? tiles : resident));
   };
   if (each >= 48) {
-    hipLaunchKernelGGL((partition_scores_kernel<FMT, Q, 4>), grid(128, ROW_TILE, 2048), dim3(256), 0, s, a, page);
+    const auto many = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid(128, 128, resident(reinterpret_cast<const void *>(kernel), 256)), dim3(256), 0, s, a, page); };
+    if (FMT != NATIVE && Q != F32 && a.c.block == 32) {
+      if constexpr (FMT != NATIVE) many(partition_many_kernel<FMT, Q, 32>);
+    } else {
+      many(partition_many_kernel<FMT, Q, Q == F32 ? 32 : 64>);
+    }
     return;
   }
   // the rows' chunks of a stage: the number that leaves the fewest places empty, the largest of those
