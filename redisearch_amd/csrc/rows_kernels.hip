@@ -475,7 +475,7 @@ struct Place {
   uint32_t g, lo, m, n, left;
 };
 struct Run {
-  uint32_t first, last;
+  uint32_t tiles, stride;
   Place at;
 };
 struct RunShared {
@@ -483,8 +483,10 @@ struct RunShared {
   Place at;
 };
 // The offsets and counts are on the device, so every workgroup sums the partitions' tiles itself, a share of the partitions a
-// thread, takes its even part of them, and the thread in whose share that begins says where.
-template <int THREADS>
+// thread, takes its even part of them, and the thread in whose share that begins says where.  TOGETHER: an eighth of the tiles, one
+// after the other, is for the workgroups b, b + 8, ... that share a die's L2, and they go through it side by side.
+constexpr uint32_t DIES = 8;
+template <int THREADS, bool TOGETHER>
 __device__ __forceinline__ Run find_run(const PartitionArgs &a, uint32_t tq, uint32_t tr, RunShared &shared) {
   const uint32_t tid = threadIdx.x, lane = tid % 64, per = (a.n_partitions + THREADS - 1) / THREADS;
   uint32_t own = 0;
@@ -511,12 +513,21 @@ __device__ __forceinline__ Run find_run(const PartitionArgs &a, uint32_t tq, uin
     total += v;
   }
   Run run;
-  run.first = (uint32_t)((uint64_t)total * blockIdx.x / gridDim.x);
-  run.last = (uint32_t)((uint64_t)total * (blockIdx.x + 1) / gridDim.x);
-  if (run.first == run.last) return run;
-  if (sum - own <= run.first && run.first < sum) {
+  uint32_t first;
+  if (TOGETHER) {
+    const uint32_t die = blockIdx.x % DIES, from = (uint32_t)((uint64_t)total * die / DIES), to = (uint32_t)((uint64_t)total * (die + 1) / DIES);
+    run.stride = gridDim.x / DIES;   // a multiple of the dies
+    first = from + blockIdx.x / DIES;
+    run.tiles = first < to ? (to - first + run.stride - 1) / run.stride : 0;
+  } else {
+    run.stride = 1;
+    first = (uint32_t)((uint64_t)total * blockIdx.x / gridDim.x);
+    run.tiles = (uint32_t)((uint64_t)total * (blockIdx.x + 1) / gridDim.x) - first;
+  }
+  if (run.tiles == 0) return run;
+  if (sum - own <= first && first < sum) {
     Place p;
-    p.left = run.first - (sum - own);
+    p.left = first - (sum - own);
     for (p.g = tid * per;; p.g++) {
       partition(a, p.g, p.lo, p.m, p.n);
       const uint32_t tiles = (p.m + tq - 1) / tq * ((p.n + tr - 1) / tr);
@@ -611,9 +622,8 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
   __shared__ RunShared run_shared;
 
   const uint32_t tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), col = lane % 16, quarter = lane / 16;
-  const Run run = find_run<64 * WAVES>(a, TQ, TR, run_shared);
-  const uint32_t first = run.first, last = run.last;
-  if (first == last) return;
+  const Run run = find_run<64 * WAVES, false>(a, TQ, TR, run_shared);
+  if (run.tiles == 0) return;
   Place at = run.at;
   const uint32_t chunks = a.c.row_bytes / 16, stages = (chunks + CS - 1) / CS;
   // blocks are one step or two, or the row
@@ -646,9 +656,9 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
 #pragma unroll
   for (int k = 0; k < S; k++) acc[k] = f32x4{0, 0, 0, 0};
   uint32_t staged_g = ~0u, staged_q = 0, staged_p = 0;   // whose queries are in LDS, from which stage on
-  uint32_t taken = first;
+  uint32_t taken = 0;
   uint32_t use_stage = 0, load_stage = stages;           // stages: on to the next tile before the next load
-  const int64_t rounds = (int64_t)(last - first) * stages;
+  const int64_t rounds = (int64_t)run.tiles * stages;
 
   for (int64_t round = -2; round < rounds; round++) {
     if (load_stage == stages) {
@@ -669,7 +679,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
         held_there |= is ? 1u << k : 0;
         scale_source[k] = a.c.scales + slot * a.c.nb;
       }
-      if (taken < last) {
+      if (taken < run.tiles) {
         uint32_t row_tiles = (at.n + TR - 1) / TR;
         while (at.left >= (at.m + TQ - 1) / TQ * row_tiles) {   // behind this partition's last tile
           at.g++;
@@ -876,12 +886,10 @@ __global__ __launch_bounds__(256, FMT == NATIVE && Q == F32 ? 1 : 2) void partit
   __shared__ RunShared run_shared;
 
   const uint32_t tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), col = lane % 32, half = lane / 32;
-  const Run run = find_run<256>(a, T, T, run_shared);
-  const uint32_t first = run.first, last = run.last;
-  if (first == last) return;
+  const Run run = find_run<256, true>(a, T, T, run_shared);
+  if (run.tiles == 0) return;
   Place at = run.at;
   const uint32_t padded = rows_padded(a.c.dim), stages = (padded + KC - 1) / KC;
-  const bool even = a.c.dim % 8 == 0;   // no eight of a query is cut by its end
   const float gone = a.form == RSGPU_SCORES_DISTANCE ? __builtin_inff() : -__builtin_inff();
   const auto slot_of = [&](uint32_t j, int32_t id, bool &there) {
     const uint64_t slot = (uint64_t)(uint32_t)id * page.d + (j - page.div(j) * page.d);
@@ -904,8 +912,8 @@ __global__ __launch_bounds__(256, FMT == NATIVE && Q == F32 ? 1 : 2) void partit
   const float *scale_source;
   u4 row_held[RT][PU], query_held[QN][QU];
   float scale_held;
-  uint32_t taken = first, load_stage = stages, use_stage = 0;
-  const int64_t rounds = (int64_t)(last - first) * stages;
+  uint32_t taken = 0, load_stage = stages, use_stage = 0;
+  const int64_t rounds = (int64_t)run.tiles * stages;
   const uint32_t wave_q = wave / 2 * 64, wave_r = wave % 2 * 64;
   f32x16 acc[2][2];
 #pragma unroll
@@ -935,17 +943,18 @@ __global__ __launch_bounds__(256, FMT == NATIVE && Q == F32 ? 1 : 2) void partit
         const uint32_t q = held.q0 + (i * 256 + tid) / C8;   // of a query behind the partition's last: the last's, not used
         queries[i] = static_cast<const uint8_t *>(a.queries) + (size_t)(q < held.q_end ? q : held.q_end ? held.q_end - 1 : 0) * a.stride * elem_size<Q>;
       }
-      if (taken < last) {
-        uint32_t query_tiles = (at.m + T - 1) / T;
-        while (at.left >= query_tiles * ((at.n + T - 1) / T)) {   // behind this partition's last tile
+      if (taken < run.tiles) {
+        uint32_t query_tiles = (at.m + T - 1) / T, tiles = query_tiles * ((at.n + T - 1) / T);
+        while (at.left >= tiles) {   // behind this partition's last tile
           at.g++;
-          at.left = 0;
+          at.left -= tiles;
           partition_of_all(a, at.g, at.lo, at.m, at.n);
           query_tiles = (at.m + T - 1) / T;
+          tiles = query_tiles * ((at.n + T - 1) / T);
         }
         const uint32_t row_tile = at.left / query_tiles;
         coming = Tile{at.g, at.lo + (at.left - row_tile * query_tiles) * T, at.lo + at.m, at.n, row_tile * T};
-        at.left++;
+        at.left += run.stride;
         taken++;
       }
       // page of row j (of a row behind the partition's last: of its first, whose scores are not written)
@@ -975,31 +984,17 @@ __global__ __launch_bounds__(256, FMT == NATIVE && Q == F32 ? 1 : 2) void partit
       const uint32_t b = (base + (FLUSH == KC ? 0 : tid / T * 32)) / a.c.block;
       scale_held = scale_source[b < a.c.nb ? b : a.c.nb - 1];
     }
-    const uint32_t query_at = base + tid % C8 * 8;
-    if (even) {
+    // (an eight that the query's end cuts is loaded from where it is whole, and moved below; rows of less than eight elements do
+    // not come here)
+    const uint32_t query_at = base + tid % C8 * 8, query_from = query_at + 8 <= a.c.dim ? query_at : a.c.dim - 8;
 #pragma unroll
-      for (int i = 0; i < QN; i++) {
-        const uint8_t *p = queries[i] + (query_at < a.c.dim ? query_at : 0) * elem_size<Q>;
-        if constexpr (Q == F32) {
-          query_held[i][0] = reinterpret_cast<const u4_any4 *>(p)[0];
-          query_held[i][1] = reinterpret_cast<const u4_any4 *>(p)[1];
-        } else {
-          query_held[i][0] = *reinterpret_cast<const u4_any *>(p);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < QN; i++) {
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-          const bool in = query_at + k < a.c.dim;
-          if constexpr (Q == F32) {
-            query_held[i][k / 4][k % 4] = reinterpret_cast<const uint32_t *>(queries[i])[in ? query_at + k : 0];
-          } else {
-            const uint32_t x = reinterpret_cast<const uint16_t *>(queries[i])[in ? query_at + k : 0];
-            query_held[i][0][k / 2] = k % 2 ? query_held[i][0][k / 2] | x << 16 : x;
-          }
-        }
+    for (int i = 0; i < QN; i++) {
+      const uint8_t *p = queries[i] + (size_t)query_from * elem_size<Q>;
+      if constexpr (Q == F32) {
+        query_held[i][0] = reinterpret_cast<const u4_any4 *>(p)[0];
+        query_held[i][1] = reinterpret_cast<const u4_any4 *>(p)[1];
+      } else {
+        query_held[i][0] = *reinterpret_cast<const u4_any *>(p);
       }
     }
     load_stage++;
@@ -1050,21 +1045,43 @@ __global__ __launch_bounds__(256, FMT == NATIVE && Q == F32 ? 1 : 2) void partit
 
     // the stage under way into the other half of LDS, which nobody has read since the last barrier
     u4 *q_to = q_lds[(round + 1) & 1], *r_to = r_lds[(round + 1) & 1];
+    if (base + KC > a.c.dim) {   // the row's end is in it: zeros behind it
+      const uint32_t by = query_at - query_from;
+#pragma unroll
+      for (int i = 0; i < QN; i++) {
+        uint32_t v[4 * QU];
+#pragma unroll
+        for (int k = 0; k < 4 * QU; k++) v[k] = by < 8 ? query_held[i][k / 4][k % 4] : 0;
+#pragma unroll
+        for (int m = 4; m >= 1; m /= 2) {
+          const bool move = by & m;
+          const int d = m * elem_size<Q> / 4;
+#pragma unroll
+          for (int k = 0; k < 4 * QU; k++) {
+            const uint32_t next = k + 1 < 4 * QU ? v[k + 1 < 4 * QU ? k + 1 : 0] : 0, far = d && k + d < 4 * QU ? v[k + d < 4 * QU ? k + d : 0] : 0;
+            v[k] = move ? (d ? far : __builtin_amdgcn_alignbit(next, v[k], 16)) : v[k];
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4 * QU; k++) query_held[i][k / 4][k % 4] = v[k];
+      }
+      if (FMT == NATIVE) {
+#pragma unroll
+        for (int i = 0; i < RT; i++)
+#pragma unroll
+          for (int k = 0; k < 4 * PU; k++) row_held[i][k / 4][k % 4] = base + tid % NP * PIECE < padded ? row_held[i][k / 4][k % 4] : 0;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < QN; i++) {
       u4 w[QP];
       if constexpr (Q == F32) {
         float v[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = query_at + (even ? 0 : k) < a.c.dim ? __uint_as_float(query_held[i][k / 4][k % 4]) : 0.0f;
+        for (int k = 0; k < 8; k++) v[k] = __uint_as_float(query_held[i][k / 4][k % 4]);
         planes8(v, w);
       } else {
         w[0] = query_held[i][0];
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-          if (even) w[0][k] = query_at < a.c.dim ? w[0][k] : 0;
-          else w[0][k] = (query_at + 2 * k < a.c.dim ? w[0][k] & 0xffffu : 0) | (query_at + 2 * k + 1 < a.c.dim ? w[0][k] & 0xffff0000u : 0);
-        }
       }
 #pragma unroll
       for (int p = 0; p < QP; p++) q_to[place(tid % C8, QP, p, (i * 256 + tid) / C8)] = w[p];
@@ -1073,9 +1090,8 @@ __global__ __launch_bounds__(256, FMT == NATIVE && Q == F32 ? 1 : 2) void partit
     for (int i = 0; i < RT; i++) {
       if (T * NP < 256 && tid >= (uint32_t)(T * NP)) break;
       P piece;
-      const bool in = base + tid % NP * PIECE < padded;
 #pragma unroll
-      for (int k = 0; k < PIECE_BYTES / 4; k++) piece.raw[k] = FMT != NATIVE || in ? row_held[i][k / 4][k % 4] : 0;
+      for (int k = 0; k < PIECE_BYTES / 4; k++) piece.raw[k] = row_held[i][k / 4][k % 4];
 #pragma unroll
       for (int f = 0; f < PIECE / 8; f++) {
         u4 w[RP];
@@ -1262,8 +1278,12 @@ void scores_as(const PartitionArgs &a, hipStream_t s) {
     const uint64_t tiles = ((uint64_t)a.n_queries / tq + asked) * ((a.most_rows + tr - 1) / tr);
     return dim3((uint32_t)(tiles < resident ? tiles : resident));
   };
-  if (each >= 48) {
-    const auto many = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid(128, 128, resident(reinterpret_cast<const void *>(kernel), 256)), dim3(256), 0, s, a, page); };
+  if (each >= 48 && a.c.dim >= 8) {
+    const auto many = [&](auto kernel) {
+      dim3 g = grid(128, 128, resident(reinterpret_cast<const void *>(kernel), 256));
+      g.x = (g.x + DIES - 1) / DIES * DIES;
+      hipLaunchKernelGGL(kernel, g, dim3(256), 0, s, a, page);
+    };
     if (FMT != NATIVE && Q != F32 && a.c.block == 32) {
       if constexpr (FMT != NATIVE) many(partition_many_kernel<FMT, Q, 32>);
     } else {
