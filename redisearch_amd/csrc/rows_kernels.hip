@@ -18,6 +18,8 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int F32 = VecSimType_FLOAT32, BF16 = VecSimType_BFLOAT16, F16 = VecSimType_FLOAT16;
@@ -361,7 +363,6 @@ __device__ __forceinline__ f32x16 mfma(u4 a, u4 b, f32x16 c) {
   }
 }
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 template <int Q>
 __device__ __forceinline__ f32x4 mfma16(u4 a, u4 b, f32x4 c) {
   if constexpr (Q == F16) {
@@ -1144,8 +1145,9 @@ constexpr uint32_t COLUMNS = 4096;   // columns of a workgroup, whose counts of 
 // A workgroup finds in the lists what falls among its columns (sums and maxima of integers: the same in any order), then goes over
 // them once.
 __global__ __launch_bounds__(256) void adjust_scores_kernel(AdjustArgs a, uint32_t tiles, uint64_t work) {
-  __shared__ uint32_t times[COLUMNS];   // how often a column was shown
-  __shared__ uint32_t boost[COLUMNS];   // 1 + the place in the list of a column's last boost, 0: none
+  constexpr int PER = COLUMNS / 1024;
+  __shared__ alignas(16) uint32_t times[COLUMNS];   // how often a column was shown
+  __shared__ alignas(16) uint32_t boost[COLUMNS];   // 1 + the place in the list of a column's last boost, 0: none
   const uint32_t tid = threadIdx.x;
   for (uint64_t w = blockIdx.x; w < work; w += gridDim.x) {
     const uint32_t m = (uint32_t)(w / tiles), c0 = (uint32_t)(w - (uint64_t)m * tiles) * COLUMNS;
@@ -1165,7 +1167,7 @@ __global__ __launch_bounds__(256) void adjust_scores_kernel(AdjustArgs a, uint32
     const bool lists = s1 > s0 || b1 > b0;
     if (lists) {
       __syncthreads();   // the last piece's counts have been read
-      for (uint32_t i = tid; i < mine; i += 256) times[i] = boost[i] = 0;
+      for (uint32_t i = tid; i < COLUMNS / 4; i += 256) reinterpret_cast<u4 *>(times)[i] = reinterpret_cast<u4 *>(boost)[i] = u4{0, 0, 0, 0};
       __syncthreads();
       for (int32_t i = s0 + (int32_t)tid; i < s1; i += 256) {
         const uint32_t c = (uint32_t)a.r.seen_ids[i] - c0;
@@ -1178,6 +1180,7 @@ __global__ __launch_bounds__(256) void adjust_scores_kernel(AdjustArgs a, uint32
       __syncthreads();
     }
     const bool distance = a.r.form == RSGPU_SCORES_DISTANCE;
+    const float gone = distance ? __builtin_inff() : -__builtin_inff();
     const float rep = a.r.repetition ? a.r.repetition[m] : 1.0f;
     const float freq = a.r.frequency ? a.r.frequency[m] : 0.0f;
     const float pres = a.r.presence ? a.r.presence[m] : 0.0f;
@@ -1188,22 +1191,52 @@ __global__ __launch_bounds__(256) void adjust_scores_kernel(AdjustArgs a, uint32
     }
     const float *in = a.in + (size_t)m * a.ld + c0;
     float *out = a.out + (size_t)m * a.ld + c0;
-    for (uint32_t i = tid; i < mine; i += 256) {
-      float v = in[i];
+    // sixteen columns a thread, all loaded before the first is written (scores_out may be scores_in)
+    f32x4 v[PER];
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+      const uint32_t i = (k * 256 + tid) * 4;
+      if (i + 4 <= mine) {
+        v[k] = *reinterpret_cast<const f32x4_any *>(in + i);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[k][e] = i + e < mine ? in[i + e] : 0.0f;
+      }
+    }
+    uint32_t allowed[PER];
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+      const uint32_t i = (k * 256 + tid) * 4;
+      allowed[k] = mask && i < mine ? mask[(c0 + i) / 32] >> (c0 + i) % 32 : 15u;   // the four are in one word
+    }
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+      const uint32_t i = (k * 256 + tid) * 4;
       if (lists) {
-        const uint32_t k = times[i], b = boost[i];
-        if (k | b) {
-          float p = distance ? 1.0f - v : v;
-          if (k) {
-            p = p > 0.0f ? p / rep : p * rep;
-            p -= __builtin_fmaf((float)k, freq, pres);
-          }
-          if (b) p += a.r.bias_values[b0 + b - 1];
-          v = distance ? 1.0f - p : p;
+        const u4 n4 = *reinterpret_cast<const u4 *>(times + i), b4 = *reinterpret_cast<const u4 *>(boost + i);
+        if (((n4[0] | n4[1]) | (n4[2] | n4[3])) | ((b4[0] | b4[1]) | (b4[2] | b4[3]))) {
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (n4[e] | b4[e]) {
+              float p = distance ? 1.0f - v[k][e] : v[k][e];
+              if (n4[e]) {
+                p = p > 0.0f ? p / rep : p * rep;
+                p -= __builtin_fmaf((float)n4[e], freq, pres);
+              }
+              if (b4[e]) p += a.r.bias_values[b0 + b4[e] - 1];
+              v[k][e] = distance ? 1.0f - p : p;
+            }
         }
       }
-      if (mask && !((mask[(c0 + i) / 32] >> ((c0 + i) % 32)) & 1u)) v = distance ? __builtin_inff() : -__builtin_inff();
-      out[i] = v;
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[k][e] = allowed[k] >> e & 1u ? v[k][e] : gone;
+      if (i + 4 <= mine) {
+        *reinterpret_cast<f32x4_any *>(out + i) = v[k];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (i + e < mine) out[i + e] = v[k][e];
+      }
     }
   }
 }
