@@ -40,7 +40,6 @@ struct FastDiv {
   }
 };
 
-__device__ __forceinline__ float bf16_to_f32(uint32_t low16) { return __uint_as_float(low16 << 16); }
 __device__ __forceinline__ float f16_to_f32(uint32_t low16) {
   const uint16_t h = (uint16_t)low16;
   _Float16 x;
@@ -48,37 +47,46 @@ __device__ __forceinline__ float f16_to_f32(uint32_t low16) {
   return (float)x;
 }
 
-// eight elements as fp32; those from `valid` on are zeros and not read
+// eight elements as they are in memory; those from `valid` on are zeros and not read
+template <int T>
+struct Raw8 {
+  u4 w[elem_size<T> / 2];
+
+  __device__ __forceinline__ void load(const void *row, uint32_t at, uint32_t valid) {
+    if (valid >= 8) {
+      if constexpr (T == F32) {
+        const u4_any4 *p = reinterpret_cast<const u4_any4 *>(static_cast<const float *>(row) + at);
+        w[0] = p[0];
+        w[1] = p[1];
+      } else {
+        w[0] = *reinterpret_cast<const u4_any *>(static_cast<const uint16_t *>(row) + at);
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < (int)(elem_size<T> / 2); i++) w[i] = u4{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if ((uint32_t)i < valid) {
+        if constexpr (T == F32) w[i / 4][i % 4] = static_cast<const uint32_t *>(row)[at + i];
+        else w[0][i / 2] |= (uint32_t)static_cast<const uint16_t *>(row)[at + i] << (16 * (i % 2));
+      }
+  }
+  __device__ __forceinline__ void floats(float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      if constexpr (T == F32) v[i] = __uint_as_float(w[i / 4][i % 4]);
+      else if constexpr (T == BF16) v[i] = __uint_as_float(i % 2 ? w[0][i / 2] & 0xffff0000u : w[0][i / 2] << 16);
+      else v[i] = f16_to_f32(i % 2 ? w[0][i / 2] >> 16 : w[0][i / 2] & 0xffffu);
+    }
+  }
+};
+
 template <int T>
 __device__ __forceinline__ void load8(const void *row, uint32_t at, uint32_t valid, float (&v)[8]) {
-  if (valid >= 8) {
-    if constexpr (T == F32) {
-      const u4_any4 *p = reinterpret_cast<const u4_any4 *>(static_cast<const float *>(row) + at);
-      const u4 a = p[0], b = p[1];
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        v[i] = __uint_as_float(a[i]);
-        v[4 + i] = __uint_as_float(b[i]);
-      }
-    } else {
-      const u4 a = *reinterpret_cast<const u4_any *>(static_cast<const uint16_t *>(row) + at);
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        v[2 * i] = T == BF16 ? __uint_as_float(a[i] << 16) : f16_to_f32(a[i] & 0xffffu);
-        v[2 * i + 1] = T == BF16 ? __uint_as_float(a[i] & 0xffff0000u) : f16_to_f32(a[i] >> 16);
-      }
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    float x = 0.0f;
-    if ((uint32_t)i < valid) {
-      if constexpr (T == F32) x = static_cast<const float *>(row)[at + i];
-      else x = T == BF16 ? bf16_to_f32(static_cast<const uint16_t *>(row)[at + i]) : f16_to_f32(static_cast<const uint16_t *>(row)[at + i]);
-    }
-    v[i] = x;
-  }
+  Raw8<T> raw;
+  raw.load(row, at, valid);
+  raw.floats(v);
 }
 
 // ---- writing ---------------------------------------------------------------------------------------------------------------
@@ -112,13 +120,12 @@ __device__ __forceinline__ void scale_of(uint32_t most, float &s, float &inv) {
     inv = __uint_as_float((254 - e) << 23);
   } else {
     s = __uint_as_float(most) / (FMT == INT8 ? 127.0f : 7.0f);
-    inv = 1.0f / s;
+    inv = __builtin_amdgcn_rcpf(s);
   }
 }
 
-// x / s to the nearest integer, ties to even, as if divided exactly.  x * inv is off by at most two ulps, so its rounding t is
-// the answer or next to it; r = x - t s is exact (one fused step: |r| is at most about s / 2 and a multiple of the smaller ulp of
-// x and s), so |r| against s / 2 says which.
+// x / s to the nearest integer, ties to even, as if divided exactly.  t is the answer or next to it; r = x - t s is exact (one fused
+// step: |r| is at most about s and a multiple of the smaller ulp of x and s), so |r| against s / 2 says which.
 __device__ __forceinline__ float settle(float x, float s, float t) {
   const float h = 0.5f * s;
   const float r = __builtin_fmaf(-t, s, x);
@@ -128,6 +135,8 @@ __device__ __forceinline__ float settle(float x, float s, float t) {
   return a > h || (a == h && odd) ? next : t;
 }
 
+// fp32 numbers in [2^23, 2^24) have their integer in the low bits: x inv + 1.5 * 2^23 is rounded to one, in two's complement.  inv is
+// off by an ulp or two, so the integer may be next to the right one where x / s is next to a border; x - t s (see settle) shows it.
 template <int FMT>
 __device__ __forceinline__ void encode8(const float (&v)[8], float s, float inv, uint32_t (&c)[2]) {
   c[0] = c[1] = 0;
@@ -141,15 +150,27 @@ __device__ __forceinline__ void encode8(const float (&v)[8], float s, float inv,
       c[i] = (uint32_t)w;
     }
   } else {
-    int q[8];
+    constexpr float magic = 12582912.0f;
+    float u[8], off = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; i++) q[i] = (int)settle(v[i], s, __builtin_rintf(v[i] * inv));
+    for (int i = 0; i < 8; i++) {
+      u[i] = __builtin_fmaf(v[i], inv, magic);
+      off = __builtin_fmaxf(off, __builtin_fabsf(__builtin_fmaf(magic - u[i], s, v[i])));
+    }
+    if (off >= 0.5f * s) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) u[i] = magic + settle(v[i], s, u[i] - magic);
+    }
+    uint32_t q[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) q[i] = __float_as_uint(u[i]);
     if constexpr (FMT == INT8) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) c[i / 4] |= ((uint32_t)q[i] & 255u) << (8 * (i % 4));
+      for (int i = 0; i < 2; i++)
+        c[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(q[4 * i + 3], q[4 * i + 2], 0x0c0c0400u), __builtin_amdgcn_perm(q[4 * i + 1], q[4 * i], 0x0c0c0400u), 0x05040100u);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; i++) c[0] |= ((uint32_t)q[i] & 15u) << (4 * i);
+      for (int i = 0; i < 8; i++) c[0] |= (q[i] & 15u) << (4 * i);
     }
   }
 }
@@ -160,33 +181,62 @@ __device__ __forceinline__ void store_codes8(uint8_t *row, uint32_t chunk, const
   else *reinterpret_cast<u2 *>(row + chunk * 8) = u2{c[0], c[1]};
 }
 
-// blocks of 8 L elements: L neighbouring lanes have a block, eight elements each
+// the largest of a value in L neighbouring lanes, all of which are active: their neighbours by twos and fours, then halves mirrored
+template <int CTRL>
+__device__ __forceinline__ uint32_t max_dpp(uint32_t x) {
+  const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
+  return x > o ? x : o;
+}
+template <int L>
+__device__ __forceinline__ uint32_t most_of_lanes(uint32_t x) {
+  x = max_dpp<0xB1>(x);                      // quad_perm [1, 0, 3, 2]
+  x = max_dpp<0x4E>(x);                      // quad_perm [2, 3, 0, 1]
+  if (L >= 8) x = max_dpp<0x141>(x);         // row_half_mirror
+  if (L >= 16) x = max_dpp<0x140>(x);        // row_mirror
+#pragma unroll
+  for (int k = 16; k < L; k *= 2) {
+    const uint32_t o = __shfl_xor(x, k, 64);
+    x = x > o ? x : o;
+  }
+  return x;
+}
+
+// blocks of 8 L elements: L neighbouring lanes have a block, eight elements each; a thread has several of them under way
 template <int T, int FMT, int L>
 __global__ __launch_bounds__(256) void row_write_kernel(RowCacheArgs c, const void *rows, size_t stride, const int64_t *slots, uint32_t n,
                                                         uint32_t rows_per_wg, FastDiv chunks) {
+  constexpr int U = 4;
+  const uint32_t padded = rows_padded(c.dim);
   for (uint64_t first = (uint64_t)blockIdx.x * rows_per_wg; first < n; first += (uint64_t)gridDim.x * rows_per_wg) {
     const uint32_t mine = n - first < rows_per_wg ? (uint32_t)(n - first) : rows_per_wg;
-    const uint32_t padded = (c.dim + 31) / 32 * 32;
-    for (uint32_t i = threadIdx.x; i < mine * chunks.d; i += 256) {
-      const uint32_t r = chunks.div(i), chunk = i - r * chunks.d;
-      const int64_t slot = slots[first + r];
-      if (slot < 0 || (uint64_t)slot >= c.capacity) continue;   // the same for all lanes of a block
-      const void *row = static_cast<const uint8_t *>(rows) + (size_t)(first + r) * stride * elem_size<T>;
-      const uint32_t at = chunk * 8;
-      float v[8];
-      load8<T>(row, at, at < c.dim ? c.dim - at : 0, v);
-      uint32_t most = most8(v);
+    for (uint32_t i0 = threadIdx.x; i0 < mine * chunks.d; i0 += 256 * U) {
+      int64_t slot[U];
+      uint32_t chunk[U];
+      Raw8<T> raw[U];
 #pragma unroll
-      for (int k = 1; k < L; k *= 2) {
-        const uint32_t o = __shfl_xor(most, k, 64);
-        most = most > o ? most : o;
+      for (int u = 0; u < U; u++) {
+        const uint32_t i = i0 + u * 256, r = chunks.div(i);
+        const bool in = i < mine * chunks.d;
+        chunk[u] = i - r * chunks.d;
+        slot[u] = in ? slots[first + r] : -1;
+        const void *row = static_cast<const uint8_t *>(rows) + (size_t)(first + r) * stride * elem_size<T>;
+        const uint32_t at = chunk[u] * 8;
+        raw[u].load(row, at, in && at < c.dim ? c.dim - at : 0);
       }
-      float s, inv;
-      scale_of<FMT>(most, s, inv);
-      uint32_t code[2];
-      encode8<FMT>(v, s, inv, code);
-      if (at < padded) store_codes8<FMT>(c.codes + (size_t)slot * c.row_bytes, chunk, code);
-      if (chunk % L == 0) c.scales[(size_t)slot * c.nb + chunk / L] = s;
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        float v[8];
+        raw[u].floats(v);
+        const uint32_t most = most_of_lanes<L>(most8(v));
+        float s, inv;
+        scale_of<FMT>(most, s, inv);
+        uint32_t code[2];
+        encode8<FMT>(v, s, inv, code);
+        if (slot[u] >= 0 && (uint64_t)slot[u] < c.capacity) {
+          if (chunk[u] * 8 < padded) store_codes8<FMT>(c.codes + (size_t)slot[u] * c.row_bytes, chunk[u], code);
+          if (chunk[u] % L == 0) c.scales[(size_t)slot[u] * c.nb + chunk[u] / L] = s;
+        }
+      }
     }
   }
 }
@@ -207,11 +257,7 @@ __global__ __launch_bounds__(256) void row_write_whole_kernel(RowCacheArgs c, co
       const uint32_t o = most8(v);
       most = most > o ? most : o;
     }
-#pragma unroll
-    for (int k = 1; k < 64; k *= 2) {
-      const uint32_t o = __shfl_xor(most, k, 64);
-      most = most > o ? most : o;
-    }
+    most = most_of_lanes<64>(most);
     float s, inv;
     scale_of<FMT>(most, s, inv);
     for (uint32_t at = lane * 8; at < padded; at += 512) {
@@ -254,25 +300,31 @@ __global__ __launch_bounds__(256) void row_copy_in_kernel(RowCacheArgs c, const 
 
 // ---- reading ---------------------------------------------------------------------------------------------------------------
 
-template <int FMT>
-__device__ __forceinline__ void decode8(const uint8_t *row, uint32_t chunk, float (&v)[8]) {
+// E neighbouring codes, as they are in memory
+template <int FMT, int E>
+__device__ __forceinline__ void load_codes(const uint8_t *row, uint32_t at, uint32_t (&w)[2]) {
   if constexpr (FMT == INT4) {
-    const uint32_t w = *reinterpret_cast<const uint32_t *>(row + chunk * 4);
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = (float)((int32_t)(w << (28 - 4 * i)) >> 28);
+    if constexpr (E == 8) w[0] = *reinterpret_cast<const uint32_t *>(row + at / 2);
+    else w[0] = *reinterpret_cast<const uint16_t *>(row + at / 2);
   } else {
-    const u2 w = *reinterpret_cast<const u2 *>(row + chunk * 8);
+    w[0] = *reinterpret_cast<const uint32_t *>(row + at);
+    if constexpr (E == 8) w[1] = reinterpret_cast<const uint32_t *>(row + at)[1];
+  }
+}
+template <int FMT, int E>
+__device__ __forceinline__ void decode(const uint32_t (&w)[2], float (&v)[E]) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      if constexpr (FMT == INT8) {
-        v[i] = (float)(int8_t)(w[i / 4] >> (8 * (i % 4)));
-      } else {
-        switch (i % 4) {
-          case 0: v[i] = __builtin_amdgcn_cvt_f32_fp8((int)w[i / 4], 0); break;
-          case 1: v[i] = __builtin_amdgcn_cvt_f32_fp8((int)w[i / 4], 1); break;
-          case 2: v[i] = __builtin_amdgcn_cvt_f32_fp8((int)w[i / 4], 2); break;
-          default: v[i] = __builtin_amdgcn_cvt_f32_fp8((int)w[i / 4], 3); break;
-        }
+  for (int i = 0; i < E; i++) {
+    if constexpr (FMT == INT4) {
+      v[i] = (float)((int32_t)(w[0] << (28 - 4 * i)) >> 28);
+    } else if constexpr (FMT == INT8) {
+      v[i] = (float)(int8_t)(w[i / 4] >> (8 * (i % 4)));
+    } else {
+      switch (i % 4) {
+        case 0: v[i] = __builtin_amdgcn_cvt_f32_fp8((int)w[i / 4], 0); break;
+        case 1: v[i] = __builtin_amdgcn_cvt_f32_fp8((int)w[i / 4], 1); break;
+        case 2: v[i] = __builtin_amdgcn_cvt_f32_fp8((int)w[i / 4], 2); break;
+        default: v[i] = __builtin_amdgcn_cvt_f32_fp8((int)w[i / 4], 3); break;
       }
     }
   }
@@ -292,50 +344,74 @@ __device__ __forceinline__ uint32_t narrow2(float a, float b) {
   return w;
 }
 
+// sixteen bytes of output a thread, neighbouring threads' next to each other; a thread has several under way
 template <int T, int FMT>
 __global__ __launch_bounds__(256) void row_read_kernel(RowCacheArgs c, const int64_t *slots, uint32_t n, void *out, size_t stride,
                                                        uint32_t rows_per_wg, FastDiv chunks, FastDiv block) {
+  constexpr int U = 4, E = 16 / elem_size<T>;
   for (uint64_t first = (uint64_t)blockIdx.x * rows_per_wg; first < n; first += (uint64_t)gridDim.x * rows_per_wg) {
-    const uint32_t mine = n - first < rows_per_wg ? (uint32_t)(n - first) : rows_per_wg;
-    for (uint32_t i = threadIdx.x; i < mine * chunks.d; i += 256) {
-      const uint32_t r = chunks.div(i), chunk = i - r * chunks.d, at = chunk * 8;
-      const int64_t slot = slots[first + r];
-      float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (slot >= 0 && (uint64_t)slot < c.capacity) {
-        const uint8_t *row = c.codes + (size_t)slot * c.row_bytes;
+    const uint32_t mine = n - first < rows_per_wg ? (uint32_t)(n - first) : rows_per_wg, all = mine * chunks.d;
+    for (uint32_t i0 = threadIdx.x; i0 < all; i0 += 256 * U) {
+      uint32_t row[U], at[U], codes[U][2];
+      int64_t slot[U];
+      u4 as_is[U];
+      float scale[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const uint32_t i = i0 + u * 256 < all ? i0 + u * 256 : i0;   // behind the end: the first again, not written
+        row[u] = chunks.div(i);
+        at[u] = (i - row[u] * chunks.d) * E;
+        slot[u] = slots[first + row[u]];
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const bool there = slot[u] >= 0 && (uint64_t)slot[u] < c.capacity;
+        const size_t from = there ? (size_t)slot[u] : 0;   // one that is not there is read from slot 0 and zeroed
+        const uint8_t *p = c.codes + from * c.row_bytes;
         if constexpr (FMT == NATIVE) {
-          load8<T>(row, at, 8, v);   // the row's memory is whole units
+          as_is[u] = *reinterpret_cast<const u4 *>(p + at[u] * elem_size<T>);
+          if (!there) as_is[u] = u4{0, 0, 0, 0};
         } else {
-          const float s = c.scales[(size_t)slot * c.nb + block.div(at)];   // a block begins at a multiple of eight
-          decode8<FMT>(row, chunk, v);
-#pragma unroll
-          for (int k = 0; k < 8; k++) v[k] *= s;
-          // a block whose codes reach past the type's range (a largest magnitude next to its end): nothing finite becomes infinite
-          constexpr float most = T == F32 ? 3.40282347e38f : T == BF16 ? 3.38953139e38f : 65504.0f;
-          if (s > most / (FMT == E4M3 ? 448.0f : FMT == INT8 ? 128.0f : 8.0f)) {
-#pragma unroll
-            for (int k = 0; k < 8; k++) v[k] = __builtin_fabsf(v[k]) > most ? __builtin_copysignf(most, v[k]) : v[k];
-          }
+          load_codes<FMT, E>(p, at[u], codes[u]);
+          scale[u] = c.scales[from * c.nb + block.div(at[u])];
+          if (!there) codes[u][0] = codes[u][1] = 0;
+          if (!there) scale[u] = 0.0f;
         }
       }
-      uint8_t *dst = static_cast<uint8_t *>(out) + ((size_t)(first + r) * stride + at) * elem_size<T>;
-      if constexpr (T == F32) {
-        if (at + 8 <= c.dim) {
-          reinterpret_cast<u4_any *>(dst)[0] = u4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
-          reinterpret_cast<u4_any *>(dst)[1] = u4{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])};
-        } else {
 #pragma unroll
-          for (int k = 0; k < 8; k++)
-            if (at + k < c.dim) reinterpret_cast<float *>(dst)[k] = v[k];
+      for (int u = 0; u < U; u++) {
+        if (i0 + u * 256 >= all) break;
+        u4 w;
+        if constexpr (FMT == NATIVE) {
+          w = as_is[u];
+        } else {
+          float v[E];
+          decode<FMT, E>(codes[u], v);
+#pragma unroll
+          for (int k = 0; k < E; k++) v[k] *= scale[u];
+          // a block whose codes reach past the type's range (a largest magnitude next to its end): nothing finite becomes infinite
+          constexpr float most = T == F32 ? 3.40282347e38f : T == BF16 ? 3.38953139e38f : 65504.0f;
+          if (scale[u] > most / (FMT == E4M3 ? 448.0f : FMT == INT8 ? 128.0f : 8.0f)) {
+#pragma unroll
+            for (int k = 0; k < E; k++) v[k] = __builtin_fabsf(v[k]) > most ? __builtin_copysignf(most, v[k]) : v[k];
+          }
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            if constexpr (T == F32) w[k] = __float_as_uint(v[k]);
+            else w[k] = narrow2<T>(v[2 * k], v[2 * k + 1]);
+          }
         }
-      } else {
-        const u4 w = {narrow2<T>(v[0], v[1]), narrow2<T>(v[2], v[3]), narrow2<T>(v[4], v[5]), narrow2<T>(v[6], v[7])};
-        if (at + 8 <= c.dim) {
-          *reinterpret_cast<u4_any *>(dst) = w;
+        uint8_t *dst = static_cast<uint8_t *>(out) + ((size_t)(first + row[u]) * stride + at[u]) * elem_size<T>;
+        if (at[u] + E <= c.dim) {
+          if constexpr (T == F32) *reinterpret_cast<u4_any4 *>(dst) = w;
+          else *reinterpret_cast<u4_any *>(dst) = w;
         } else {
 #pragma unroll
-          for (int k = 0; k < 8; k++)
-            if (at + k < c.dim) reinterpret_cast<uint16_t *>(dst)[k] = (uint16_t)(w[k / 2] >> (16 * (k % 2)));
+          for (int k = 0; k < E; k++)
+            if (at[u] + k < c.dim) {
+              if constexpr (T == F32) reinterpret_cast<uint32_t *>(dst)[k] = w[k];
+              else reinterpret_cast<uint16_t *>(dst)[k] = (uint16_t)(w[k / 2] >> (16 * (k % 2)));
+            }
         }
       }
     }
@@ -1281,7 +1357,8 @@ void write_from(const RowCacheArgs &c, const void *rows, size_t stride, const in
 
 template <int T>
 void read_to(const RowCacheArgs &c, const int64_t *slots, uint32_t n, void *out, size_t stride, hipStream_t s) {
-  const uint32_t chunks = (c.dim + 7) / 8, per = rows_a_workgroup(n, chunks);
+  constexpr uint32_t E = 16 / elem_size<T>;
+  const uint32_t chunks = (c.dim + E - 1) / E, per = rows_a_workgroup(n, chunks);
   const dim3 grid(workgroups(((uint64_t)n + per - 1) / per));
   const FastDiv d(chunks), b(c.block);
   switch (c.format) {
