@@ -37,7 +37,7 @@ typedef struct RSGPU_RowCache {
   int format;             /* RSGPU_RowFormat */
   uint32_t dim;           /* 1 .. 65536 */
   uint32_t block;         /* elements a scale: 32, 64, 128, or 0: the whole row */
-  uint64_t capacity;      /* slots */
+  uint64_t capacity;      /* slots, at most 2^32 - 1 */
   void *codes;            /* capacity * RowBytes, 16-byte aligned */
   float *scales;          /* capacity * RowScales, 4-byte aligned (NULL for NATIVE) */
 } RSGPU_RowCache;

@@ -756,7 +756,7 @@ void FlatIndex::cache_rows(size_t row_begin, size_t n, const RowCacheArgs &cache
   HIP_CHECK(hipSetDevice(device));
   if (row_begin > n_rows_ || n > n_rows_ - row_begin) throw std::runtime_error("cache_rows: range beyond the stored rows");
   if (!n) return;
-  launch_row_write(cache, d_rows_ + row_begin * stride_, stride_ / type_size(type), slots, (uint32_t)n, wstream_);
+  launch_row_write(cache, d_rows_ + row_begin * stride_, (uint32_t)(stride_ / type_size(type)), slots, (uint32_t)n, wstream_);
   HIP_CHECK(hipStreamSynchronize(wstream_));
 }
 
@@ -769,7 +769,7 @@ int FlatIndex::add_cached_rows(const RowCacheArgs &cache, const int64_t *slots, 
   grow((size_t)n_rows_ + n);
   uint8_t *dst = d_rows_ + (size_t)n_rows_ * stride_;
   if (stride_ != elem_bytes_) HIP_CHECK(hipMemsetAsync(dst, 0, n * stride_, wstream_));
-  launch_row_read(cache, slots, (uint32_t)n, dst, stride_ / type_size(type), wstream_);
+  launch_row_read(cache, slots, (uint32_t)n, dst, (uint32_t)(stride_ / type_size(type)), wstream_);
   commit_bulk_rows(n, first_label);
   return (int)n;
 }

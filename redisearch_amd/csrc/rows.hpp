@@ -43,8 +43,8 @@ struct AdjustArgs {
 // throws std::runtime_error on anything that is not served
 RowCacheArgs check_row_cache(const RSGPU_RowCache *c);
 
-void launch_row_write(const RowCacheArgs &c, const void *rows, size_t stride, const int64_t *slots, uint32_t n, hipStream_t s);
-void launch_row_read(const RowCacheArgs &c, const int64_t *slots, uint32_t n, void *out, size_t stride, hipStream_t s);
+void launch_row_write(const RowCacheArgs &c, const void *rows, uint32_t stride, const int64_t *slots, uint32_t n, hipStream_t s);
+void launch_row_read(const RowCacheArgs &c, const int64_t *slots, uint32_t n, void *out, uint32_t stride, hipStream_t s);
 void launch_partition_scores(const PartitionArgs &a, hipStream_t s);
 void launch_adjust_scores(const AdjustArgs &a, hipStream_t s);
 

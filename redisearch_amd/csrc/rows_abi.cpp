@@ -85,7 +85,7 @@ RowCacheArgs check_row_cache(const RSGPU_RowCache *c) {
   need(bytes != 0, "cache: type FLOAT32 / FLOAT16 / BFLOAT16, dim 1 .. 65536, format NATIVE (block 0) / INT8 / E4M3 / INT4, block 0 / 32 / 64 / 128");
   need(c->codes && c->capacity && aligned(c->codes, 16), "cache: codes are capacity > 0 rows, 16-byte aligned");
   need(c->format == RSGPU_ROWS_NATIVE || (c->scales && aligned(c->scales, 4)), "cache: scales are fp32, 4-byte aligned");
-  need(c->capacity <= (uint64_t)1 << 48, "cache: capacity");
+  need(c->capacity <= UINT32_MAX, "cache: at most 2^32 - 1 slots");
   RowCacheArgs a;
   a.codes = static_cast<uint8_t *>(c->codes);
   a.scales = c->scales;
@@ -111,10 +111,10 @@ int RSGPU_RowCache_Write(const RSGPU_RowCache *cache, const void *rows, size_t s
     if (!n) return 0;
     need(rows && slots, "rows or slots are NULL");
     need(n <= MOST, "at most 2^31 - 1 rows a call");
-    need(stride >= c.dim && stride <= SIZE_MAX / 8 / n, "stride: elements from row to row, at least dim");
+    need(stride >= c.dim && stride <= MOST, "stride: elements from row to row, dim .. 2^31 - 1");
     need(aligned(rows, type_size((VecSimType)c.type)) && aligned(slots, 8), "rows or slots are not aligned to their elements");
     OnDevice on(cache->device, c.codes);
-    launch_row_write(c, rows, stride, slots, (uint32_t)n, (hipStream_t)stream);
+    launch_row_write(c, rows, (uint32_t)stride, slots, (uint32_t)n, (hipStream_t)stream);
     return 0;
   });
 }
@@ -125,10 +125,10 @@ int RSGPU_RowCache_Read(const RSGPU_RowCache *cache, const int64_t *slots, size_
     if (!n) return 0;
     need(rows_out && slots, "rows_out or slots are NULL");
     need(n <= MOST, "at most 2^31 - 1 rows a call");
-    need(stride >= c.dim && stride <= SIZE_MAX / 8 / n, "stride: elements from row to row, at least dim");
+    need(stride >= c.dim && stride <= MOST, "stride: elements from row to row, dim .. 2^31 - 1");
     need(aligned(rows_out, type_size((VecSimType)c.type)) && aligned(slots, 8), "rows_out or slots are not aligned to their elements");
     OnDevice on(cache->device, c.codes);
-    launch_row_read(c, slots, (uint32_t)n, rows_out, stride, (hipStream_t)stream);
+    launch_row_read(c, slots, (uint32_t)n, rows_out, (uint32_t)stride, (hipStream_t)stream);
     return 0;
   });
 }

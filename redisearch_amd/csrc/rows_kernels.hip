@@ -47,13 +47,14 @@ __device__ __forceinline__ float f16_to_f32(uint32_t low16) {
   return (float)x;
 }
 
-// eight elements as they are in memory; those from `valid` on are zeros and not read
+// eight elements as they are in memory; those from `valid` on are zeros.  They are read all the same where `more` says that the
+// memory goes on behind them (another row follows)
 template <int T>
 struct Raw8 {
   u4 w[elem_size<T> / 2];
 
-  __device__ __forceinline__ void load(const void *row, uint32_t at, uint32_t valid) {
-    if (valid >= 8) {
+  __device__ __forceinline__ void load(const void *row, uint32_t at, uint32_t valid, bool more = false) {
+    if (valid >= 8 || (more && valid)) {
       if constexpr (T == F32) {
         const u4_any4 *p = reinterpret_cast<const u4_any4 *>(static_cast<const float *>(row) + at);
         w[0] = p[0];
@@ -63,14 +64,27 @@ struct Raw8 {
       }
       return;
     }
-#pragma unroll
-    for (int i = 0; i < (int)(elem_size<T> / 2); i++) w[i] = u4{0, 0, 0, 0};
+    zero();
+    if (!valid) return;
 #pragma unroll
     for (int i = 0; i < 8; i++)
       if ((uint32_t)i < valid) {
         if constexpr (T == F32) w[i / 4][i % 4] = static_cast<const uint32_t *>(row)[at + i];
         else w[0][i / 2] |= (uint32_t)static_cast<const uint16_t *>(row)[at + i] << (16 * (i % 2));
       }
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < (int)(elem_size<T> / 2); i++) w[i] = u4{0, 0, 0, 0};
+  }
+  // what was read behind the row's end is not of the row
+  __device__ __forceinline__ void cut(uint32_t valid) {
+    if (valid >= 8) return;
+#pragma unroll
+    for (int i = 0; i < 2 * (int)elem_size<T>; i++) {
+      if constexpr (T == F32) w[i / 4][i % 4] = (uint32_t)i < valid ? w[i / 4][i % 4] : 0;
+      else w[0][i] &= (uint32_t)(2 * i + 1) < valid ? 0xffffffffu : (uint32_t)(2 * i) < valid ? 0xffffu : 0;
+    }
   }
   __device__ __forceinline__ void floats(float (&v)[8]) const {
 #pragma unroll
@@ -203,12 +217,14 @@ __device__ __forceinline__ uint32_t most_of_lanes(uint32_t x) {
 
 // blocks of 8 L elements: L neighbouring lanes have a block, eight elements each; a thread has several of them under way
 template <int T, int FMT, int L>
-__global__ __launch_bounds__(256) void row_write_kernel(RowCacheArgs c, const void *rows, size_t stride, const int64_t *slots, uint32_t n,
+__global__ __launch_bounds__(256) void row_write_kernel(RowCacheArgs c, const void *rows, uint32_t stride, const int64_t *slots, uint32_t n,
                                                         uint32_t rows_per_wg, FastDiv chunks) {
   constexpr int U = 4;
   const uint32_t padded = rows_padded(c.dim);
+  const uint64_t row_stride = (uint64_t)stride * elem_size<T>;
   for (uint64_t first = (uint64_t)blockIdx.x * rows_per_wg; first < n; first += (uint64_t)gridDim.x * rows_per_wg) {
     const uint32_t mine = n - first < rows_per_wg ? (uint32_t)(n - first) : rows_per_wg;
+    const uint8_t *from = static_cast<const uint8_t *>(rows) + first * row_stride;
     for (uint32_t i0 = threadIdx.x; i0 < mine * chunks.d; i0 += 256 * U) {
       int64_t slot[U];
       uint32_t chunk[U];
@@ -219,13 +235,14 @@ __global__ __launch_bounds__(256) void row_write_kernel(RowCacheArgs c, const vo
         const bool in = i < mine * chunks.d;
         chunk[u] = i - r * chunks.d;
         slot[u] = in ? slots[first + r] : -1;
-        const void *row = static_cast<const uint8_t *>(rows) + (size_t)(first + r) * stride * elem_size<T>;
         const uint32_t at = chunk[u] * 8;
-        raw[u].load(row, at, in && at < c.dim ? c.dim - at : 0);
+        raw[u].load(from + (uint64_t)r * row_stride, at, in && at < c.dim ? c.dim - at : 0, first + r + 1 < n);
       }
 #pragma unroll
       for (int u = 0; u < U; u++) {
         float v[8];
+        const uint32_t at = chunk[u] * 8;
+        raw[u].cut(at < c.dim ? c.dim - at : 0);
         raw[u].floats(v);
         const uint32_t most = most_of_lanes<L>(most8(v));
         float s, inv;
@@ -233,8 +250,9 @@ __global__ __launch_bounds__(256) void row_write_kernel(RowCacheArgs c, const vo
         uint32_t code[2];
         encode8<FMT>(v, s, inv, code);
         if (slot[u] >= 0 && (uint64_t)slot[u] < c.capacity) {
-          if (chunk[u] * 8 < padded) store_codes8<FMT>(c.codes + (size_t)slot[u] * c.row_bytes, chunk[u], code);
-          if (chunk[u] % L == 0) c.scales[(size_t)slot[u] * c.nb + chunk[u] / L] = s;
+          const uint32_t to = (uint32_t)slot[u];
+          if (at < padded) store_codes8<FMT>(c.codes + (uint64_t)to * c.row_bytes, chunk[u], code);
+          if (chunk[u] % L == 0) c.scales[(uint64_t)to * c.nb + chunk[u] / L] = s;
         }
       }
     }
@@ -243,7 +261,7 @@ __global__ __launch_bounds__(256) void row_write_kernel(RowCacheArgs c, const vo
 
 // one scale a row: a wavefront has a row, and reads it again (from the caches) once its largest magnitude is known
 template <int T, int FMT>
-__global__ __launch_bounds__(256) void row_write_whole_kernel(RowCacheArgs c, const void *rows, size_t stride, const int64_t *slots, uint32_t n) {
+__global__ __launch_bounds__(256) void row_write_whole_kernel(RowCacheArgs c, const void *rows, uint32_t stride, const int64_t *slots, uint32_t n) {
   const uint32_t lane = threadIdx.x % 64;
   for (uint64_t r = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64; r < n; r += (uint64_t)gridDim.x * 4) {
     const int64_t slot = slots[r];
@@ -272,7 +290,7 @@ __global__ __launch_bounds__(256) void row_write_whole_kernel(RowCacheArgs c, co
 
 // rows kept as they are: sixteen bytes a thread
 template <int T>
-__global__ __launch_bounds__(256) void row_copy_in_kernel(RowCacheArgs c, const void *rows, size_t stride, const int64_t *slots, uint32_t n,
+__global__ __launch_bounds__(256) void row_copy_in_kernel(RowCacheArgs c, const void *rows, uint32_t stride, const int64_t *slots, uint32_t n,
                                                           uint32_t rows_per_wg, FastDiv chunks) {
   constexpr int E = 16 / elem_size<T>;
   for (uint64_t first = (uint64_t)blockIdx.x * rows_per_wg; first < n; first += (uint64_t)gridDim.x * rows_per_wg) {
@@ -346,11 +364,13 @@ __device__ __forceinline__ uint32_t narrow2(float a, float b) {
 
 // sixteen bytes of output a thread, neighbouring threads' next to each other; a thread has several under way
 template <int T, int FMT>
-__global__ __launch_bounds__(256) void row_read_kernel(RowCacheArgs c, const int64_t *slots, uint32_t n, void *out, size_t stride,
+__global__ __launch_bounds__(256) void row_read_kernel(RowCacheArgs c, const int64_t *slots, uint32_t n, void *out, uint32_t stride,
                                                        uint32_t rows_per_wg, FastDiv chunks, FastDiv block) {
   constexpr int U = 4, E = 16 / elem_size<T>;
   for (uint64_t first = (uint64_t)blockIdx.x * rows_per_wg; first < n; first += (uint64_t)gridDim.x * rows_per_wg) {
     const uint32_t mine = n - first < rows_per_wg ? (uint32_t)(n - first) : rows_per_wg, all = mine * chunks.d;
+    const uint64_t row_stride = (uint64_t)stride * elem_size<T>;
+    uint8_t *to = static_cast<uint8_t *>(out) + first * row_stride;
     for (uint32_t i0 = threadIdx.x; i0 < all; i0 += 256 * U) {
       uint32_t row[U], at[U], codes[U][2];
       int64_t slot[U];
@@ -366,7 +386,7 @@ __global__ __launch_bounds__(256) void row_read_kernel(RowCacheArgs c, const int
 #pragma unroll
       for (int u = 0; u < U; u++) {
         const bool there = slot[u] >= 0 && (uint64_t)slot[u] < c.capacity;
-        const size_t from = there ? (size_t)slot[u] : 0;   // one that is not there is read from slot 0 and zeroed
+        const uint64_t from = there ? (uint32_t)slot[u] : 0;   // one that is not there is read from slot 0 and zeroed
         const uint8_t *p = c.codes + from * c.row_bytes;
         if constexpr (FMT == NATIVE) {
           as_is[u] = *reinterpret_cast<const u4 *>(p + at[u] * elem_size<T>);
@@ -401,7 +421,7 @@ __global__ __launch_bounds__(256) void row_read_kernel(RowCacheArgs c, const int
             else w[k] = narrow2<T>(v[2 * k], v[2 * k + 1]);
           }
         }
-        uint8_t *dst = static_cast<uint8_t *>(out) + ((size_t)(first + row[u]) * stride + at[u]) * elem_size<T>;
+        uint8_t *dst = to + (uint64_t)row[u] * row_stride + at[u] * elem_size<T>;
         if (at[u] + E <= c.dim) {
           if constexpr (T == F32) *reinterpret_cast<u4_any4 *>(dst) = w;
           else *reinterpret_cast<u4_any *>(dst) = w;
@@ -714,7 +734,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
   const auto slot_of = [&](uint32_t j, int32_t id, bool &there) {
     const uint64_t slot = (uint64_t)(uint32_t)id * page.d + (j - page.div(j) * page.d);
     there = id >= 0 && slot < a.c.capacity;
-    return there ? slot : 0;
+    return (uint64_t)(uint32_t)(there ? slot : 0);
   };
 
   // Three tiles: `now` is multiplied, `held` is in registers or LDS (its rows in `source`), the pages of `coming` are looked up.
@@ -971,7 +991,7 @@ __global__ __launch_bounds__(256, FMT == NATIVE && Q == F32 ? 1 : 2) void partit
   const auto slot_of = [&](uint32_t j, int32_t id, bool &there) {
     const uint64_t slot = (uint64_t)(uint32_t)id * page.d + (j - page.div(j) * page.d);
     there = id >= 0 && slot < a.c.capacity;
-    return there ? slot : 0;   // one that is not there is read from slot 0 and not used
+    return (uint64_t)(uint32_t)(there ? slot : 0);   // one that is not there is read from slot 0 and not used
   };
   // the place of eight elements (number c of the stage) of row r in an operand of plane p
   const auto place = [](uint32_t c, uint32_t planes, uint32_t p, uint32_t r) {
@@ -1329,7 +1349,7 @@ uint32_t rows_a_workgroup(uint32_t n, uint32_t chunks) {
 }
 
 template <int T, int FMT>
-void write_as(const RowCacheArgs &c, const void *rows, size_t stride, const int64_t *slots, uint32_t n, hipStream_t s) {
+void write_as(const RowCacheArgs &c, const void *rows, uint32_t stride, const int64_t *slots, uint32_t n, hipStream_t s) {
   if (c.block != 32 && c.block != 64 && c.block != 128) {
     hipLaunchKernelGGL((row_write_whole_kernel<T, FMT>), dim3(workgroups(((uint64_t)n + 3) / 4)), dim3(256), 0, s, c, rows, stride, slots, n);
     return;
@@ -1343,7 +1363,7 @@ void write_as(const RowCacheArgs &c, const void *rows, size_t stride, const int6
 }
 
 template <int T>
-void write_from(const RowCacheArgs &c, const void *rows, size_t stride, const int64_t *slots, uint32_t n, hipStream_t s) {
+void write_from(const RowCacheArgs &c, const void *rows, uint32_t stride, const int64_t *slots, uint32_t n, hipStream_t s) {
   switch (c.format) {
     case INT8: return write_as<T, INT8>(c, rows, stride, slots, n, s);
     case E4M3: return write_as<T, E4M3>(c, rows, stride, slots, n, s);
@@ -1356,7 +1376,7 @@ void write_from(const RowCacheArgs &c, const void *rows, size_t stride, const in
 }
 
 template <int T>
-void read_to(const RowCacheArgs &c, const int64_t *slots, uint32_t n, void *out, size_t stride, hipStream_t s) {
+void read_to(const RowCacheArgs &c, const int64_t *slots, uint32_t n, void *out, uint32_t stride, hipStream_t s) {
   constexpr uint32_t E = 16 / elem_size<T>;
   const uint32_t chunks = (c.dim + E - 1) / E, per = rows_a_workgroup(n, chunks);
   const dim3 grid(workgroups(((uint64_t)n + per - 1) / per));
@@ -1435,14 +1455,14 @@ void scores_from(const PartitionArgs &a, hipStream_t s) {
 
 }  // namespace
 
-void launch_row_write(const RowCacheArgs &c, const void *rows, size_t stride, const int64_t *slots, uint32_t n, hipStream_t s) {
+void launch_row_write(const RowCacheArgs &c, const void *rows, uint32_t stride, const int64_t *slots, uint32_t n, hipStream_t s) {
   if (c.type == F32) write_from<F32>(c, rows, stride, slots, n, s);
   else if (c.type == F16) write_from<F16>(c, rows, stride, slots, n, s);
   else write_from<BF16>(c, rows, stride, slots, n, s);
   HIP_CHECK(hipGetLastError());
 }
 
-void launch_row_read(const RowCacheArgs &c, const int64_t *slots, uint32_t n, void *out, size_t stride, hipStream_t s) {
+void launch_row_read(const RowCacheArgs &c, const int64_t *slots, uint32_t n, void *out, uint32_t stride, hipStream_t s) {
   if (c.type == F32) read_to<F32>(c, slots, n, out, stride, s);
   else if (c.type == F16) read_to<F16>(c, slots, n, out, stride, s);
   else read_to<BF16>(c, slots, n, out, stride, s);
