@@ -227,7 +227,7 @@ __global__ __launch_bounds__(256) void row_write_kernel(RowCacheArgs c, const vo
     const uint8_t *from = static_cast<const uint8_t *>(rows) + first * row_stride;
     for (uint32_t i0 = threadIdx.x; i0 < mine * chunks.d; i0 += 256 * U) {
       int64_t slot[U];
-      uint32_t chunk[U];
+      uint32_t chunk[U], row[U];
       Raw8<T> raw[U];
 #pragma unroll
       for (int u = 0; u < U; u++) {
@@ -235,8 +235,13 @@ __global__ __launch_bounds__(256) void row_write_kernel(RowCacheArgs c, const vo
         const bool in = i < mine * chunks.d;
         chunk[u] = i - r * chunks.d;
         slot[u] = in ? slots[first + r] : -1;
+        row[u] = r;
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++) {   // a row that is left out is not read
         const uint32_t at = chunk[u] * 8;
-        raw[u].load(from + (uint64_t)r * row_stride, at, in && at < c.dim ? c.dim - at : 0, first + r + 1 < n);
+        const bool there = slot[u] >= 0 && (uint64_t)slot[u] < c.capacity;
+        raw[u].load(from + (uint64_t)row[u] * row_stride, at, there && at < c.dim ? c.dim - at : 0, first + row[u] + 1 < n);
       }
 #pragma unroll
       for (int u = 0; u < U; u++) {
