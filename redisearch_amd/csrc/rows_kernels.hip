@@ -969,191 +969,137 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
 }
 
 // Many queries a partition: the matrix cores' work.  A workgroup has a run of tiles of 128 queries x 128 rows, a wavefront 64 x 64 of
-// each; both sides go through LDS in stages of KC elements as operands of the 32 x 32 x 16 product, the rows' codes widened once on
-// the way there.  One stage is multiplied while the next one, of this tile or the next, is on its way in registers.  In LDS an
-// operand's 32 rows change places with the number of its eight elements, so that neither side meets a bank twice.  A block's
-// products are summed by themselves and multiplied by the row's scale at every FLUSH elements.
+// each; both sides go through LDS as operands of the 32 x 32 x 16 product, the rows' codes widened once on the way there.  A stage is
+// 64 elements in two halves: one half is multiplied, the next is in the other half of LDS, and the two behind it are on their way in
+// registers, of this tile or the next one's (with one on its way every half waited for memory: 132 us instead of the figure at the
+// launch below).  In LDS an operand's 32 rows change places with the number of its eight elements, so that neither side meets a bank
+// twice.  A block's products are summed by themselves and multiplied by the row's scale at every FLUSH elements.
+// rows of a tile: 128 queries meet 256 rows where the sums of a tile are all that the registers hold
+template <int FMT, int Q>
+constexpr int MANY_ROWS = FMT == NATIVE && Q != F32 ? 256 : 128;
 template <int FMT, int Q, int FLUSH>
 __global__ __launch_bounds__(256, FMT == NATIVE && Q == F32 ? 1 : 2) void partition_many_kernel(PartitionArgs a, FastDiv page) {
-  constexpr int T = 128, KC = Q == F32 ? 32 : 64, QP = Q == F32 ? 3 : 1, RP = FMT == NATIVE && Q == F32 ? 3 : 1;
-  constexpr int C8 = KC / 8;                                                 // eights of a stage
+  constexpr int TQ = 128, TR = MANY_ROWS<FMT, Q>, X = TR / 64, Y = 2, KC = 32, QP = Q == F32 ? 3 : 1, RP = FMT == NATIVE && Q == F32 ? 3 : 1;
+  constexpr int C8 = KC / 8;                                                 // eights of a half
   constexpr int PIECE = FMT == NATIVE ? 8 : FMT == INT4 ? 32 : 16;           // elements of a row that a thread loads together
   constexpr int PIECE_BYTES = FMT == NATIVE ? 8 * elem_size<Q> : 16, PU = PIECE_BYTES / 16;
-  constexpr int NP = KC / PIECE, RT = (T * NP + 255) / 256;                  // pieces of a row in a stage, of a thread
-  constexpr int QU = Q == F32 ? 2 : 1, QN = T * C8 / 256;                    // 16 bytes of eight elements of a query, eights of a thread
-  static_assert(FLUSH == 32 || FLUSH == KC, "");
+  constexpr int NP = KC / PIECE, RT = (TR * NP + 255) / 256;                  // pieces of a row in a half, of a thread
+  constexpr int QU = Q == F32 ? 2 : 1, QN = TQ * C8 / 256;                    // 16 bytes of eight elements of a query, eights of a thread
   typedef Piece<FMT, Q, PIECE> P;
-  __shared__ u4 q_lds[2][KC / 16 * QP * 4 * 64], r_lds[2][KC / 16 * RP * 4 * 64];
-  __shared__ float s_lds[2][2][T];
+  __shared__ u4 q_lds[2][KC / 16 * QP * TQ * 2], r_lds[2][KC / 16 * RP * TR * 2];
+  __shared__ float s_lds[2][TR];
   __shared__ RunShared run_shared;
 
-  const uint32_t tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), col = lane % 32, half = lane / 32;
-  const Run run = find_run<256, true>(a, T, T, run_shared);
+  const uint32_t tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), col = lane % 32, half_wave = lane / 32;
+  const Run run = find_run<256, true>(a, TQ, TR, run_shared);
   if (run.tiles == 0) return;
-  Place at = run.at;
-  const uint32_t padded = rows_padded(a.c.dim), stages = (padded + KC - 1) / KC;
+  const uint32_t padded = rows_padded(a.c.dim), stages = (padded + 2 * KC - 1) / (2 * KC);
   const float gone = a.form == RSGPU_SCORES_DISTANCE ? __builtin_inff() : -__builtin_inff();
   const auto slot_of = [&](uint32_t j, int32_t id, bool &there) {
     const uint64_t slot = (uint64_t)(uint32_t)id * page.d + (j - page.div(j) * page.d);
     there = id >= 0 && slot < a.c.capacity;
     return (uint64_t)(uint32_t)(there ? slot : 0);   // one that is not there is read from slot 0 and not used
   };
-  // the place of eight elements (number c of the stage) of row r in an operand of plane p
-  const auto place = [](uint32_t c, uint32_t planes, uint32_t p, uint32_t r) {
-    return ((c / 2 * planes + p) * 4 + r / 32) * 64 + c % 2 * 32 + (r % 32 ^ c * (8 / C8));
+  // the place of eight elements (number c of the half) of row r in an operand of plane p
+  const auto place = [](uint32_t rows, uint32_t c, uint32_t planes, uint32_t p, uint32_t r) {
+    return ((c / 2 * planes + p) * (rows / 32) + r / 32) * 64 + c % 2 * 32 + (r % 32 ^ c * (8 / C8));
   };
-
   struct Tile {
     uint32_t g, q0, q_end, n, j0;
   };
-  Tile now = {}, held = {}, coming = {};
-  uint32_t there = 0, held_there = 0;
-  // thread: piece i is of row (i * 256 + tid) / NP, eight i of query (i * 256 + tid) / C8; its scale is row tid % 128's
-  int32_t id[RT], col_id[2], scale_id;
+  const auto take = [&](Place &at) {
+    uint32_t query_tiles = (at.m + TQ - 1) / TQ, tiles = query_tiles * ((at.n + TR - 1) / TR);
+    while (at.left >= tiles) {   // behind this partition's last tile
+      at.g++;
+      at.left -= tiles;
+      partition_of_all(a, at.g, at.lo, at.m, at.n);
+      query_tiles = (at.m + TQ - 1) / TQ;
+      tiles = query_tiles * ((at.n + TR - 1) / TR);
+    }
+    const uint32_t row_tile = at.left / query_tiles;
+    const Tile t = {at.g, at.lo + (at.left - row_tile * query_tiles) * TQ, at.lo + at.m, at.n, row_tile * TR};
+    at.left += run.stride;
+    return t;
+  };
+  // page of row j (of a row behind the partition's last: of its first, whose scores are not written)
+  const auto page_of = [&](const Tile &t, uint32_t j) { return a.pages[(size_t)t.g * a.max_pages + (j < t.n ? page.div(j) : 0)]; };
+
+  // ---- the loads: `loading` is the tile they are at, the pages of `coming` are looked up.  Piece i of a thread is of row
+  // (i * 256 + tid) / NP, eight i of query (i * 256 + tid) / C8; its scale is row tid % TR's
+  Place load_at = run.at;
+  uint32_t loads_taken = 1, load_stage = 0;
+  Tile loading = {}, coming = take(load_at);
+  int32_t id[RT], scale_id;
   const uint8_t *source[RT], *queries[QN];
   const float *scale_source;
-  u4 row_held[RT][PU], query_held[QN][QU];
-  float scale_held;
-  uint32_t taken = 0, load_stage = stages, use_stage = 0;
-  const int64_t rounds = (int64_t)run.tiles * stages;
-  const uint32_t wave_q = wave / 2 * 64, wave_r = wave % 2 * 64;
-  f32x16 acc[2][2];
+  const auto look_up = [&]() {
 #pragma unroll
-  for (int x = 0; x < 2; x++)
+    for (int i = 0; i < RT; i++) id[i] = page_of(coming, coming.j0 + (i * 256 + tid) / NP % TR);
+    if (FMT != NATIVE) scale_id = page_of(coming, coming.j0 + tid % TR);
+  };
+  // on to the tile whose pages are known (behind the run's last tile: that one again)
+  const auto next_tile = [&]() {
+    loading = coming;
+    bool is;
 #pragma unroll
-    for (int y = 0; y < 2; y++)
-#pragma unroll
-      for (int r = 0; r < 16; r++) acc[x][y][r] = 0.0f;
-
-  for (int64_t round = -2; round < rounds; round++) {
-    if (load_stage == stages) {
-      // the tile whose pages are known is loaded from now on (behind the run's last tile: that one again)
-      load_stage = 0;
-      held = coming;
-      held_there = 0;
-      bool is;
-#pragma unroll
-      for (int i = 0; i < RT; i++) source[i] = a.c.codes + slot_of(held.j0 + (i * 256 + tid) / NP % T, round == -2 ? -1 : id[i], is) * a.c.row_bytes;
-#pragma unroll
-      for (int y = 0; y < 2; y++) {
-        slot_of(held.j0 + wave_r + y * 32 + col, round == -2 ? -1 : col_id[y], is);
-        held_there |= is ? 1u << y : 0;
-      }
-      if (FMT != NATIVE) scale_source = a.c.scales + slot_of(held.j0 + tid % T, round == -2 ? -1 : scale_id, is) * a.c.nb;
-#pragma unroll
-      for (int i = 0; i < QN; i++) {
-        const uint32_t q = held.q0 + (i * 256 + tid) / C8;   // of a query behind the partition's last: the last's, not used
-        queries[i] = static_cast<const uint8_t *>(a.queries) + (size_t)(q < held.q_end ? q : held.q_end ? held.q_end - 1 : 0) * a.stride * elem_size<Q>;
-      }
-      if (taken < run.tiles) {
-        uint32_t query_tiles = (at.m + T - 1) / T, tiles = query_tiles * ((at.n + T - 1) / T);
-        while (at.left >= tiles) {   // behind this partition's last tile
-          at.g++;
-          at.left -= tiles;
-          partition_of_all(a, at.g, at.lo, at.m, at.n);
-          query_tiles = (at.m + T - 1) / T;
-          tiles = query_tiles * ((at.n + T - 1) / T);
-        }
-        const uint32_t row_tile = at.left / query_tiles;
-        coming = Tile{at.g, at.lo + (at.left - row_tile * query_tiles) * T, at.lo + at.m, at.n, row_tile * T};
-        at.left += run.stride;
-        taken++;
-      }
-      // page of row j (of a row behind the partition's last: of its first, whose scores are not written)
-      const int32_t *pages = a.pages + (size_t)coming.g * a.max_pages;
-      const auto page_of = [&](uint32_t j) { return pages[j < coming.n ? page.div(j) : 0]; };
-#pragma unroll
-      for (int i = 0; i < RT; i++) id[i] = page_of(coming.j0 + (i * 256 + tid) / NP % T);
-#pragma unroll
-      for (int y = 0; y < 2; y++) col_id[y] = page_of(coming.j0 + wave_r + y * 32 + col);
-      if (FMT != NATIVE) scale_id = page_of(coming.j0 + tid % T);
-      if (round == -2) {
-        load_stage = stages;
-        continue;
-      }
-    }
-
-    // a stage under way
-    const uint32_t base = load_stage * KC;
-#pragma unroll
-    for (int i = 0; i < RT; i++) {
-      const uint32_t e = base + tid % NP * PIECE;
-      const u4 *p = reinterpret_cast<const u4 *>(source[i] + (e < padded ? e : 0) / PIECE * PIECE_BYTES);
-#pragma unroll
-      for (int u = 0; u < PU; u++) row_held[i][u] = p[u];
-    }
-    if (FMT != NATIVE) {
-      const uint32_t b = (base + (FLUSH == KC ? 0 : tid / T * 32)) / a.c.block;
-      scale_held = scale_source[b < a.c.nb ? b : a.c.nb - 1];
-    }
-    // (an eight that the query's end cuts is loaded from where it is whole, and moved below; rows of less than eight elements do
-    // not come here)
-    const uint32_t query_at = base + tid % C8 * 8, query_from = query_at + 8 <= a.c.dim ? query_at : a.c.dim - 8;
+    for (int i = 0; i < RT; i++) source[i] = a.c.codes + slot_of(loading.j0 + (i * 256 + tid) / NP % TR, id[i], is) * a.c.row_bytes;
+    if (FMT != NATIVE) scale_source = a.c.scales + slot_of(loading.j0 + tid % TR, scale_id, is) * a.c.nb;
 #pragma unroll
     for (int i = 0; i < QN; i++) {
-      const uint8_t *p = queries[i] + (size_t)query_from * elem_size<Q>;
+      const uint32_t q = loading.q0 + (i * 256 + tid) / C8;   // of a query behind the partition's last: the last's, not used
+      queries[i] = static_cast<const uint8_t *>(a.queries) + (size_t)(q < loading.q_end ? q : loading.q_end - 1) * a.stride * elem_size<Q>;
+    }
+    if (loads_taken < run.tiles) {
+      coming = take(load_at);
+      loads_taken++;
+    }
+    look_up();
+  };
+  u4 row_held[2][RT][PU], query_held[2][QN][QU];
+  float scale_held[2];
+  uint32_t held_base[2];
+  const auto load = [&](auto which) {
+    constexpr int H = decltype(which)::value;
+    const uint32_t base = held_base[H] = (load_stage * 2 + H) * KC, e = base + tid % NP * PIECE;
+#pragma unroll
+    for (int i = 0; i < RT; i++) {
+      const u4 *p = reinterpret_cast<const u4 *>(source[i] + (e < padded ? e : 0) / PIECE * PIECE_BYTES);
+#pragma unroll
+      for (int u = 0; u < PU; u++) row_held[H][i][u] = p[u];
+    }
+    if (FMT != NATIVE) {
+      const uint32_t b = base / a.c.block;
+      scale_held[H] = scale_source[b < a.c.nb ? b : a.c.nb - 1];
+    }
+    // an eight that the query's end cuts is loaded from where it is whole, and moved below (rows of less than eight elements do not
+    // come here)
+    const uint32_t at = base + tid % C8 * 8;
+#pragma unroll
+    for (int i = 0; i < QN; i++) {
+      const uint8_t *p = queries[i] + (size_t)(at + 8 <= a.c.dim ? at : a.c.dim - 8) * elem_size<Q>;
       if constexpr (Q == F32) {
-        query_held[i][0] = reinterpret_cast<const u4_any4 *>(p)[0];
-        query_held[i][1] = reinterpret_cast<const u4_any4 *>(p)[1];
+        query_held[H][i][0] = reinterpret_cast<const u4_any4 *>(p)[0];
+        query_held[H][i][1] = reinterpret_cast<const u4_any4 *>(p)[1];
       } else {
-        query_held[i][0] = *reinterpret_cast<const u4_any *>(p);
+        query_held[H][i][0] = *reinterpret_cast<const u4_any *>(p);
       }
     }
-    load_stage++;
-
-    if (round >= 0) {
-      const u4 *q_at = q_lds[round & 1], *r_at = r_lds[round & 1];
-#pragma unroll
-      for (int k0 = 0; k0 < KC / 16; k0 += FLUSH / 16) {
-        f32x16 part[2][2];
-#pragma unroll
-        for (int x = 0; x < 2; x++)
-#pragma unroll
-          for (int y = 0; y < 2; y++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) part[x][y][r] = FMT == NATIVE ? acc[x][y][r] : 0.0f;
-#pragma unroll
-        for (int k = k0; k < k0 + FLUSH / 16; k++) {
-          u4 q[2][QP], r[2][RP];
-#pragma unroll
-          for (int x = 0; x < 2; x++) {
-#pragma unroll
-            for (int p = 0; p < QP; p++) q[x][p] = q_at[place(2 * k + half, QP, p, wave_q + x * 32 + col)];
-#pragma unroll
-            for (int p = 0; p < RP; p++) r[x][p] = r_at[place(2 * k + half, RP, p, wave_r + x * 32 + col)];
-          }
-#pragma unroll
-          for (int p = QP - 1; p >= 0; p--)   // the smallest first
-#pragma unroll
-            for (int c = RP - 1; c >= 0; c--)
-              if (p + c < 3) {   // the planes left out are below 2^-24 of the product
-#pragma unroll
-                for (int x = 0; x < 2; x++)
-#pragma unroll
-                  for (int y = 0; y < 2; y++) part[x][y] = mfma<Q>(q[x][p], r[y][c], part[x][y]);
-              }
-        }
-#pragma unroll
-        for (int y = 0; y < 2; y++) {
-          const float scale = FMT == NATIVE ? 1.0f : s_lds[round & 1][FLUSH == KC ? 0 : k0 / 2][wave_r + y * 32 + col];
-#pragma unroll
-          for (int x = 0; x < 2; x++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) acc[x][y][r] = FMT == NATIVE ? part[x][y][r] : __builtin_fmaf(scale, part[x][y][r], acc[x][y][r]);
-        }
-      }
-      use_stage++;
+    if (H == 1 && ++load_stage == stages) {
+      load_stage = 0;
+      next_tile();
     }
-
-    // the stage under way into the other half of LDS, which nobody has read since the last barrier
-    u4 *q_to = q_lds[(round + 1) & 1], *r_to = r_lds[(round + 1) & 1];
-    if (base + KC > a.c.dim) {   // the row's end is in it: zeros behind it
-      const uint32_t by = query_at - query_from;
+  };
+  // a half in registers into its half of LDS, which nobody has read since the last barrier
+  const auto put = [&](auto which) {
+    constexpr int H = decltype(which)::value;
+    const uint32_t base = held_base[H];
+    if (base + KC > a.c.dim) {   // the row's end is in it or before it: zeros behind it
+      const uint32_t at = base + tid % C8 * 8, by = at - (at + 8 <= a.c.dim ? at : a.c.dim - 8);
 #pragma unroll
       for (int i = 0; i < QN; i++) {
         uint32_t v[4 * QU];
 #pragma unroll
-        for (int k = 0; k < 4 * QU; k++) v[k] = by < 8 ? query_held[i][k / 4][k % 4] : 0;
+        for (int k = 0; k < 4 * QU; k++) v[k] = by < 8 ? query_held[H][i][k / 4][k % 4] : 0;
 #pragma unroll
         for (int m = 4; m >= 1; m /= 2) {
           const bool move = by & m;
@@ -1165,13 +1111,13 @@ __global__ __launch_bounds__(256, FMT == NATIVE && Q == F32 ? 1 : 2) void partit
           }
         }
 #pragma unroll
-        for (int k = 0; k < 4 * QU; k++) query_held[i][k / 4][k % 4] = v[k];
+        for (int k = 0; k < 4 * QU; k++) query_held[H][i][k / 4][k % 4] = v[k];
       }
       if (FMT == NATIVE) {
 #pragma unroll
         for (int i = 0; i < RT; i++)
 #pragma unroll
-          for (int k = 0; k < 4 * PU; k++) row_held[i][k / 4][k % 4] = base + tid % NP * PIECE < padded ? row_held[i][k / 4][k % 4] : 0;
+          for (int k = 0; k < 4 * PU; k++) row_held[H][i][k / 4][k % 4] = base + tid % NP * PIECE < padded ? row_held[H][i][k / 4][k % 4] : 0;
       }
     }
 #pragma unroll
@@ -1180,62 +1126,170 @@ __global__ __launch_bounds__(256, FMT == NATIVE && Q == F32 ? 1 : 2) void partit
       if constexpr (Q == F32) {
         float v[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = __uint_as_float(query_held[i][k / 4][k % 4]);
+        for (int k = 0; k < 8; k++) v[k] = __uint_as_float(query_held[H][i][k / 4][k % 4]);
         planes8(v, w);
       } else {
-        w[0] = query_held[i][0];
+        w[0] = query_held[H][i][0];
       }
 #pragma unroll
-      for (int p = 0; p < QP; p++) q_to[place(tid % C8, QP, p, (i * 256 + tid) / C8)] = w[p];
+      for (int p = 0; p < QP; p++) q_lds[H][place(TQ, tid % C8, QP, p, (i * 256 + tid) / C8)] = w[p];
     }
 #pragma unroll
     for (int i = 0; i < RT; i++) {
-      if (T * NP < 256 && tid >= (uint32_t)(T * NP)) break;
+      if (TR * NP < 256 && tid >= (uint32_t)(TR * NP)) break;
       P piece;
 #pragma unroll
-      for (int k = 0; k < PIECE_BYTES / 4; k++) piece.raw[k] = row_held[i][k / 4][k % 4];
+      for (int k = 0; k < PIECE_BYTES / 4; k++) piece.raw[k] = row_held[H][i][k / 4][k % 4];
 #pragma unroll
       for (int f = 0; f < PIECE / 8; f++) {
         u4 w[RP];
         piece.fragment(f, w);
 #pragma unroll
-        for (int p = 0; p < RP; p++) r_to[place(tid % NP * (PIECE / 8) + f, RP, p, (i * 256 + tid) / NP)] = w[p];
+        for (int p = 0; p < RP; p++) r_lds[H][place(TR, tid % NP * (PIECE / 8) + f, RP, p, (i * 256 + tid) / NP)] = w[p];
       }
     }
-    if (FMT != NATIVE) s_lds[(round + 1) & 1][tid / T][tid % T] = scale_held;
-    __syncthreads();
+    if (FMT != NATIVE && tid < TR) s_lds[H][tid] = scale_held[H];
+  };
 
-    if (use_stage == stages) {
+  // ---- the products
+  const uint32_t wave_q = X == 2 ? wave / 2 * 64 : 0, wave_r = X == 2 ? wave % 2 * 64 : wave * 64;
+  f32x16 acc[X][Y], part[X][Y];
 #pragma unroll
-      for (int y = 0; y < 2; y++) {
-        const uint32_t j = now.j0 + wave_r + y * 32 + col;
+  for (int x = 0; x < X; x++)
 #pragma unroll
-        for (int x = 0; x < 2; x++)
+    for (int y = 0; y < Y; y++)
 #pragma unroll
-          for (int r = 0; r < 16; r++) {
-            const uint32_t q = now.q0 + wave_q + x * 32 + 8 * (r / 4) + 4 * half + r % 4;
-            float p = acc[x][y][r] * CODE_UNIT<FMT, Q>;
-            acc[x][y][r] = 0.0f;
-            if (j < now.n && q < now.q_end) {
-              if constexpr (FMT == NATIVE && Q == F32) {
-                // an infinity meets the other side's planes, some of them 0: the sum is taken again, element by element
-                if (p != p && (there >> y & 1)) {
-                  bool is;
-                  const uint64_t slot = slot_of(j, a.pages[(size_t)now.g * a.max_pages + page.div(j)], is);
-                  p = plain_product(reinterpret_cast<const float *>(a.c.codes + slot * a.c.row_bytes), static_cast<const float *>(a.queries) + q * a.stride, a.c.dim);
-                }
-              }
-              if (a.form == RSGPU_SCORES_DISTANCE) p = 1.0f - p;
-              a.scores[(size_t)q * a.ld + j] = there >> y & 1 ? p : gone;
-            }
+      for (int r = 0; r < 16; r++) acc[x][y][r] = 0.0f;
+  const auto multiply = [&](auto which) {
+    constexpr int H = decltype(which)::value;
+    if (FMT != NATIVE && (H == 0 || FLUSH == KC)) {
+#pragma unroll
+      for (int x = 0; x < X; x++)
+#pragma unroll
+        for (int y = 0; y < Y; y++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) part[x][y][r] = 0.0f;
+    }
+    f32x16(&sum)[X][Y] = FMT == NATIVE ? acc : part;
+#pragma unroll
+    for (int k = 0; k < KC / 16; k++) {
+      u4 q[X][QP], r[Y][RP];
+#pragma unroll
+      for (int y = 0; y < Y; y++)
+#pragma unroll
+        for (int p = 0; p < RP; p++) r[y][p] = r_lds[H][place(TR, 2 * k + half_wave, RP, p, wave_r + y * 32 + col)];
+#pragma unroll
+      for (int x = 0; x < X; x++)
+#pragma unroll
+        for (int p = 0; p < QP; p++) q[x][p] = q_lds[H][place(TQ, 2 * k + half_wave, QP, p, wave_q + x * 32 + col)];
+#pragma unroll
+      for (int p = QP - 1; p >= 0; p--)   // the smallest first
+#pragma unroll
+        for (int c = RP - 1; c >= 0; c--)
+          if (p + c < 3) {   // the planes left out are below 2^-24 of the product
+#pragma unroll
+            for (int x = 0; x < X; x++)
+#pragma unroll
+              for (int y = 0; y < Y; y++) sum[x][y] = mfma<Q>(q[x][p], r[y][c], sum[x][y]);
           }
+    }
+    if (FMT != NATIVE && (H == 1 || FLUSH == KC)) {
+#pragma unroll
+      for (int y = 0; y < Y; y++) {
+        const float scale = s_lds[H][wave_r + y * 32 + col];
+#pragma unroll
+        for (int x = 0; x < X; x++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) acc[x][y][r] = __builtin_fmaf(scale, part[x][y][r], acc[x][y][r]);
       }
-      use_stage = 0;
     }
-    if (use_stage == 0) {
-      now = held;
-      there = held_there;
+  };
+
+  // ---- the scores, an eighth of a wavefront's at a time
+  const auto write = [&](auto which, const Tile &t, uint32_t there, const auto &sums) {
+    constexpr int W = decltype(which)::value, x = W / 4, y = W / 2 % 2, R = W % 2 * 8;
+    const uint32_t j = t.j0 + wave_r + y * 32 + col;
+    float *at = a.scores + j;
+    if (j >= t.n) return;
+#pragma unroll
+    for (int r = R; r < R + 8; r++) {
+      const uint32_t q = t.q0 + wave_q + x * 32 + 8 * (r / 4) + 4 * half_wave + r % 4;
+      if (q >= t.q_end) continue;
+      float p = sums[x][y][r] * CODE_UNIT<FMT, Q>;
+      if constexpr (FMT == NATIVE && Q == F32) {
+        // an infinity meets the other side's planes, some of them 0: the sum is taken again, element by element
+        if (p != p && (there >> y & 1)) {
+          bool is;
+          const uint64_t slot = slot_of(j, page_of(t, j), is);
+          p = plain_product(reinterpret_cast<const float *>(a.c.codes + slot * a.c.row_bytes), static_cast<const float *>(a.queries) + q * a.stride, a.c.dim);
+        }
+      }
+      if (a.form == RSGPU_SCORES_DISTANCE) p = 1.0f - p;
+      __builtin_nontemporal_store(there >> y & 1 ? p : gone, at + (uint64_t)q * a.ld);
     }
+  };
+  const std::integral_constant<int, 0> first_half;
+  const std::integral_constant<int, 1> second_half;
+  look_up();
+  next_tile();
+  load(first_half);
+  load(second_half);
+  Place use_at = run.at;
+  Tile now = take(use_at);
+  int32_t col_id[2];
+#pragma unroll
+  for (int y = 0; y < Y; y++) col_id[y] = page_of(now, now.j0 + wave_r + y * 32 + col);
+  put(first_half);
+  load(first_half);
+  __syncthreads();
+  uint32_t use_stage = 0, used = 0;
+  for (;;) {
+    multiply(first_half);
+    put(second_half);
+    load(second_half);
+    __syncthreads();
+    multiply(second_half);
+    put(first_half);
+    load(first_half);
+    __syncthreads();
+    if (++use_stage < stages) continue;
+
+    uint32_t there = 0;
+#pragma unroll
+    for (int y = 0; y < Y; y++) {
+      bool is;
+      slot_of(now.j0 + wave_r + y * 32 + col, col_id[y], is);
+      there |= is ? 1u << y : 0;
+    }
+    write(std::integral_constant<int, 0>(), now, there, acc);
+    write(std::integral_constant<int, 1>(), now, there, acc);
+    write(std::integral_constant<int, 2>(), now, there, acc);
+    write(std::integral_constant<int, 3>(), now, there, acc);
+    write(std::integral_constant<int, 4>(), now, there, acc);
+    write(std::integral_constant<int, 5>(), now, there, acc);
+    write(std::integral_constant<int, 6>(), now, there, acc);
+    write(std::integral_constant<int, 7>(), now, there, acc);
+    if constexpr (X == 4) {
+      write(std::integral_constant<int, 8>(), now, there, acc);
+      write(std::integral_constant<int, 9>(), now, there, acc);
+      write(std::integral_constant<int, 10>(), now, there, acc);
+      write(std::integral_constant<int, 11>(), now, there, acc);
+      write(std::integral_constant<int, 12>(), now, there, acc);
+      write(std::integral_constant<int, 13>(), now, there, acc);
+      write(std::integral_constant<int, 14>(), now, there, acc);
+      write(std::integral_constant<int, 15>(), now, there, acc);
+    }
+#pragma unroll
+    for (int x = 0; x < X; x++)
+#pragma unroll
+      for (int y = 0; y < Y; y++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[x][y][r] = 0.0f;
+    if (++used == run.tiles) break;
+    use_stage = 0;
+    now = take(use_at);
+#pragma unroll
+    for (int y = 0; y < Y; y++) col_id[y] = page_of(now, now.j0 + wave_r + y * 32 + col);
   }
 }
 
@@ -1415,15 +1469,13 @@ void scores_as(const PartitionArgs &a, hipStream_t s) {
   };
   if (each >= 48 && a.c.dim >= 8) {
     const auto many = [&](auto kernel) {
-      dim3 g = grid(128, 128, resident(reinterpret_cast<const void *>(kernel), 256));
+      dim3 g = grid(128, MANY_ROWS<FMT, Q>, resident(reinterpret_cast<const void *>(kernel), 256));
       g.x = (g.x + DIES - 1) / DIES * DIES;
       hipLaunchKernelGGL(kernel, g, dim3(256), 0, s, a, page);
     };
-    if (FMT != NATIVE && Q != F32 && a.c.block == 32) {
-      if constexpr (FMT != NATIVE) many(partition_many_kernel<FMT, Q, 32>);
-    } else {
-      many(partition_many_kernel<FMT, Q, Q == F32 ? 32 : 64>);
-    }
+    if constexpr (FMT == NATIVE) many(partition_many_kernel<FMT, Q, 64>);
+    else if (a.c.block == 32) many(partition_many_kernel<FMT, Q, 32>);
+    else many(partition_many_kernel<FMT, Q, 64>);
     return;
   }
   // the rows' chunks of a stage: the number that leaves the fewest places empty, the largest of those
