@@ -1162,14 +1162,7 @@ __global__ __launch_bounds__(256, FMT == NATIVE && Q == F32 ? 1 : 2) void partit
       for (int r = 0; r < 16; r++) acc[x][y][r] = 0.0f;
   const auto multiply = [&](auto which) {
     constexpr int H = decltype(which)::value;
-    if (FMT != NATIVE && (H == 0 || FLUSH == KC)) {
-#pragma unroll
-      for (int x = 0; x < X; x++)
-#pragma unroll
-        for (int y = 0; y < Y; y++)
-#pragma unroll
-          for (int r = 0; r < 16; r++) part[x][y][r] = 0.0f;
-    }
+    constexpr bool FRESH = FMT != NATIVE && (H == 0 || FLUSH == KC);   // a block's sums begin
     f32x16(&sum)[X][Y] = FMT == NATIVE ? acc : part;
 #pragma unroll
     for (int k = 0; k < KC / 16; k++) {
@@ -1190,7 +1183,10 @@ __global__ __launch_bounds__(256, FMT == NATIVE && Q == F32 ? 1 : 2) void partit
 #pragma unroll
             for (int x = 0; x < X; x++)
 #pragma unroll
-              for (int y = 0; y < Y; y++) sum[x][y] = mfma<Q>(q[x][p], r[y][c], sum[x][y]);
+              for (int y = 0; y < Y; y++) {
+                const f32x16 none = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+                sum[x][y] = mfma<Q>(q[x][p], r[y][c], FRESH && k == 0 && p == QP - 1 ? none : sum[x][y]);   // (one plane of rows there)
+              }
           }
     }
     if (FMT != NATIVE && (H == 1 || FLUSH == KC)) {
@@ -1201,6 +1197,12 @@ __global__ __launch_bounds__(256, FMT == NATIVE && Q == F32 ? 1 : 2) void partit
         for (int x = 0; x < X; x++)
 #pragma unroll
           for (int r = 0; r < 16; r++) acc[x][y][r] = __builtin_fmaf(scale, part[x][y][r], acc[x][y][r]);
+      }
+      if (FLUSH == KC) {   // here and not with the next half's, whose sums take part's registers
+#pragma unroll
+        for (int x = 0; x < X; x++)
+#pragma unroll
+          for (int y = 0; y < Y; y++) asm volatile("" : "+v"(acc[x][y]));
       }
     }
   };
