@@ -24,7 +24,7 @@ COMMON = ["-O3", "-std=c++17", "-fPIC", "-I" + os.path.join(ROOT, "include"), "-
 
 # library name -> sources
 LIBS = {
-    "libVectorSimilarity.so": ["scan_kernels.hip", "scan_mq_kernels.hip", "select_kernels.hip", "gemm_kernels.hip", "gemm_qs_kernels.hip", "fusion_kernels.hip", "postings_kernels.hip", "hybrid_kernels.hip", "corpus_kernels.hip", "exchange_kernels.hip", "rows_kernels.hip",
+    "libVectorSimilarity.so": ["scan_kernels.hip", "scan_mq_kernels.hip", "select_kernels.hip", "gemm_kernels.hip", "gemm_qs_kernels.hip", "fusion_kernels.hip", "postings_kernels.hip", "hybrid_kernels.hip", "corpus_kernels.hip", "exchange_kernels.hip", "rows_kernels.hip", "partition_f32.hip", "partition_f16.hip", "partition_bf16.hip",
                                "flat_index.cpp", "label_table.cpp", "grow_buffer.cpp", "batch_query.cpp", "sharded_index.cpp", "shard_comm.cpp", "vecsim_abi.cpp", "search_abi.cpp", "rows_abi.cpp"],
 }
 
@@ -40,7 +40,9 @@ def _deps_mtime():
 
 # per-source extra flags: the scorers must not contract a*b+c behind the C source's back
 # (packed fp32 instructions are left out of the row cache's kernels: some of their forms are not reliable on this hardware)
-EXTRA = {"rows_kernels.hip": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"],
+_NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+EXTRA = {"rows_kernels.hip": _NO_PACKED_FP32, "partition_f32.hip": _NO_PACKED_FP32, "partition_f16.hip": _NO_PACKED_FP32,
+         "partition_bf16.hip": _NO_PACKED_FP32,
          "postings_kernels.hip": ["-ffp-contract=off"], "hybrid_kernels.hip": ["-ffp-contract=off"], "fusion_kernels.hip": ["-ffp-contract=off"]}
 
 

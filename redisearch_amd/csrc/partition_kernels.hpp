@@ -1,0 +1,933 @@
+// partition_kernels.hpp -- the products of ragged groups of queries with the paged rows of their partitions (include/rsgpu_rows.h) on
+// gfx950.  Included by one source file for each type of queries, partition_{f32,f16,bf16}.hip, which compile side by side.
+#pragma once
+#include <type_traits>
+
+#include "rows_device.hpp"
+
+namespace rsgpu {
+namespace {
+
+// ---- products with a partition's rows --------------------------------------------------------------------------------------
+//
+// p[m][j] = sum_k q[m][k] c[j][k] s[j][k / block].  The codes are integers or e4m3 values that a 16-bit float holds exactly, so the
+// matrix cores multiply codes with queries, and a block's sum is multiplied by its scale in fp32: no operand is rounded.
+// fp32 operands go in as three bf16 each (8 + 8 + 8 bits of the significand, cut off exactly).
+
+template <int Q>
+__device__ __forceinline__ f32x16 mfma(u4 a, u4 b, f32x16 c) {
+  if constexpr (Q == F16) {
+    half8 x, y;
+    __builtin_memcpy(&x, &a, 16);
+    __builtin_memcpy(&y, &b, 16);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0);
+  } else {
+    bf16x8 x, y;
+    __builtin_memcpy(&x, &a, 16);
+    __builtin_memcpy(&y, &b, 16);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
+  }
+}
+
+template <int Q>
+__device__ __forceinline__ f32x4 mfma16(u4 a, u4 b, f32x4 c) {
+  if constexpr (Q == F16) {
+    half8 x, y;
+    __builtin_memcpy(&x, &a, 16);
+    __builtin_memcpy(&y, &b, 16);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0);
+  } else {
+    bf16x8 x, y;
+    __builtin_memcpy(&x, &a, 16);
+    __builtin_memcpy(&y, &b, 16);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0);
+  }
+}
+
+// x = hi + mid + lo, each a bf16 in the upper half of its dword.  An infinity or a NaN is hi alone.
+__device__ __forceinline__ void split3(uint32_t x, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
+  const bool special = (x & 0x7f800000u) == 0x7f800000u;
+  hi = (x & 0xffff0000u) | (special && (x & 0xffffu) ? 0x400000u : 0);   // a NaN whose payload sits in the bits cut off stays one
+  const float r = special ? 0.0f : __uint_as_float(x) - __uint_as_float(hi);
+  mid = __float_as_uint(r) & 0xffff0000u;
+  lo = __float_as_uint(r - __uint_as_float(mid));
+}
+__device__ __forceinline__ uint32_t upper2(uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
+
+// eight fp32 -> eight bf16 in each of three planes
+__device__ __forceinline__ void planes8(const float (&v)[8], u4 (&p)[3]) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    uint32_t a[3], b[3];
+    split3(__float_as_uint(v[2 * i]), a[0], a[1], a[2]);
+    split3(__float_as_uint(v[2 * i + 1]), b[0], b[1], b[2]);
+#pragma unroll
+    for (int k = 0; k < 3; k++) p[k][i] = upper2(a[k], b[k]);
+  }
+}
+
+// eight codes -> eight 16-bit floats (INT4 with bf16: sixteenths of the codes, CODE_UNIT)
+template <int FMT, int Q>
+constexpr float CODE_UNIT = FMT == INT4 && Q != F16 ? 16.0f : 1.0f;
+
+__device__ __forceinline__ uint32_t minus2(uint32_t x, float y) {
+  half2v h;
+  __builtin_memcpy(&h, &x, 4);
+  h -= half2v{(_Float16)y, (_Float16)y};
+  __builtin_memcpy(&x, &h, 4);
+  return x;
+}
+
+template <int FMT, int Q>
+__device__ __forceinline__ u4 widen8(uint32_t w0, uint32_t w1) {
+  u4 r;
+  if constexpr (FMT == E4M3) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int w = (int)(i < 2 ? w0 : w1);
+      if constexpr (Q == F16) {
+        const half2v h = i % 2 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false);
+        uint32_t x;
+        __builtin_memcpy(&x, &h, 4);
+        r[i] = x;
+      } else {
+        const bf16x2 h = i % 2 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false);
+        uint32_t x;
+        __builtin_memcpy(&x, &h, 4);
+        r[i] = x;
+      }
+    }
+  } else if constexpr (Q == F16) {
+    // an fp16 number in [1024, 2048) has its integer in the low bits: 1024 + (code + bias), and the bias goes off exactly
+    if constexpr (FMT == INT8) {
+      const uint32_t a = w0 ^ 0x80808080u, b = w1 ^ 0x80808080u;
+      r = u4{minus2(__builtin_amdgcn_perm(0x64646464u, a, 0x04010400u), 1152.0f), minus2(__builtin_amdgcn_perm(0x64646464u, a, 0x04030402u), 1152.0f),
+             minus2(__builtin_amdgcn_perm(0x64646464u, b, 0x04010400u), 1152.0f), minus2(__builtin_amdgcn_perm(0x64646464u, b, 0x04030402u), 1152.0f)};
+    } else {
+      const uint32_t t = w0 ^ 0x88888888u, even = t & 0x0f0f0f0fu, odd = t >> 4 & 0x0f0f0f0fu;
+#pragma unroll
+      for (int i = 0; i < 4; i++) r[i] = minus2(__builtin_amdgcn_perm(odd, even, 0x0c040c00u + 0x00010001u * i) | 0x64006400u, 1032.0f);
+    }
+  } else {
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      if constexpr (FMT == INT8) f[i] = (float)(int8_t)((i < 4 ? w0 : w1) >> (8 * (i % 4)));
+      else f[i] = __builtin_amdgcn_cvt_off_f32_i4((int)(w0 >> (4 * i)));   // the low four bits, two's complement, by 16
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) r[i] = upper2(__float_as_uint(f[2 * i]), __float_as_uint(f[2 * i + 1]));
+  }
+  return r;
+}
+
+// queries [lo, lo + m) and rows of partition g
+__device__ __forceinline__ void partition(const PartitionArgs &a, uint32_t g, uint32_t &lo, uint32_t &m, uint32_t &n) {
+  const int32_t from = cut(a.query_offsets[g], (int32_t)a.n_queries), to = cut(a.query_offsets[g + 1], (int32_t)a.n_queries);
+  lo = (uint32_t)from;
+  m = to > from ? (uint32_t)(to - from) : 0;
+  n = (uint32_t)cut(a.row_counts[g], (int32_t)a.most_rows);
+}
+
+__device__ __noinline__ float plain_product(const float *row, const float *query, uint32_t dim) {
+  float p = 0.0f;
+  for (uint32_t k = 0; k < dim; k++) p = __builtin_fmaf(query[k], row[k], p);
+  return p;
+}
+
+// A workgroup's run of tiles, and where its first one is: the partition, that partition's queries and rows, the tile's number in it
+struct Place {
+  uint32_t g, lo, m, n, left;
+};
+struct Run {
+  uint32_t tiles, stride;
+  Place at;
+};
+struct RunShared {
+  uint32_t wave_sums[16];
+  Place at;
+};
+// The offsets and counts are on the device, so every workgroup sums the partitions' tiles itself, a share of the partitions a
+// thread, takes its even part of them, and the thread in whose share that begins says where.  TOGETHER: an eighth of the tiles, one
+// after the other, is for the workgroups b, b + 8, ... that share a die's L2, and they go through it side by side.
+constexpr uint32_t DIES = 8;
+template <int THREADS, bool TOGETHER>
+__device__ __forceinline__ Run find_run(const PartitionArgs &a, uint32_t tq, uint32_t tr, RunShared &shared) {
+  const uint32_t tid = threadIdx.x, lane = tid % 64, per = (a.n_partitions + THREADS - 1) / THREADS;
+  uint32_t own = 0;
+  for (uint32_t i = 0; i < per; i++) {
+    const uint32_t g = tid * per + i;
+    if (g >= a.n_partitions) break;
+    uint32_t lo, m, n;
+    partition(a, g, lo, m, n);
+    own += (m + tq - 1) / tq * ((n + tr - 1) / tr);
+  }
+  uint32_t sum = own;
+#pragma unroll
+  for (int k = 1; k < 64; k *= 2) {
+    const uint32_t v = __shfl_up(sum, k, 64);
+    if (lane >= (uint32_t)k) sum += v;
+  }
+  if (lane == 63) shared.wave_sums[tid / 64] = sum;
+  __syncthreads();
+  uint32_t total = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < THREADS / 64; w++) {
+    const uint32_t v = shared.wave_sums[w];
+    if (w < tid / 64) sum += v;
+    total += v;
+  }
+  Run run;
+  uint32_t first;
+  if (TOGETHER) {
+    const uint32_t die = blockIdx.x % DIES, from = (uint32_t)((uint64_t)total * die / DIES), to = (uint32_t)((uint64_t)total * (die + 1) / DIES);
+    run.stride = gridDim.x / DIES;   // a multiple of the dies
+    first = from + blockIdx.x / DIES;
+    run.tiles = first < to ? (to - first + run.stride - 1) / run.stride : 0;
+  } else {
+    run.stride = 1;
+    first = (uint32_t)((uint64_t)total * blockIdx.x / gridDim.x);
+    run.tiles = (uint32_t)((uint64_t)total * (blockIdx.x + 1) / gridDim.x) - first;
+  }
+  if (run.tiles == 0) return run;
+  if (sum - own <= first && first < sum) {
+    Place p;
+    p.left = first - (sum - own);
+    for (p.g = tid * per;; p.g++) {
+      partition(a, p.g, p.lo, p.m, p.n);
+      const uint32_t tiles = (p.m + tq - 1) / tq * ((p.n + tr - 1) / tr);
+      if (p.left < tiles) break;
+      p.left -= tiles;
+    }
+    shared.at = p;
+  }
+  __syncthreads();
+  run.at.g = __builtin_amdgcn_readfirstlane(shared.at.g);
+  run.at.lo = __builtin_amdgcn_readfirstlane(shared.at.lo);
+  run.at.m = __builtin_amdgcn_readfirstlane(shared.at.m);
+  run.at.n = __builtin_amdgcn_readfirstlane(shared.at.n);
+  run.at.left = __builtin_amdgcn_readfirstlane(shared.at.left);
+  return run;
+}
+
+// eight elements of a query as 16-bit fragments (an fp32 query: three planes)
+template <int Q>
+__device__ __forceinline__ void stage8(const PartitionArgs &a, uint32_t query, uint32_t at, u4 (&w)[Q == F32 ? 3 : 1]) {
+  const uint8_t *src = static_cast<const uint8_t *>(a.queries) + (size_t)query * a.stride * elem_size<Q>;
+  if constexpr (Q == F32) {
+    float v[8];
+    load8<F32>(src, at, at < a.c.dim ? a.c.dim - at : 0, v);
+    planes8(v, w);
+  } else if (at + 8 <= a.c.dim) {
+    w[0] = *reinterpret_cast<const u4_any *>(src + at * 2);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      uint32_t x = 0;
+      if (at + 2 * i < a.c.dim) x = reinterpret_cast<const uint16_t *>(src)[at + 2 * i];
+      if (at + 2 * i + 1 < a.c.dim) x |= (uint32_t)reinterpret_cast<const uint16_t *>(src)[at + 2 * i + 1] << 16;
+      w[0][i] = x;
+    }
+  }
+}
+
+// the same where all lanes ask for one partition: scalar loads
+typedef const __attribute__((address_space(4))) int32_t *scalar_i32;
+__device__ __forceinline__ void partition_of_all(const PartitionArgs &a, uint32_t g, uint32_t &lo, uint32_t &m, uint32_t &n) {
+  const scalar_i32 offsets = (scalar_i32)(uintptr_t)a.query_offsets, counts = (scalar_i32)(uintptr_t)a.row_counts;
+  const int32_t from = cut(offsets[g], (int32_t)a.n_queries), to = cut(offsets[g + 1], (int32_t)a.n_queries);
+  lo = (uint32_t)from;
+  m = to > from ? (uint32_t)(to - from) : 0;
+  n = (uint32_t)cut(counts[g], (int32_t)a.most_rows);
+}
+
+// W neighbouring elements of a row, as a lane takes them from LDS
+template <int FMT, int Q, int W>
+struct Piece {
+  static constexpr int BYTES = FMT == NATIVE ? W * elem_size<Q> : FMT == INT4 ? W / 2 : W;
+  static constexpr int PLANES = FMT == NATIVE && Q == F32 ? 3 : 1;
+  uint32_t raw[BYTES / 4];
+
+  // elements 8 f .. 8 f + 7
+  __device__ __forceinline__ void fragment(int f, u4 (&out)[PLANES]) const {
+    if constexpr (FMT == NATIVE && Q == F32) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = __uint_as_float(raw[i]);
+      planes8(v, out);
+    } else if constexpr (FMT == NATIVE) {
+      out[0] = u4{raw[0], raw[1], raw[2], raw[3]};
+    } else if constexpr (FMT == INT4) {
+      out[0] = widen8<INT4, Q>(raw[f], 0);
+    } else {
+      out[0] = widen8<FMT, Q>(raw[2 * f], raw[2 * f + 1]);
+    }
+  }
+};
+
+// Few queries a partition: the rows' bytes are what it takes.  A workgroup has a run of tiles of 16 queries x 16 S rows a wavefront;
+// the queries of a partition are put into LDS once for all its tiles (in parts of KP stages if the rows are longer than that).
+// A wavefront takes its rows in stages of 4 KiB, 16 S rows x 256 / S bytes: four loads of 16 neighbouring bytes a lane, whole lines of
+// the rows, one stage in registers under way (across tiles too) while the one before is multiplied.  (Loads in the shape of the matrix
+// instruction's operand touch 16 lines each and cost the same whatever they bring: 2.4 TB/s with 8 bytes a lane, 4.6 with 16.)  A stage
+// passes through 4 KiB of LDS that the wavefront has to itself, so nothing but the order of its own instructions guards it, and comes
+// back as operands; the sixteen-byte chunks of a row change places with its number, so that neither side meets a bank twice.
+// ONCE: the rows are read past the caches' keeping (a batch of 256 over 64 partitions: 57 us for 63; with three query tiles a
+// partition, which read the rows three times, 170 for 134).
+// Every part of the loop is in the code once: a small call is mostly the first pass of its instructions through the caches.
+template <int FMT, int Q, int W, int S, int WAVES, bool ONCE>
+__global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionArgs a, FastDiv page) {
+  typedef Piece<FMT, Q, W> P;
+  constexpr int QP = Q == F32 ? 3 : 1, FR = W / 8, TQ = 16, WR = 16 * S, TR = WR * WAVES;
+  constexpr int CS = 16 / S;                                  // chunks of a row in a stage
+  constexpr int SP = CS * 16 / (4 * P::BYTES);                // steps of 4 W elements in a stage
+  constexpr int QS = FMT == NATIVE ? 0 : (SP + 3) / 4;        // scale loads a stage and row group: a lane's quarter has every fourth
+  constexpr int KP = (Q == F32 ? 24 : 32) / (SP * FR);        // stages of queries in LDS at a time: 72 or 32 KiB
+  static_assert(SP >= 1 && KP >= 1, "");
+  __shared__ u4 staged[KP * SP * FR * QP * 64];
+  __shared__ u4 passing[WAVES][256];
+  __shared__ RunShared run_shared;
+
+  const uint32_t tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), col = lane % 16, quarter = lane / 16;
+  const Run run = find_run<64 * WAVES, false>(a, TQ, TR, run_shared);
+  if (run.tiles == 0) return;
+  Place at = run.at;
+  const uint32_t chunks = a.c.row_bytes / 16, stages = (chunks + CS - 1) / CS;
+  // blocks are one step or two, or the row
+  const uint32_t block_shift = a.c.block >= a.c.dim ? 31 : a.c.block / (4 * W) >= 2 ? 1 : 0;
+  const float gone = a.form == RSGPU_SCORES_DISTANCE ? __builtin_inff() : -__builtin_inff();
+
+  struct Tile {
+    uint32_t g, query_tile, q0, q_end, n, j0;   // j0: the first row of this wavefront
+  };
+  // slot of row j in page `id`; one that is not there is read from slot 0 and not used
+  const auto slot_of = [&](uint32_t j, int32_t id, bool &there) {
+    const uint64_t slot = (uint64_t)(uint32_t)id * page.d + (j - page.div(j) * page.d);
+    there = id >= 0 && slot < a.c.capacity;
+    return (uint64_t)(uint32_t)(there ? slot : 0);
+  };
+
+  // Three tiles: `now` is multiplied, `held` is in registers or LDS (its rows in `source`), the pages of `coming` are looked up.
+  // Chunk i of a lane is of row i * 64 / CS + lane / CS of the wavefront.
+  constexpr uint32_t ROWS_A_LOAD = 64 / CS;
+  const uint32_t my_row = lane / CS;
+  Tile now = {}, held = {}, coming = {};
+  uint32_t there = 0, held_there = 0;             // which of the rows 16 k + col are there
+  int32_t id[4], col_id[S];
+  const uint8_t *source[4];
+  const float *scale_source[S];
+  u4 chunk[4];
+  float next_scale[S][QS ? QS : 1], scale[S][QS ? QS : 1];
+  u4 *const mine = passing[wave];
+  f32x4 acc[S];
+#pragma unroll
+  for (int k = 0; k < S; k++) acc[k] = f32x4{0, 0, 0, 0};
+  uint32_t staged_g = ~0u, staged_q = 0, staged_p = 0;   // whose queries are in LDS, from which stage on
+  uint32_t taken = 0;
+  uint32_t use_stage = 0, load_stage = stages;           // stages: on to the next tile before the next load
+  const int64_t rounds = (int64_t)run.tiles * stages;
+
+  for (int64_t round = -2; round < rounds; round++) {
+    if (load_stage == stages) {
+      // the tile whose pages are known is loaded from now on (behind the run's last tile: that one again)
+      load_stage = 0;
+      held = coming;
+      held_there = 0;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        bool is;
+        const uint64_t slot = slot_of(held.j0 + i * ROWS_A_LOAD + my_row, round == -2 ? -1 : id[i], is);
+        source[i] = a.c.codes + slot * a.c.row_bytes;
+      }
+#pragma unroll
+      for (int k = 0; k < S; k++) {
+        bool is;
+        const uint64_t slot = slot_of(held.j0 + k * 16 + col, round == -2 ? -1 : col_id[k], is);
+        held_there |= is ? 1u << k : 0;
+        scale_source[k] = a.c.scales + slot * a.c.nb;
+      }
+      if (taken < run.tiles) {
+        uint32_t row_tiles = (at.n + TR - 1) / TR;
+        while (at.left >= (at.m + TQ - 1) / TQ * row_tiles) {   // behind this partition's last tile
+          at.g++;
+          at.left = 0;
+          partition_of_all(a, at.g, at.lo, at.m, at.n);
+          row_tiles = (at.n + TR - 1) / TR;
+        }
+        const uint32_t query_tile = at.left / row_tiles;
+        coming = Tile{at.g, query_tile, at.lo + query_tile * TQ, at.lo + at.m, at.n, (at.left - query_tile * row_tiles) * TR + wave * WR};
+        at.left++;
+        taken++;
+      }
+      // page of row j (of a row behind the partition's last: of its first, whose scores are not written)
+      const int32_t *pages = a.pages + (size_t)coming.g * a.max_pages;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const uint32_t j = coming.j0 + i * ROWS_A_LOAD + my_row;
+        id[i] = pages[j < coming.n ? page.div(j) : 0];
+      }
+#pragma unroll
+      for (int k = 0; k < S; k++) {
+        const uint32_t j = coming.j0 + k * 16 + col;
+        col_id[k] = pages[j < coming.n ? page.div(j) : 0];
+      }
+      if (round == -2) {
+        load_stage = stages;
+        continue;
+      }
+    }
+
+    // a stage under way
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t row = i * ROWS_A_LOAD + my_row, c = load_stage * CS + (lane % CS ^ (CS == 4 ? row >> 1 & 3 : row & (CS - 1)));
+      const u4 *p = reinterpret_cast<const u4 *>(source[i] + (c < chunks ? c : chunks - 1) * 16);
+      chunk[i] = ONCE ? __builtin_nontemporal_load(p) : *p;
+    }
+#pragma unroll
+    for (int k = 0; k < S; k++)
+#pragma unroll
+      for (int q = 0; q < QS; q++) {
+        const uint32_t b = ((load_stage * SP) >> block_shift) + q * 4 + quarter;
+        next_scale[k][q] = scale_source[k][b < a.c.nb ? b : a.c.nb - 1];
+      }
+    load_stage++;
+
+    if (round >= 0) {
+      // the one in LDS multiplied
+      const u4 *queries = staged + use_stage % KP * (SP * FR * QP * 64) + lane;
+      const uint32_t first_block = (use_stage * SP) >> block_shift;
+      P piece[SP][S];
+#pragma unroll
+      for (int st = 0; st < SP; st++)
+#pragma unroll
+        for (int k = 0; k < S; k++) {
+          const uint32_t row = k * 16 + col, bytes = st * 4 * P::BYTES + quarter * P::BYTES, turn = CS == 4 ? row >> 1 & 3 : row & (CS - 1);
+#pragma unroll
+          for (int e = 0; e < (P::BYTES + 15) / 16; e++) {
+            const uint8_t *p = reinterpret_cast<const uint8_t *>(mine + row * CS + ((bytes / 16 + e) ^ turn)) + bytes % 16;
+            if constexpr (P::BYTES == 4) {
+              piece[st][k].raw[0] = *reinterpret_cast<const uint32_t *>(p);
+            } else if constexpr (P::BYTES == 8) {
+              const u2 w = *reinterpret_cast<const u2 *>(p);
+              piece[st][k].raw[0] = w[0];
+              piece[st][k].raw[1] = w[1];
+            } else {
+              const u4 w = *reinterpret_cast<const u4 *>(p);
+#pragma unroll
+              for (int i = 0; i < 4; i++) piece[st][k].raw[4 * e + i] = w[i];
+            }
+          }
+        }
+#pragma unroll
+      for (int st = 0; st < SP; st++) {
+        f32x4 part[S];
+#pragma unroll
+        for (int k = 0; k < S; k++) part[k] = FMT == NATIVE ? acc[k] : f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int f = 0; f < FR; f++) {
+          u4 q[QP];
+#pragma unroll
+          for (int p = 0; p < QP; p++) q[p] = queries[((st * FR + f) * QP + p) * 64];
+#pragma unroll
+          for (int k = 0; k < S; k++) {
+            u4 b[P::PLANES];
+            piece[st][k].fragment(f, b);
+            if (FMT == NATIVE) {   // behind the row's end its last chunk comes again: an infinity there would meet a zero
+              const bool in = (use_stage * SP + st) * 4 * W + quarter * W < a.c.row_bytes / elem_size<Q>;
+#pragma unroll
+              for (int c = 0; c < P::PLANES; c++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) b[c][e] = in ? b[c][e] : 0;
+            }
+#pragma unroll
+            for (int p = QP - 1; p >= 0; p--)   // the smallest first
+#pragma unroll
+              for (int c = P::PLANES - 1; c >= 0; c--)
+                if (p + c < 3) part[k] = mfma16<Q>(q[p], b[c], part[k]);   // the planes left out are below 2^-24 of the product
+          }
+        }
+        // a step's sum, times the scale of the block that it is in (no branch for the block's end: the steps overlap)
+        const uint32_t block = ((use_stage * SP + st) >> block_shift) - first_block;
+#pragma unroll
+        for (int k = 0; k < S; k++) {
+          if (FMT == NATIVE) {
+            acc[k] = part[k];
+          } else {
+            float v = scale[k][0];
+#pragma unroll
+            for (int q = 1; q < QS; q++) v = block / 4 == (uint32_t)q ? scale[k][q] : v;
+            v = __uint_as_float(__builtin_amdgcn_ds_bpermute((block % 4 * 16 + col) * 4, __float_as_uint(v)));
+#pragma unroll
+            for (int r = 0; r < 4; r++) acc[k][r] = __builtin_fmaf(v, part[k][r], acc[k][r]);
+          }
+        }
+      }
+      use_stage++;
+    }
+
+    // the queries that the next stage meets, if they are not in LDS yet; they and the stage under way come together
+    const bool turned = round < 0 || use_stage == stages;
+    const uint32_t meets_g = turned ? held.g : now.g, meets_q = turned ? held.query_tile : now.query_tile, p0 = turned ? 0 : use_stage / KP * KP;
+    if ((staged_g != meets_g || staged_q != meets_q || staged_p != p0) && round + 1 < rounds) {
+      const uint32_t q0 = turned ? held.q0 : now.q0, q_end = turned ? held.q_end : now.q_end;
+      __syncthreads();
+      const uint32_t np = stages - p0 < KP ? stages - p0 : KP, asked = q_end - q0 < TQ ? q_end - q0 : TQ;
+      const uint32_t shift = asked > 8 ? 4 : asked > 4 ? 3 : asked > 2 ? 2 : asked > 1 ? 1 : 0;
+      for (uint32_t i = tid; i < np * (SP * FR * 4) << shift; i += 64 * WAVES) {
+        const uint32_t q = i & ((1u << shift) - 1), e = i >> shift, f = e % FR, h = e / FR % 4, st = e / (4 * FR);
+        if (q >= asked) continue;   // what is in LDS behind them is multiplied and not used
+        u4 w[QP];
+        stage8<Q>(a, q0 + q, (p0 * SP + st) * (4 * W) + h * W + f * 8, w);
+#pragma unroll
+        for (int p = 0; p < QP; p++) staged[((st * FR + f) * QP + p) * 64 + h * 16 + q] = w[p];
+      }
+      __syncthreads();
+      staged_g = meets_g;
+      staged_q = meets_q;
+      staged_p = p0;
+    }
+
+    // the stage under way into LDS, behind the reads of the one before it
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < 4; i++) mine[i * 64 + lane] = chunk[i];
+#pragma unroll
+    for (int k = 0; k < S; k++)
+#pragma unroll
+      for (int q = 0; q < QS; q++) scale[k][q] = next_scale[k][q];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+
+    if (use_stage == stages) {
+#pragma unroll
+      for (int k = 0; k < S; k++) {
+        const uint32_t j = now.j0 + k * 16 + col;
+        if (j < now.n) {
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const uint32_t q = now.q0 + quarter * 4 + r;
+            if (q < now.q_end) {
+              float p = acc[k][r] * CODE_UNIT<FMT, Q>;
+              if constexpr (FMT == NATIVE && Q == F32) {
+                // an infinity meets the other side's planes, some of them 0: the sum is taken again, element by element
+                if (p != p && (there >> k & 1)) {
+                  bool is;
+                  const uint64_t slot = slot_of(j, a.pages[(size_t)now.g * a.max_pages + page.div(j)], is);
+                  p = plain_product(reinterpret_cast<const float *>(a.c.codes + slot * a.c.row_bytes), static_cast<const float *>(a.queries) + q * a.stride, a.c.dim);
+                }
+              }
+              if (a.form == RSGPU_SCORES_DISTANCE) p = 1.0f - p;
+              a.scores[(size_t)q * a.ld + j] = there >> k & 1 ? p : gone;
+            }
+          }
+        }
+        acc[k] = f32x4{0, 0, 0, 0};
+      }
+      use_stage = 0;
+    }
+    if (use_stage == 0) {
+      now = held;
+      there = held_there;
+    }
+  }
+}
+
+// Many queries a partition: the matrix cores' work.  A workgroup has a run of tiles of 128 queries x 128 rows, a wavefront 64 x 64 of
+// each; both sides go through LDS as operands of the 32 x 32 x 16 product, the rows' codes widened once on the way there.  A stage is
+// 64 elements in two halves: one half is multiplied, the next is in the other half of LDS, and the two behind it are on their way in
+// registers, of this tile or the next one's (with one on its way every half waited for memory: 132 us instead of the figure at the
+// launch below).  In LDS an operand's 32 rows change places with the number of its eight elements, so that neither side meets a bank
+// twice.  A block's products are summed by themselves and multiplied by the row's scale at every FLUSH elements.
+// rows of a tile: 128 queries meet 256 rows where the sums of a tile are all that the registers hold
+template <int FMT, int Q>
+constexpr int MANY_ROWS = FMT == NATIVE && Q != F32 ? 256 : 128;
+template <int FMT, int Q, int FLUSH>
+__global__ __launch_bounds__(256, FMT == NATIVE && Q == F32 ? 1 : 2) void partition_many_kernel(PartitionArgs a, FastDiv page) {
+  constexpr int TQ = 128, TR = MANY_ROWS<FMT, Q>, X = TR / 64, Y = 2, KC = 32, QP = Q == F32 ? 3 : 1, RP = FMT == NATIVE && Q == F32 ? 3 : 1;
+  constexpr int C8 = KC / 8;                                                 // eights of a half
+  constexpr int PIECE = FMT == NATIVE ? 8 : FMT == INT4 ? 32 : 16;           // elements of a row that a thread loads together
+  constexpr int PIECE_BYTES = FMT == NATIVE ? 8 * elem_size<Q> : 16, PU = PIECE_BYTES / 16;
+  constexpr int NP = KC / PIECE, RT = (TR * NP + 255) / 256;                  // pieces of a row in a half, of a thread
+  constexpr int QU = Q == F32 ? 2 : 1, QN = TQ * C8 / 256;                    // 16 bytes of eight elements of a query, eights of a thread
+  typedef Piece<FMT, Q, PIECE> P;
+  __shared__ u4 q_lds[2][KC / 16 * QP * TQ * 2], r_lds[2][KC / 16 * RP * TR * 2];
+  __shared__ float s_lds[2][TR];
+  __shared__ RunShared run_shared;
+
+  const uint32_t tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), col = lane % 32, half_wave = lane / 32;
+  const Run run = find_run<256, true>(a, TQ, TR, run_shared);
+  if (run.tiles == 0) return;
+  const uint32_t padded = rows_padded(a.c.dim), stages = (padded + 2 * KC - 1) / (2 * KC);
+  const float gone = a.form == RSGPU_SCORES_DISTANCE ? __builtin_inff() : -__builtin_inff();
+  const auto slot_of = [&](uint32_t j, int32_t id, bool &there) {
+    const uint64_t slot = (uint64_t)(uint32_t)id * page.d + (j - page.div(j) * page.d);
+    there = id >= 0 && slot < a.c.capacity;
+    return (uint64_t)(uint32_t)(there ? slot : 0);   // one that is not there is read from slot 0 and not used
+  };
+  // the place of eight elements (number c of the half) of row r in an operand of plane p
+  const auto place = [](uint32_t rows, uint32_t c, uint32_t planes, uint32_t p, uint32_t r) {
+    return ((c / 2 * planes + p) * (rows / 32) + r / 32) * 64 + c % 2 * 32 + (r % 32 ^ c * (8 / C8));
+  };
+  struct Tile {
+    uint32_t g, q0, q_end, n, j0;
+  };
+  const auto take = [&](Place &at) {
+    uint32_t query_tiles = (at.m + TQ - 1) / TQ, tiles = query_tiles * ((at.n + TR - 1) / TR);
+    while (at.left >= tiles) {   // behind this partition's last tile
+      at.g++;
+      at.left -= tiles;
+      partition_of_all(a, at.g, at.lo, at.m, at.n);
+      query_tiles = (at.m + TQ - 1) / TQ;
+      tiles = query_tiles * ((at.n + TR - 1) / TR);
+    }
+    const uint32_t row_tile = at.left / query_tiles;
+    const Tile t = {at.g, at.lo + (at.left - row_tile * query_tiles) * TQ, at.lo + at.m, at.n, row_tile * TR};
+    at.left += run.stride;
+    return t;
+  };
+  // page of row j (of a row behind the partition's last: of its first, whose scores are not written)
+  const auto page_of = [&](const Tile &t, uint32_t j) { return a.pages[(size_t)t.g * a.max_pages + (j < t.n ? page.div(j) : 0)]; };
+
+  // ---- the loads: `loading` is the tile they are at, the pages of `coming` are looked up.  Piece i of a thread is of row
+  // (i * 256 + tid) / NP, eight i of query (i * 256 + tid) / C8; its scale is row tid % TR's
+  Place load_at = run.at;
+  uint32_t loads_taken = 1, load_stage = 0;
+  Tile loading = {}, coming = take(load_at);
+  int32_t id[RT], scale_id;
+  const uint8_t *source[RT], *queries[QN];
+  const float *scale_source;
+  const auto look_up = [&]() {
+#pragma unroll
+    for (int i = 0; i < RT; i++) id[i] = page_of(coming, coming.j0 + (i * 256 + tid) / NP % TR);
+    if (FMT != NATIVE) scale_id = page_of(coming, coming.j0 + tid % TR);
+  };
+  // on to the tile whose pages are known (behind the run's last tile: that one again)
+  const auto next_tile = [&]() {
+    loading = coming;
+    bool is;
+#pragma unroll
+    for (int i = 0; i < RT; i++) source[i] = a.c.codes + slot_of(loading.j0 + (i * 256 + tid) / NP % TR, id[i], is) * a.c.row_bytes;
+    if (FMT != NATIVE) scale_source = a.c.scales + slot_of(loading.j0 + tid % TR, scale_id, is) * a.c.nb;
+#pragma unroll
+    for (int i = 0; i < QN; i++) {
+      const uint32_t q = loading.q0 + (i * 256 + tid) / C8;   // of a query behind the partition's last: the last's, not used
+      queries[i] = static_cast<const uint8_t *>(a.queries) + (size_t)(q < loading.q_end ? q : loading.q_end - 1) * a.stride * elem_size<Q>;
+    }
+    if (loads_taken < run.tiles) {
+      coming = take(load_at);
+      loads_taken++;
+    }
+    look_up();
+  };
+  u4 row_held[2][RT][PU], query_held[2][QN][QU];
+  float scale_held[2];
+  uint32_t held_base[2];
+  const auto load = [&](auto which) {
+    constexpr int H = decltype(which)::value;
+    const uint32_t base = held_base[H] = (load_stage * 2 + H) * KC, e = base + tid % NP * PIECE;
+#pragma unroll
+    for (int i = 0; i < RT; i++) {
+      const u4 *p = reinterpret_cast<const u4 *>(source[i] + (e < padded ? e : 0) / PIECE * PIECE_BYTES);
+#pragma unroll
+      for (int u = 0; u < PU; u++) row_held[H][i][u] = p[u];
+    }
+    if (FMT != NATIVE) {
+      const uint32_t b = base / a.c.block;
+      scale_held[H] = scale_source[b < a.c.nb ? b : a.c.nb - 1];
+    }
+    // an eight that the query's end cuts is loaded from where it is whole, and moved below (rows of less than eight elements do not
+    // come here)
+    const uint32_t at = base + tid % C8 * 8;
+#pragma unroll
+    for (int i = 0; i < QN; i++) {
+      const uint8_t *p = queries[i] + (size_t)(at + 8 <= a.c.dim ? at : a.c.dim - 8) * elem_size<Q>;
+      if constexpr (Q == F32) {
+        query_held[H][i][0] = reinterpret_cast<const u4_any4 *>(p)[0];
+        query_held[H][i][1] = reinterpret_cast<const u4_any4 *>(p)[1];
+      } else {
+        query_held[H][i][0] = *reinterpret_cast<const u4_any *>(p);
+      }
+    }
+    if (H == 1 && ++load_stage == stages) {
+      load_stage = 0;
+      next_tile();
+    }
+  };
+  // a half in registers into its half of LDS, which nobody has read since the last barrier
+  const auto put = [&](auto which) {
+    constexpr int H = decltype(which)::value;
+    const uint32_t base = held_base[H];
+    if (base + KC > a.c.dim) {   // the row's end is in it or before it: zeros behind it
+      const uint32_t at = base + tid % C8 * 8, by = at - (at + 8 <= a.c.dim ? at : a.c.dim - 8);
+#pragma unroll
+      for (int i = 0; i < QN; i++) {
+        uint32_t v[4 * QU];
+#pragma unroll
+        for (int k = 0; k < 4 * QU; k++) v[k] = by < 8 ? query_held[H][i][k / 4][k % 4] : 0;
+#pragma unroll
+        for (int m = 4; m >= 1; m /= 2) {
+          const bool move = by & m;
+          const int d = m * elem_size<Q> / 4;
+#pragma unroll
+          for (int k = 0; k < 4 * QU; k++) {
+            const uint32_t next = k + 1 < 4 * QU ? v[k + 1 < 4 * QU ? k + 1 : 0] : 0, far = d && k + d < 4 * QU ? v[k + d < 4 * QU ? k + d : 0] : 0;
+            v[k] = move ? (d ? far : __builtin_amdgcn_alignbit(next, v[k], 16)) : v[k];
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4 * QU; k++) query_held[H][i][k / 4][k % 4] = v[k];
+      }
+      if (FMT == NATIVE) {
+#pragma unroll
+        for (int i = 0; i < RT; i++)
+#pragma unroll
+          for (int k = 0; k < 4 * PU; k++) row_held[H][i][k / 4][k % 4] = base + tid % NP * PIECE < padded ? row_held[H][i][k / 4][k % 4] : 0;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < QN; i++) {
+      u4 w[QP];
+      if constexpr (Q == F32) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = __uint_as_float(query_held[H][i][k / 4][k % 4]);
+        planes8(v, w);
+      } else {
+        w[0] = query_held[H][i][0];
+      }
+#pragma unroll
+      for (int p = 0; p < QP; p++) q_lds[H][place(TQ, tid % C8, QP, p, (i * 256 + tid) / C8)] = w[p];
+    }
+#pragma unroll
+    for (int i = 0; i < RT; i++) {
+      if (TR * NP < 256 && tid >= (uint32_t)(TR * NP)) break;
+      P piece;
+#pragma unroll
+      for (int k = 0; k < PIECE_BYTES / 4; k++) piece.raw[k] = row_held[H][i][k / 4][k % 4];
+#pragma unroll
+      for (int f = 0; f < PIECE / 8; f++) {
+        u4 w[RP];
+        piece.fragment(f, w);
+#pragma unroll
+        for (int p = 0; p < RP; p++) r_lds[H][place(TR, tid % NP * (PIECE / 8) + f, RP, p, (i * 256 + tid) / NP)] = w[p];
+      }
+    }
+    if (FMT != NATIVE && tid < TR) s_lds[H][tid] = scale_held[H];
+  };
+
+  // ---- the products
+  const uint32_t wave_q = X == 2 ? wave / 2 * 64 : 0, wave_r = X == 2 ? wave % 2 * 64 : wave * 64;
+  f32x16 acc[X][Y], part[X][Y];
+#pragma unroll
+  for (int x = 0; x < X; x++)
+#pragma unroll
+    for (int y = 0; y < Y; y++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[x][y][r] = 0.0f;
+  const auto multiply = [&](auto which) {
+    constexpr int H = decltype(which)::value;
+    constexpr bool FRESH = FMT != NATIVE && (H == 0 || FLUSH == KC);   // a block's sums begin
+    f32x16(&sum)[X][Y] = FMT == NATIVE ? acc : part;
+#pragma unroll
+    for (int k = 0; k < KC / 16; k++) {
+      u4 q[X][QP], r[Y][RP];
+#pragma unroll
+      for (int y = 0; y < Y; y++)
+#pragma unroll
+        for (int p = 0; p < RP; p++) r[y][p] = r_lds[H][place(TR, 2 * k + half_wave, RP, p, wave_r + y * 32 + col)];
+#pragma unroll
+      for (int x = 0; x < X; x++)
+#pragma unroll
+        for (int p = 0; p < QP; p++) q[x][p] = q_lds[H][place(TQ, 2 * k + half_wave, QP, p, wave_q + x * 32 + col)];
+#pragma unroll
+      for (int p = QP - 1; p >= 0; p--)   // the smallest first
+#pragma unroll
+        for (int c = RP - 1; c >= 0; c--)
+          if (p + c < 3) {   // the planes left out are below 2^-24 of the product
+#pragma unroll
+            for (int x = 0; x < X; x++)
+#pragma unroll
+              for (int y = 0; y < Y; y++) {
+                const f32x16 none = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+                sum[x][y] = mfma<Q>(q[x][p], r[y][c], FRESH && k == 0 && p == QP - 1 ? none : sum[x][y]);   // (one plane of rows there)
+              }
+          }
+    }
+    if (FMT != NATIVE && (H == 1 || FLUSH == KC)) {
+#pragma unroll
+      for (int y = 0; y < Y; y++) {
+        const float scale = s_lds[H][wave_r + y * 32 + col];
+#pragma unroll
+        for (int x = 0; x < X; x++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) acc[x][y][r] = __builtin_fmaf(scale, part[x][y][r], acc[x][y][r]);
+      }
+      if (FLUSH == KC) {   // here and not with the next half's, whose sums take part's registers
+#pragma unroll
+        for (int x = 0; x < X; x++)
+#pragma unroll
+          for (int y = 0; y < Y; y++) asm volatile("" : "+v"(acc[x][y]));
+      }
+    }
+  };
+
+  // ---- the scores, an eighth of a wavefront's at a time
+  const auto write = [&](auto which, const Tile &t, uint32_t there, const auto &sums) {
+    constexpr int W = decltype(which)::value, x = W / 4, y = W / 2 % 2, R = W % 2 * 8;
+    const uint32_t j = t.j0 + wave_r + y * 32 + col;
+    float *at = a.scores + j;
+    if (j >= t.n) return;
+#pragma unroll
+    for (int r = R; r < R + 8; r++) {
+      const uint32_t q = t.q0 + wave_q + x * 32 + 8 * (r / 4) + 4 * half_wave + r % 4;
+      if (q >= t.q_end) continue;
+      float p = sums[x][y][r] * CODE_UNIT<FMT, Q>;
+      if constexpr (FMT == NATIVE && Q == F32) {
+        // an infinity meets the other side's planes, some of them 0: the sum is taken again, element by element
+        if (p != p && (there >> y & 1)) {
+          bool is;
+          const uint64_t slot = slot_of(j, page_of(t, j), is);
+          p = plain_product(reinterpret_cast<const float *>(a.c.codes + slot * a.c.row_bytes), static_cast<const float *>(a.queries) + q * a.stride, a.c.dim);
+        }
+      }
+      if (a.form == RSGPU_SCORES_DISTANCE) p = 1.0f - p;
+      __builtin_nontemporal_store(there >> y & 1 ? p : gone, at + (uint64_t)q * a.ld);
+    }
+  };
+  const std::integral_constant<int, 0> first_half;
+  const std::integral_constant<int, 1> second_half;
+  look_up();
+  next_tile();
+  load(first_half);
+  load(second_half);
+  Place use_at = run.at;
+  Tile now = take(use_at);
+  int32_t col_id[2];
+#pragma unroll
+  for (int y = 0; y < Y; y++) col_id[y] = page_of(now, now.j0 + wave_r + y * 32 + col);
+  put(first_half);
+  load(first_half);
+  __syncthreads();
+  uint32_t use_stage = 0, used = 0;
+  for (;;) {
+    multiply(first_half);
+    put(second_half);
+    load(second_half);
+    __syncthreads();
+    multiply(second_half);
+    put(first_half);
+    load(first_half);
+    __syncthreads();
+    if (++use_stage < stages) continue;
+
+    uint32_t there = 0;
+#pragma unroll
+    for (int y = 0; y < Y; y++) {
+      bool is;
+      slot_of(now.j0 + wave_r + y * 32 + col, col_id[y], is);
+      there |= is ? 1u << y : 0;
+    }
+    write(std::integral_constant<int, 0>(), now, there, acc);
+    write(std::integral_constant<int, 1>(), now, there, acc);
+    write(std::integral_constant<int, 2>(), now, there, acc);
+    write(std::integral_constant<int, 3>(), now, there, acc);
+    write(std::integral_constant<int, 4>(), now, there, acc);
+    write(std::integral_constant<int, 5>(), now, there, acc);
+    write(std::integral_constant<int, 6>(), now, there, acc);
+    write(std::integral_constant<int, 7>(), now, there, acc);
+    if constexpr (X == 4) {
+      write(std::integral_constant<int, 8>(), now, there, acc);
+      write(std::integral_constant<int, 9>(), now, there, acc);
+      write(std::integral_constant<int, 10>(), now, there, acc);
+      write(std::integral_constant<int, 11>(), now, there, acc);
+      write(std::integral_constant<int, 12>(), now, there, acc);
+      write(std::integral_constant<int, 13>(), now, there, acc);
+      write(std::integral_constant<int, 14>(), now, there, acc);
+      write(std::integral_constant<int, 15>(), now, there, acc);
+    }
+#pragma unroll
+    for (int x = 0; x < X; x++)
+#pragma unroll
+      for (int y = 0; y < Y; y++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[x][y][r] = 0.0f;
+    if (++used == run.tiles) break;
+    use_stage = 0;
+    now = take(use_at);
+#pragma unroll
+    for (int y = 0; y < Y; y++) col_id[y] = page_of(now, now.j0 + wave_r + y * 32 + col);
+  }
+}
+
+// workgroups of a kernel that the device holds at once: kernels that go round give each of them the same share
+uint32_t resident(const void *kernel, uint32_t threads) {
+  int device = 0, units = 0, each = 0;
+  HIP_CHECK(hipGetDevice(&device));
+  HIP_CHECK(hipDeviceGetAttribute(&units, hipDeviceAttributeMultiprocessorCount, device));
+  HIP_CHECK(hipOccupancyMaxActiveBlocksPerMultiprocessor(&each, kernel, (int)threads, 0));
+  return (uint32_t)(units > 0 && each > 0 ? units * each : 256);
+}
+
+template <int FMT, int Q>
+void scores_as(const PartitionArgs &a, hipStream_t s) {
+  const FastDiv page(a.page_rows);
+  const uint32_t asked = a.n_partitions < a.n_queries ? a.n_partitions : a.n_queries;   // partitions with queries, at most
+  const uint32_t each = a.n_queries / a.n_partitions;
+  // no more workgroups than there can be tiles, and no more than are resident at once
+  const auto grid = [&](uint32_t tq, uint32_t tr, uint64_t resident) {
+    const uint64_t tiles = ((uint64_t)a.n_queries / tq + asked) * ((a.most_rows + tr - 1) / tr);
+    return dim3((uint32_t)(tiles < resident ? tiles : resident));
+  };
+  if (each >= 48 && a.c.dim >= 8) {
+    const auto many = [&](auto kernel) {
+      dim3 g = grid(128, MANY_ROWS<FMT, Q>, resident(reinterpret_cast<const void *>(kernel), 256));
+      g.x = (g.x + DIES - 1) / DIES * DIES;
+      hipLaunchKernelGGL(kernel, g, dim3(256), 0, s, a, page);
+    };
+    if constexpr (FMT == NATIVE) many(partition_many_kernel<FMT, Q, 64>);
+    else if (a.c.block == 32) many(partition_many_kernel<FMT, Q, 32>);
+    else many(partition_many_kernel<FMT, Q, 64>);
+    return;
+  }
+  // the rows' chunks of a stage: the number that leaves the fewest places empty, the largest of those
+  const uint32_t chunks = a.c.row_bytes / 16;
+  uint32_t cs = 16;
+  constexpr bool widest = Q == F32;   // an fp32 step is eight chunks, and 64 rows of three planes do not fit into 128 registers
+  for (uint32_t c : {8u, 4u})
+    if (!(widest && c == 4) && (chunks + c - 1) / c * c < (chunks + cs - 1) / cs * cs) cs = c;
+  const auto few = [&](auto w) {
+    constexpr int W = decltype(w)::value, WAVES = Q == F32 ? 16 : 8;
+    const auto launch = [&](auto kernel, uint32_t tr) {
+      hipLaunchKernelGGL(kernel, grid(16, tr, resident(reinterpret_cast<const void *>(kernel), 64 * WAVES)), dim3(64 * WAVES), 0, s, a, page);
+    };
+    // at eight queries a partition hardly one has more than the sixteen of a tile, so that its rows are read once
+    const auto sized = [&](auto once) {
+      constexpr bool ONCE = decltype(once)::value;
+      if (cs == 16) launch(partition_few_kernel<FMT, Q, W, 1, WAVES, ONCE>, 16 * WAVES);
+      else if (cs == 8) launch(partition_few_kernel<FMT, Q, W, 2, WAVES, ONCE>, 32 * WAVES);
+      else if constexpr (!widest) launch(partition_few_kernel<FMT, Q, W, 4, WAVES, ONCE>, 64 * WAVES);
+    };
+    if (each <= 8) sized(std::true_type());
+    else sized(std::false_type());
+  };
+  // a lane's piece of a row: as wide as four of them fit into a block
+  if constexpr (FMT != NATIVE) {
+    if (a.c.block != 32) return few(std::integral_constant<int, 16>());
+  }
+  few(std::integral_constant<int, 8>());
+}
+
+template <int Q>
+void scores_from(const PartitionArgs &a, hipStream_t s) {
+  switch (a.c.format) {
+    case INT8: return scores_as<INT8, Q>(a, s);
+    case E4M3: return scores_as<E4M3, Q>(a, s);
+    case INT4: return scores_as<INT4, Q>(a, s);
+    default: return scores_as<NATIVE, Q>(a, s);
+  }
+}
+
+}  // namespace
+}  // namespace rsgpu

@@ -1,4 +1,4 @@
-// rows.hpp -- launchers of the row cache's kernels (rows_kernels.hip), called by the C entry points in rows_abi.cpp.
+// rows.hpp -- launchers of the row cache's kernels (rows_kernels.hip, partition_kernels.hpp), called by the C entry points in rows_abi.cpp.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -45,7 +45,10 @@ RowCacheArgs check_row_cache(const RSGPU_RowCache *c);
 
 void launch_row_write(const RowCacheArgs &c, const void *rows, uint32_t stride, const int64_t *slots, uint32_t n, hipStream_t s);
 void launch_row_read(const RowCacheArgs &c, const int64_t *slots, uint32_t n, void *out, uint32_t stride, hipStream_t s);
-void launch_partition_scores(const PartitionArgs &a, hipStream_t s);
+// by the type of the queries
+void launch_partition_scores_f32(const PartitionArgs &a, hipStream_t s);
+void launch_partition_scores_f16(const PartitionArgs &a, hipStream_t s);
+void launch_partition_scores_bf16(const PartitionArgs &a, hipStream_t s);
 void launch_adjust_scores(const AdjustArgs &a, hipStream_t s);
 
 }  // namespace rsgpu

@@ -163,7 +163,8 @@ int RSGPU_RowCache_PartitionScores(const RSGPU_RowCache *cache, const void *quer
     a.scores = scores;
     a.ld = ld;
     OnDevice on(cache->device, a.c.codes);
-    launch_partition_scores(a, (hipStream_t)stream);
+    const auto launch = a.c.type == VecSimType_FLOAT32 ? launch_partition_scores_f32 : a.c.type == VecSimType_FLOAT16 ? launch_partition_scores_f16 : launch_partition_scores_bf16;
+    launch(a, (hipStream_t)stream);
     return 0;
   });
 }
