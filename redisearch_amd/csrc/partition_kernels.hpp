@@ -550,7 +550,7 @@ __global__ __launch_bounds__(256, FMT == NATIVE && Q == F32 ? 1 : 2) void partit
   constexpr int PIECE = FMT == NATIVE ? 8 : FMT == INT4 ? 32 : 16;           // elements of a row that a thread loads together
   constexpr int PIECE_BYTES = FMT == NATIVE ? 8 * elem_size<Q> : 16, PU = PIECE_BYTES / 16;
   constexpr int NP = KC / PIECE, RT = (TR * NP + 255) / 256;                  // pieces of a row in a half, of a thread
-  constexpr int QU = Q == F32 ? 2 : 1, QN = TQ * C8 / 256;                    // 16 bytes of eight elements of a query, eights of a thread
+  constexpr int QN = TQ * C8 / 256;                                          // eights of the queries in a half, of a thread
   typedef Piece<FMT, Q, PIECE> P;
   __shared__ u4 q_lds[2][KC / 16 * QP * TQ * 2], r_lds[2][KC / 16 * RP * TR * 2];
   __shared__ float s_lds[2][TR];
@@ -621,7 +621,8 @@ __global__ __launch_bounds__(256, FMT == NATIVE && Q == F32 ? 1 : 2) void partit
     }
     look_up();
   };
-  u4 row_held[2][RT][PU], query_held[2][QN][QU];
+  u4 row_held[2][RT][PU];
+  Raw8<Q> query_held[2][QN];
   float scale_held[2];
   uint32_t held_base[2];
   const auto load = [&](auto which) {
@@ -641,15 +642,7 @@ __global__ __launch_bounds__(256, FMT == NATIVE && Q == F32 ? 1 : 2) void partit
     // come here)
     const uint32_t at = base + tid % C8 * 8;
 #pragma unroll
-    for (int i = 0; i < QN; i++) {
-      const uint8_t *p = queries[i] + (size_t)(at + 8 <= a.c.dim ? at : a.c.dim - 8) * elem_size<Q>;
-      if constexpr (Q == F32) {
-        query_held[H][i][0] = reinterpret_cast<const u4_any4 *>(p)[0];
-        query_held[H][i][1] = reinterpret_cast<const u4_any4 *>(p)[1];
-      } else {
-        query_held[H][i][0] = *reinterpret_cast<const u4_any *>(p);
-      }
-    }
+    for (int i = 0; i < QN; i++) query_held[H][i].load_whole(queries[i], at + 8 <= a.c.dim ? at : a.c.dim - 8);
     if (H == 1 && ++load_stage == stages) {
       load_stage = 0;
       next_tile();
@@ -663,21 +656,8 @@ __global__ __launch_bounds__(256, FMT == NATIVE && Q == F32 ? 1 : 2) void partit
       const uint32_t at = base + tid % C8 * 8, by = at - (at + 8 <= a.c.dim ? at : a.c.dim - 8);
 #pragma unroll
       for (int i = 0; i < QN; i++) {
-        uint32_t v[4 * QU];
-#pragma unroll
-        for (int k = 0; k < 4 * QU; k++) v[k] = by < 8 ? query_held[H][i][k / 4][k % 4] : 0;
-#pragma unroll
-        for (int m = 4; m >= 1; m /= 2) {
-          const bool move = by & m;
-          const int d = m * elem_size<Q> / 4;
-#pragma unroll
-          for (int k = 0; k < 4 * QU; k++) {
-            const uint32_t next = k + 1 < 4 * QU ? v[k + 1 < 4 * QU ? k + 1 : 0] : 0, far = d && k + d < 4 * QU ? v[k + d < 4 * QU ? k + d : 0] : 0;
-            v[k] = move ? (d ? far : __builtin_amdgcn_alignbit(next, v[k], 16)) : v[k];
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < 4 * QU; k++) query_held[H][i][k / 4][k % 4] = v[k];
+        if (by >= 8) query_held[H][i].zero();
+        else query_held[H][i].drop(by);
       }
       if (FMT == NATIVE) {
 #pragma unroll
@@ -691,11 +671,10 @@ __global__ __launch_bounds__(256, FMT == NATIVE && Q == F32 ? 1 : 2) void partit
       u4 w[QP];
       if constexpr (Q == F32) {
         float v[8];
-#pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = __uint_as_float(query_held[H][i][k / 4][k % 4]);
+        query_held[H][i].floats(v);
         planes8(v, w);
       } else {
-        w[0] = query_held[H][i][0];
+        w[0] = query_held[H][i].w[0];
       }
 #pragma unroll
       for (int p = 0; p < QP; p++) q_lds[H][place(TQ, tid % C8, QP, p, (i * 256 + tid) / C8)] = w[p];

@@ -45,31 +45,55 @@ __device__ __forceinline__ float f16_to_f32(uint32_t low16) {
   return (float)x;
 }
 
-// eight elements as they are in memory; those from `valid` on are zeros.  They are read all the same where `more` says that the
-// memory goes on behind them (another row follows)
+// Eight elements as they are in memory; those from `valid` on are zeros.  They are read all the same where `more` says that the
+// memory goes on behind them (another row follows): see cut().
 template <int T>
 struct Raw8 {
   u4 w[elem_size<T> / 2];
 
+  __device__ __forceinline__ void load_whole(const void *row, uint32_t at) {
+    if constexpr (T == F32) {
+      const u4_any4 *p = reinterpret_cast<const u4_any4 *>(static_cast<const float *>(row) + at);
+      w[0] = p[0];
+      w[1] = p[1];
+    } else {
+      w[0] = *reinterpret_cast<const u4_any *>(static_cast<const uint16_t *>(row) + at);
+    }
+  }
   __device__ __forceinline__ void load(const void *row, uint32_t at, uint32_t valid, bool more = false) {
     if (valid >= 8 || (more && valid)) {
-      if constexpr (T == F32) {
-        const u4_any4 *p = reinterpret_cast<const u4_any4 *>(static_cast<const float *>(row) + at);
-        w[0] = p[0];
-        w[1] = p[1];
-      } else {
-        w[0] = *reinterpret_cast<const u4_any *>(static_cast<const uint16_t *>(row) + at);
-      }
+      load_whole(row, at);
       return;
     }
     zero();
     if (!valid) return;
+    if (at) {   // the row's last elements: the last eight, of which the first go
+      load_whole(row, at + valid - 8);
+      drop(8 - valid);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < 8; i++)
       if ((uint32_t)i < valid) {
-        if constexpr (T == F32) w[i / 4][i % 4] = static_cast<const uint32_t *>(row)[at + i];
-        else w[0][i / 2] |= (uint32_t)static_cast<const uint16_t *>(row)[at + i] << (16 * (i % 2));
+        if constexpr (T == F32) w[i / 4][i % 4] = static_cast<const uint32_t *>(row)[i];
+        else w[0][i / 2] |= (uint32_t)static_cast<const uint16_t *>(row)[i] << (16 * (i % 2));
       }
+  }
+  // the first `by` < 8 elements go, zeros follow
+  __device__ __forceinline__ void drop(uint32_t by) {
+    constexpr int N = 2 * elem_size<T>;
+#pragma unroll
+    for (int m = 4; m >= 1; m /= 2) {
+      const bool move = by & m;
+      constexpr int per = 4 / elem_size<T>;
+      const int d = m / per;   // dwords; 0: half of one
+#pragma unroll
+      for (int k = 0; k < N; k++) {
+        const uint32_t here = w[k / 4][k % 4], next = k + 1 < N ? w[(k + 1) / 4 % (N / 4)][(k + 1) % 4] : 0;
+        const uint32_t far = k + d < N ? w[(k + d) / 4 % (N / 4)][(k + d) % 4] : 0;
+        w[k / 4][k % 4] = move ? (d ? far : __builtin_amdgcn_alignbit(next, here, 16)) : here;
+      }
+    }
   }
   __device__ __forceinline__ void zero() {
 #pragma unroll

@@ -166,32 +166,59 @@ __global__ __launch_bounds__(256) void row_write_kernel(RowCacheArgs c, const vo
   }
 }
 
-// one scale a row: a wavefront has a row, and reads it again (from the caches) once its largest magnitude is known
-template <int T, int FMT>
+// one scale a row of more than 512 elements: a wavefront has a row, in C eights a lane; C = 0, and the last row:
+// read a second time (from the caches) once the largest magnitude is known
+template <int T, int FMT, int C>
 __global__ __launch_bounds__(256) void row_write_whole_kernel(RowCacheArgs c, const void *rows, uint32_t stride, const int64_t *slots, uint32_t n) {
-  const uint32_t lane = threadIdx.x % 64;
+  const uint32_t lane = threadIdx.x % 64, padded = rows_padded(c.dim);
   for (uint64_t r = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64; r < n; r += (uint64_t)gridDim.x * 4) {
     const int64_t slot = slots[r];
     if (slot < 0 || (uint64_t)slot >= c.capacity) continue;
-    const void *row = static_cast<const uint8_t *>(rows) + (size_t)r * stride * elem_size<T>;
-    const uint32_t padded = (c.dim + 31) / 32 * 32;
-    float v[8];
-    uint32_t most = 0;
-    for (uint32_t at = lane * 8; at < c.dim; at += 512) {
-      load8<T>(row, at, c.dim - at, v);
-      const uint32_t o = most8(v);
-      most = most > o ? most : o;
+    const uint8_t *row = static_cast<const uint8_t *>(rows) + r * ((uint64_t)stride * elem_size<T>);
+    uint8_t *to = c.codes + (uint64_t)(uint32_t)slot * c.row_bytes;
+    const bool more = r + 1 < n;   // the memory goes on behind this row
+    float v[8], s, inv;
+    uint32_t most = 0, code[2];
+    if (C > 0 && more) {
+      Raw8<T> raw[C ? C : 1];
+#pragma unroll
+      for (int k = 0; k < C; k++) {
+        const uint32_t at = (k * 64 + lane) * 8;
+        raw[k].zero();
+        if (at < c.dim) raw[k].load_whole(row, at);
+      }
+#pragma unroll
+      for (int k = 0; k < C; k++) {
+        const uint32_t at = (k * 64 + lane) * 8;
+        raw[k].cut(at < c.dim ? c.dim - at : 0);
+        raw[k].floats(v);
+        const uint32_t o = most8(v);
+        most = most > o ? most : o;
+      }
+      most = most_of_lanes<64>(most);
+      scale_of<FMT>(most, s, inv);
+#pragma unroll
+      for (int k = 0; k < C; k++) {
+        const uint32_t at = (k * 64 + lane) * 8;
+        raw[k].floats(v);
+        encode8<FMT>(v, s, inv, code);
+        if (at < padded) store_codes8<FMT>(to, at / 8, code);
+      }
+    } else {
+      for (uint32_t at = lane * 8; at < c.dim; at += 512) {
+        load8<T>(row, at, c.dim - at, v);
+        const uint32_t o = most8(v);
+        most = most > o ? most : o;
+      }
+      most = most_of_lanes<64>(most);
+      scale_of<FMT>(most, s, inv);
+      for (uint32_t at = lane * 8; at < padded; at += 512) {
+        load8<T>(row, at, at < c.dim ? c.dim - at : 0, v);
+        encode8<FMT>(v, s, inv, code);
+        store_codes8<FMT>(to, at / 8, code);
+      }
     }
-    most = most_of_lanes<64>(most);
-    float s, inv;
-    scale_of<FMT>(most, s, inv);
-    for (uint32_t at = lane * 8; at < padded; at += 512) {
-      load8<T>(row, at, at < c.dim ? c.dim - at : 0, v);
-      uint32_t code[2];
-      encode8<FMT>(v, s, inv, code);
-      store_codes8<FMT>(c.codes + (size_t)slot * c.row_bytes, at / 8, code);
-    }
-    if (lane == 0) c.scales[slot] = s;
+    if (lane == 0) c.scales[(uint32_t)slot] = s;
   }
 }
 
@@ -447,16 +474,27 @@ uint32_t rows_a_workgroup(uint32_t n, uint32_t chunks) {
 
 template <int T, int FMT>
 void write_as(const RowCacheArgs &c, const void *rows, uint32_t stride, const int64_t *slots, uint32_t n, hipStream_t s) {
-  if (c.block != 32 && c.block != 64 && c.block != 128) {
-    hipLaunchKernelGGL((row_write_whole_kernel<T, FMT>), dim3(workgroups(((uint64_t)n + 3) / 4)), dim3(256), 0, s, c, rows, stride, slots, n);
+  if (c.nb == 1 && c.dim > 512) {
+    const dim3 grid(workgroups(((uint64_t)n + 3) / 4));
+    if (c.dim <= 1024) hipLaunchKernelGGL((row_write_whole_kernel<T, FMT, 2>), grid, dim3(256), 0, s, c, rows, stride, slots, n);
+    else if constexpr (T == F32) hipLaunchKernelGGL((row_write_whole_kernel<T, FMT, 0>), grid, dim3(256), 0, s, c, rows, stride, slots, n);
+    else if (c.dim <= 2048) hipLaunchKernelGGL((row_write_whole_kernel<T, FMT, 4>), grid, dim3(256), 0, s, c, rows, stride, slots, n);
+    else hipLaunchKernelGGL((row_write_whole_kernel<T, FMT, 0>), grid, dim3(256), 0, s, c, rows, stride, slots, n);
     return;
   }
-  const uint32_t chunks = c.nb * (c.block / 8), per = rows_a_workgroup(n, chunks);
+  // the lanes of a block, or of a row that is one
+  uint32_t lanes = 4;
+  while (lanes * 8 < (c.nb == 1 ? rows_padded(c.dim) : c.block)) lanes *= 2;
+  const uint32_t chunks = c.nb * lanes, per = rows_a_workgroup(n, chunks);
   const dim3 grid(workgroups(((uint64_t)n + per - 1) / per));
   const FastDiv d(chunks);
-  if (c.block == 32) hipLaunchKernelGGL((row_write_kernel<T, FMT, 4>), grid, dim3(256), 0, s, c, rows, stride, slots, n, per, d);
-  else if (c.block == 64) hipLaunchKernelGGL((row_write_kernel<T, FMT, 8>), grid, dim3(256), 0, s, c, rows, stride, slots, n, per, d);
-  else hipLaunchKernelGGL((row_write_kernel<T, FMT, 16>), grid, dim3(256), 0, s, c, rows, stride, slots, n, per, d);
+  switch (lanes) {
+    case 4: hipLaunchKernelGGL((row_write_kernel<T, FMT, 4>), grid, dim3(256), 0, s, c, rows, stride, slots, n, per, d); break;
+    case 8: hipLaunchKernelGGL((row_write_kernel<T, FMT, 8>), grid, dim3(256), 0, s, c, rows, stride, slots, n, per, d); break;
+    case 16: hipLaunchKernelGGL((row_write_kernel<T, FMT, 16>), grid, dim3(256), 0, s, c, rows, stride, slots, n, per, d); break;
+    case 32: hipLaunchKernelGGL((row_write_kernel<T, FMT, 32>), grid, dim3(256), 0, s, c, rows, stride, slots, n, per, d); break;
+    default: hipLaunchKernelGGL((row_write_kernel<T, FMT, 64>), grid, dim3(256), 0, s, c, rows, stride, slots, n, per, d); break;
+  }
 }
 
 template <int T>
