@@ -265,7 +265,7 @@ struct Piece {
   }
 };
 
-// Few queries a partition: the rows' bytes are what it takes.  A workgroup has a run of tiles of 16 queries x 16 S rows a wavefront;
+// Few queries a partition: the rows' bytes are what it takes.  A workgroup has a run of tiles of 16 QT queries x 16 S rows a wavefront;
 // the queries of a partition are put into LDS once for all its tiles (in parts of KP stages if the rows are longer than that).
 // A wavefront takes its rows in stages of 4 KiB, 16 S rows x 256 / S bytes: four loads of 16 neighbouring bytes a lane, whole lines of
 // the rows, one stage in registers under way (across tiles too) while the one before is multiplied.  (Loads in the shape of the matrix
@@ -275,16 +275,16 @@ struct Piece {
 // ONCE: the rows are read past the caches' keeping (a batch of 256 over 64 partitions: 57 us for 63; with three query tiles a
 // partition, which read the rows three times, 170 for 134).
 // Every part of the loop is in the code once: a small call is mostly the first pass of its instructions through the caches.
-template <int FMT, int Q, int W, int S, int WAVES, bool ONCE>
+template <int FMT, int Q, int W, int QT, int S, int WAVES, bool ONCE>
 __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionArgs a, FastDiv page) {
   typedef Piece<FMT, Q, W> P;
-  constexpr int QP = Q == F32 ? 3 : 1, FR = W / 8, TQ = 16, WR = 16 * S, TR = WR * WAVES;
+  constexpr int QP = Q == F32 ? 3 : 1, FR = W / 8, TQ = 16 * QT, WR = 16 * S, TR = WR * WAVES;
   constexpr int CS = 16 / S;                                  // chunks of a row in a stage
   constexpr int SP = CS * 16 / (4 * P::BYTES);                // steps of 4 W elements in a stage
   constexpr int QS = FMT == NATIVE ? 0 : (SP + 3) / 4;        // scale loads a stage and row group: a lane's quarter has every fourth
-  constexpr int KP = (Q == F32 ? 24 : 32) / (SP * FR);        // stages of queries in LDS at a time: 72 or 32 KiB
+  constexpr int KP = (Q == F32 ? 24 : 32) / (SP * FR);        // stages of queries in LDS at a time: 72 or 32 QT KiB
   static_assert(SP >= 1 && KP >= 1, "");
-  __shared__ u4 staged[KP * SP * FR * QP * 64];
+  __shared__ u4 staged[KP * SP * FR * QP * QT * 64];
   __shared__ u4 passing[WAVES][256];
   __shared__ RunShared run_shared;
 
@@ -319,9 +319,11 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
   u4 chunk[4];
   float next_scale[S][QS ? QS : 1], scale[S][QS ? QS : 1];
   u4 *const mine = passing[wave];
-  f32x4 acc[S];
+  f32x4 acc[S][QT];
 #pragma unroll
-  for (int k = 0; k < S; k++) acc[k] = f32x4{0, 0, 0, 0};
+  for (int k = 0; k < S; k++)
+#pragma unroll
+    for (int t = 0; t < QT; t++) acc[k][t] = f32x4{0, 0, 0, 0};
   uint32_t staged_g = ~0u, staged_q = 0, staged_p = 0;   // whose queries are in LDS, from which stage on
   uint32_t taken = 0;
   uint32_t use_stage = 0, load_stage = stages;           // stages: on to the next tile before the next load
@@ -395,7 +397,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
 
     if (round >= 0) {
       // the one in LDS multiplied
-      const u4 *queries = staged + use_stage % KP * (SP * FR * QP * 64) + lane;
+      const u4 *queries = staged + use_stage % KP * (SP * FR * QP * QT * 64) + lane;
       const uint32_t first_block = (use_stage * SP) >> block_shift;
       P piece[SP][S];
 #pragma unroll
@@ -421,14 +423,18 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
         }
 #pragma unroll
       for (int st = 0; st < SP; st++) {
-        f32x4 part[S];
+        f32x4 part[S][QT];
 #pragma unroll
-        for (int k = 0; k < S; k++) part[k] = FMT == NATIVE ? acc[k] : f32x4{0, 0, 0, 0};
+        for (int k = 0; k < S; k++)
+#pragma unroll
+          for (int t = 0; t < QT; t++) part[k][t] = FMT == NATIVE ? acc[k][t] : f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int f = 0; f < FR; f++) {
-          u4 q[QP];
+          u4 q[QT][QP];
 #pragma unroll
-          for (int p = 0; p < QP; p++) q[p] = queries[((st * FR + f) * QP + p) * 64];
+          for (int t = 0; t < QT; t++)
+#pragma unroll
+            for (int p = 0; p < QP; p++) q[t][p] = queries[(((st * FR + f) * QP + p) * QT + t) * 64];
 #pragma unroll
           for (int k = 0; k < S; k++) {
             u4 b[P::PLANES];
@@ -444,7 +450,9 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
             for (int p = QP - 1; p >= 0; p--)   // the smallest first
 #pragma unroll
               for (int c = P::PLANES - 1; c >= 0; c--)
-                if (p + c < 3) part[k] = mfma16<Q>(q[p], b[c], part[k]);   // the planes left out are below 2^-24 of the product
+#pragma unroll
+                for (int t = 0; t < QT; t++)
+                  if (p + c < 3) part[k][t] = mfma16<Q>(q[t][p], b[c], part[k][t]);   // the planes left out are below 2^-24 of the product
           }
         }
         // a step's sum, times the scale of the block that it is in (no branch for the block's end: the steps overlap)
@@ -452,14 +460,17 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
 #pragma unroll
         for (int k = 0; k < S; k++) {
           if (FMT == NATIVE) {
-            acc[k] = part[k];
+#pragma unroll
+            for (int t = 0; t < QT; t++) acc[k][t] = part[k][t];
           } else {
             float v = scale[k][0];
 #pragma unroll
             for (int q = 1; q < QS; q++) v = block / 4 == (uint32_t)q ? scale[k][q] : v;
             v = __uint_as_float(__builtin_amdgcn_ds_bpermute((block % 4 * 16 + col) * 4, __float_as_uint(v)));
 #pragma unroll
-            for (int r = 0; r < 4; r++) acc[k][r] = __builtin_fmaf(v, part[k][r], acc[k][r]);
+            for (int t = 0; t < QT; t++)
+#pragma unroll
+              for (int r = 0; r < 4; r++) acc[k][t][r] = __builtin_fmaf(v, part[k][t][r], acc[k][t][r]);
           }
         }
       }
@@ -473,14 +484,14 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
       const uint32_t q0 = turned ? held.q0 : now.q0, q_end = turned ? held.q_end : now.q_end;
       __syncthreads();
       const uint32_t np = stages - p0 < KP ? stages - p0 : KP, asked = q_end - q0 < TQ ? q_end - q0 : TQ;
-      const uint32_t shift = asked > 8 ? 4 : asked > 4 ? 3 : asked > 2 ? 2 : asked > 1 ? 1 : 0;
+      const uint32_t shift = asked > 16 ? 5 : asked > 8 ? 4 : asked > 4 ? 3 : asked > 2 ? 2 : asked > 1 ? 1 : 0;
       for (uint32_t i = tid; i < np * (SP * FR * 4) << shift; i += 64 * WAVES) {
         const uint32_t q = i & ((1u << shift) - 1), e = i >> shift, f = e % FR, h = e / FR % 4, st = e / (4 * FR);
         if (q >= asked) continue;   // what is in LDS behind them is multiplied and not used
         u4 w[QP];
         stage8<Q>(a, q0 + q, (p0 * SP + st) * (4 * W) + h * W + f * 8, w);
 #pragma unroll
-        for (int p = 0; p < QP; p++) staged[((st * FR + f) * QP + p) * 64 + h * 16 + q] = w[p];
+        for (int p = 0; p < QP; p++) staged[(((st * FR + f) * QP + p) * QT + q / 16) * 64 + h * 16 + q % 16] = w[p];
       }
       __syncthreads();
       staged_g = meets_g;
@@ -506,10 +517,10 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
         const uint32_t j = now.j0 + k * 16 + col;
         if (j < now.n) {
 #pragma unroll
-          for (int r = 0; r < 4; r++) {
-            const uint32_t q = now.q0 + quarter * 4 + r;
+          for (int e = 0; e < 4 * QT; e++) {
+            const uint32_t q = now.q0 + e / 4 * 16 + quarter * 4 + e % 4;
             if (q < now.q_end) {
-              float p = acc[k][r] * CODE_UNIT<FMT, Q>;
+              float p = acc[k][e / 4][e % 4] * CODE_UNIT<FMT, Q>;
               if constexpr (FMT == NATIVE && Q == F32) {
                 // an infinity meets the other side's planes, some of them 0: the sum is taken again, element by element
                 if (p != p && (there >> k & 1)) {
@@ -523,7 +534,8 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
             }
           }
         }
-        acc[k] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < QT; t++) acc[k][t] = f32x4{0, 0, 0, 0};
       }
       use_stage = 0;
     }
@@ -849,6 +861,13 @@ uint32_t resident(const void *kernel, uint32_t threads) {
   return (uint32_t)(units > 0 && each > 0 ? units * each : 256);
 }
 
+// Which kernel, by the queries of a partition on average (64 partitions x 5461 rows of 768, us; 20 / 40 / 60 queries):
+//   int8 with fp16 queries    16 a tile 92 / 134 / -, 32 a tile 60 / 97 / -, the tiles of 128 107 / 115 / 126
+//   bf16 as it is             160 / 340, 120 / 166, 134 / 149 / 168
+//   int8 with fp32 queries    95 / 146, (no 32 a tile), 229 / 232 / 237
+//   INT4 of 100 wide, 300 x 1000 (rows of 64 bytes)   27 / 35, 29 / 41, 45 / 47 / 51
+constexpr uint32_t TWO_TILES = 13, MANY = 48, MANY_LATE = 80;   // late: fp32 queries, and rows of few chunks
+
 template <int FMT, int Q>
 void scores_as(const PartitionArgs &a, hipStream_t s) {
   const FastDiv page(a.page_rows);
@@ -859,7 +878,13 @@ void scores_as(const PartitionArgs &a, hipStream_t s) {
     const uint64_t tiles = ((uint64_t)a.n_queries / tq + asked) * ((a.most_rows + tr - 1) / tr);
     return dim3((uint32_t)(tiles < resident ? tiles : resident));
   };
-  if (each >= 48 && a.c.dim >= 8) {
+  // the rows' chunks of a stage: the number that leaves the fewest places empty, the largest of those
+  const uint32_t chunks = a.c.row_bytes / 16;
+  uint32_t cs = 16;
+  constexpr bool widest = Q == F32;   // an fp32 step is eight chunks, and 64 rows of three planes do not fit into 128 registers
+  for (uint32_t c : {8u, 4u})
+    if (!(widest && c == 4) && (chunks + c - 1) / c * c < (chunks + cs - 1) / cs * cs) cs = c;
+  if (each >= (Q == F32 || cs == 4 ? MANY_LATE : MANY) && a.c.dim >= 8) {
     const auto many = [&](auto kernel) {
       dim3 g = grid(128, MANY_ROWS<FMT, Q>, resident(reinterpret_cast<const void *>(kernel), 256));
       g.x = (g.x + DIES - 1) / DIES * DIES;
@@ -870,26 +895,27 @@ void scores_as(const PartitionArgs &a, hipStream_t s) {
     else many(partition_many_kernel<FMT, Q, 64>);
     return;
   }
-  // the rows' chunks of a stage: the number that leaves the fewest places empty, the largest of those
-  const uint32_t chunks = a.c.row_bytes / 16;
-  uint32_t cs = 16;
-  constexpr bool widest = Q == F32;   // an fp32 step is eight chunks, and 64 rows of three planes do not fit into 128 registers
-  for (uint32_t c : {8u, 4u})
-    if (!(widest && c == 4) && (chunks + c - 1) / c * c < (chunks + cs - 1) / cs * cs) cs = c;
   const auto few = [&](auto w) {
     constexpr int W = decltype(w)::value, WAVES = Q == F32 ? 16 : 8;
-    const auto launch = [&](auto kernel, uint32_t tr) {
-      hipLaunchKernelGGL(kernel, grid(16, tr, resident(reinterpret_cast<const void *>(kernel), 64 * WAVES)), dim3(64 * WAVES), 0, s, a, page);
+    const auto launch = [&](auto kernel, uint32_t tq, uint32_t tr, uint32_t waves) {
+      hipLaunchKernelGGL(kernel, grid(tq, tr, resident(reinterpret_cast<const void *>(kernel), 64 * waves)), dim3(64 * waves), 0, s, a, page);
     };
     // at eight queries a partition hardly one has more than the sixteen of a tile, so that its rows are read once
     const auto sized = [&](auto once) {
       constexpr bool ONCE = decltype(once)::value;
-      if (cs == 16) launch(partition_few_kernel<FMT, Q, W, 1, WAVES, ONCE>, 16 * WAVES);
-      else if (cs == 8) launch(partition_few_kernel<FMT, Q, W, 2, WAVES, ONCE>, 32 * WAVES);
-      else if constexpr (!widest) launch(partition_few_kernel<FMT, Q, W, 4, WAVES, ONCE>, 64 * WAVES);
+      if (cs == 16) launch(partition_few_kernel<FMT, Q, W, 1, 1, WAVES, ONCE>, 16, 16 * WAVES, WAVES);
+      else if (cs == 8) launch(partition_few_kernel<FMT, Q, W, 1, 2, WAVES, ONCE>, 16, 32 * WAVES, WAVES);
+      else if constexpr (!widest) launch(partition_few_kernel<FMT, Q, W, 1, 4, WAVES, ONCE>, 16, 64 * WAVES, WAVES);
     };
-    if (each <= 8) sized(std::true_type());
-    else sized(std::false_type());
+    if (each <= 8) return sized(std::true_type());
+    if constexpr (Q != F32) {   // (three planes of 32 queries leave no room for whole rows)
+      if (each >= TWO_TILES && cs != 4) {
+        if (cs == 16) launch(partition_few_kernel<FMT, Q, W, 2, 1, 16, false>, 32, 256, 16);
+        else launch(partition_few_kernel<FMT, Q, W, 2, 2, 16, false>, 32, 512, 16);
+        return;
+      }
+    }
+    sized(std::false_type());
   };
   // a lane's piece of a row: as wide as four of them fit into a block
   if constexpr (FMT != NATIVE) {
