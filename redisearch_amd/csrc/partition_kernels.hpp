@@ -140,11 +140,12 @@ struct Place {
   uint32_t g, lo, m, n, left;
 };
 struct Run {
-  uint32_t tiles, stride;
+  uint64_t tiles;
+  uint32_t stride;
   Place at;
 };
 struct RunShared {
-  uint32_t wave_sums[16];
+  uint64_t wave_sums[16];
   Place at;
 };
 // The offsets and counts are on the device, so every workgroup sums the partitions' tiles itself, a share of the partitions a
@@ -154,7 +155,7 @@ constexpr uint32_t DIES = 8;
 template <int THREADS, bool TOGETHER>
 __device__ __forceinline__ Run find_run(const PartitionArgs &a, uint32_t tq, uint32_t tr, RunShared &shared) {
   const uint32_t tid = threadIdx.x, lane = tid % 64, per = (a.n_partitions + THREADS - 1) / THREADS;
-  uint32_t own = 0;
+  uint64_t own = 0;   // (offsets that rise and fall can name more tiles than 32 bits count)
   for (uint32_t i = 0; i < per; i++) {
     const uint32_t g = tid * per + i;
     if (g >= a.n_partitions) break;
@@ -162,43 +163,44 @@ __device__ __forceinline__ Run find_run(const PartitionArgs &a, uint32_t tq, uin
     partition(a, g, lo, m, n);
     own += (m + tq - 1) / tq * ((n + tr - 1) / tr);
   }
-  uint32_t sum = own;
+  uint64_t sum = own;
 #pragma unroll
   for (int k = 1; k < 64; k *= 2) {
-    const uint32_t v = __shfl_up(sum, k, 64);
+    const uint64_t v = __shfl_up((unsigned long long)sum, k, 64);
     if (lane >= (uint32_t)k) sum += v;
   }
   if (lane == 63) shared.wave_sums[tid / 64] = sum;
   __syncthreads();
-  uint32_t total = 0;
+  uint64_t total = 0;
 #pragma unroll
   for (uint32_t w = 0; w < THREADS / 64; w++) {
-    const uint32_t v = shared.wave_sums[w];
+    const uint64_t v = shared.wave_sums[w];
     if (w < tid / 64) sum += v;
     total += v;
   }
   Run run;
-  uint32_t first;
+  uint64_t first;
   if (TOGETHER) {
-    const uint32_t die = blockIdx.x % DIES, from = (uint32_t)((uint64_t)total * die / DIES), to = (uint32_t)((uint64_t)total * (die + 1) / DIES);
+    const uint64_t die = blockIdx.x % DIES, from = total * die / DIES, to = total * (die + 1) / DIES;
     run.stride = gridDim.x / DIES;   // a multiple of the dies
     first = from + blockIdx.x / DIES;
     run.tiles = first < to ? (to - first + run.stride - 1) / run.stride : 0;
   } else {
     run.stride = 1;
-    first = (uint32_t)((uint64_t)total * blockIdx.x / gridDim.x);
-    run.tiles = (uint32_t)((uint64_t)total * (blockIdx.x + 1) / gridDim.x) - first;
+    first = total * blockIdx.x / gridDim.x;
+    run.tiles = total * (blockIdx.x + 1) / gridDim.x - first;
   }
   if (run.tiles == 0) return run;
   if (sum - own <= first && first < sum) {
     Place p;
-    p.left = first - (sum - own);
+    uint64_t left = first - (sum - own);
     for (p.g = tid * per;; p.g++) {
       partition(a, p.g, p.lo, p.m, p.n);
       const uint32_t tiles = (p.m + tq - 1) / tq * ((p.n + tr - 1) / tr);
-      if (p.left < tiles) break;
-      p.left -= tiles;
+      if (left < tiles) break;
+      left -= tiles;
     }
+    p.left = (uint32_t)left;
     shared.at = p;
   }
   __syncthreads();
@@ -325,7 +327,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
 #pragma unroll
     for (int t = 0; t < QT; t++) acc[k][t] = f32x4{0, 0, 0, 0};
   uint32_t staged_g = ~0u, staged_q = 0, staged_p = 0;   // whose queries are in LDS, from which stage on
-  uint32_t taken = 0;
+  uint64_t taken = 0;
   uint32_t use_stage = 0, load_stage = stages;           // stages: on to the next tile before the next load
   const int64_t rounds = (int64_t)run.tiles * stages;
 
@@ -605,7 +607,8 @@ __global__ __launch_bounds__(256, FMT == NATIVE && Q == F32 ? 1 : 2) void partit
   // ---- the loads: `loading` is the tile they are at, the pages of `coming` are looked up.  Piece i of a thread is of row
   // (i * 256 + tid) / NP, eight i of query (i * 256 + tid) / C8; its scale is row tid % TR's
   Place load_at = run.at;
-  uint32_t loads_taken = 1, load_stage = 0;
+  uint64_t loads_taken = 1;
+  uint32_t load_stage = 0;
   Tile loading = {}, coming = take(load_at);
   int32_t id[RT], scale_id;
   const uint8_t *source[RT], *queries[QN];
@@ -801,7 +804,8 @@ __global__ __launch_bounds__(256, FMT == NATIVE && Q == F32 ? 1 : 2) void partit
   put(first_half);
   load(first_half);
   __syncthreads();
-  uint32_t use_stage = 0, used = 0;
+  uint32_t use_stage = 0;
+  uint64_t used = 0;
   for (;;) {
     multiply(first_half);
     put(second_half);

@@ -658,3 +658,78 @@ def test_an_index_refuses_another_cache():
     with pytest.raises(RuntimeError, match="label range overlaps"):
         cache.c.add_to(index, slots.data_ptr(), 4, 2)
     assert index.index_size() == 4 and not cache.codes.any()
+
+
+@pytest.mark.parametrize("vtype,fmt,block", ALL)
+@pytest.mark.parametrize("dim,counts,offsets", [(33, [300, 50], [0, 33, 40]), (768, [130, 257], [0, 32, 33]), (1500, [40], [0, 47]), (200, [70, 0, 65], [1, 17, 40, 90])])
+def test_scores_of_a_few_dozen_queries(vtype, fmt, block, dim, counts, offsets):
+    """13 to 47 queries a partition on average: tiles of 32 queries, one of them cut, rows longer than what LDS holds of the queries."""
+    gen = torch.Generator().manual_seed(dim)
+    page_rows = 13
+    need = -(-max(counts) // page_rows)
+    cache = filled(gen, vtype, dim, fmt, block, page_rows * need * len(counts))
+    pages = torch.randperm(need * len(counts), generator=gen).to(torch.int32).view(len(counts), need).contiguous().cuda()
+    check_scores(cache.c, cache.codes, cache.scales, values(gen, offsets[-1] + 2, dim, vtype), offsets, pages, page_rows, counts, R.DISTANCE, max(counts) + 1)
+
+
+@pytest.mark.parametrize("vtype,fmt,block", [(P.F32, R.INT8, 128), (P.F16, R.INT4, 64), (P.BF16, R.NATIVE, 0), (P.F32, R.NATIVE, 0)])
+def test_scores_where_one_partition_has_all_the_queries(vtype, fmt, block):
+    """The average says few queries a partition, one partition has hundreds."""
+    gen = torch.Generator().manual_seed(77)
+    cache = filled(gen, vtype, 96, fmt, block, 640)
+    pages = torch.arange(640 // 16, dtype=torch.int32).view(40, 1).cuda()
+    offsets = [0] * 20 + [210] * 21
+    check_scores(cache.c, cache.codes, cache.scales, values(gen, 210, 96, vtype), offsets, pages, 16, [16] * 40, R.PRODUCT, 16)
+
+
+@pytest.mark.parametrize("vtype", list(TYPES), ids=ids)
+@pytest.mark.parametrize("dim", [1, 5, 7, 8, 9, 15, 31, 63, 65, 95])
+def test_scores_of_many_queries_of_every_odd_width(vtype, dim):
+    """The ends of queries that are no multiple of anything, in the kernel that takes a hundred and more a partition; the memory right
+    behind the last query is not the caller's."""
+    gen = torch.Generator().manual_seed(dim)
+    for fmt, block in ((R.INT8, 0), (R.NATIVE, 0), (R.INT4, 32)):
+        cache = filled(gen, vtype, dim, fmt, block, 160)
+        pages = torch.arange(10, dtype=torch.int32).view(1, 10).cuda()
+        q = values(gen, 131, dim, vtype)
+        guarded = torch.full((131 * dim + 64,), float("nan"), dtype=q.dtype, device="cuda")
+        guarded[: 131 * dim] = q.reshape(-1)
+        check_scores(cache.c, cache.codes, cache.scales, guarded[: 131 * dim].view(131, dim), [0, 131], pages, 16, [150], R.PRODUCT, 160)
+
+
+def test_writes_at_the_end_of_memory():
+    """The last row of an array of odd width: what lies behind it (NaN here) does not get into its block."""
+    for vtype in TYPES:
+        for dim in (3, 9, 33, 100, 515, 1037):
+            for block in (0, 32):
+                data = torch.full((5 * dim + 16,), float("nan"), dtype=TYPES[vtype], device="cuda")
+                data[: 5 * dim] = torch.randn(5 * dim, device="cuda").to(TYPES[vtype])
+                rows = data[: 5 * dim].view(5, dim)
+                cache = Cache(vtype, dim, R.INT8, block, 5)
+                cache.write(rows, torch.arange(5, device="cuda"))
+                codes, scales = cache.plain()
+                want_codes, want_scales = P.quantise(as64(rows), R.INT8, block)
+                np.testing.assert_array_equal(scales, want_scales)
+                np.testing.assert_array_equal(codes, want_codes)
+
+
+def test_a_row_with_nan_leaves_its_neighbours_alone():
+    """A full load of a row's end reads into the next row; a NaN there stays out of this one's block."""
+    for vtype in TYPES:
+        for dim, block in ((33, 0), (100, 32), (517, 0), (1030, 0), (1030, 128)):
+            rows = torch.randn((6, dim), device="cuda").to(TYPES[vtype])
+            rows[1::2, 0] = float("nan")
+            cache = Cache(vtype, dim, R.E4M3, block, 6)
+            cache.write(rows, torch.arange(6, device="cuda"))
+            codes, scales = cache.plain()
+            want_codes, want_scales = P.quantise(as64(rows), R.E4M3, block)
+            np.testing.assert_array_equal(scales, want_scales)
+            np.testing.assert_array_equal(codes, want_codes)
+
+
+def test_overlapping_ranges_of_queries_stay_in_bounds():
+    """Offsets that fall and rise again: every range that is one is answered."""
+    gen = torch.Generator().manual_seed(8)
+    cache = filled(gen, P.F16, 64, R.INT8, 0, 64)
+    pages = torch.zeros((5, 1), dtype=torch.int32, device="cuda")
+    check_scores(cache.c, cache.codes, cache.scales, values(gen, 20, 64, P.F16), [0, 20, 0, 20, 5, 9], pages, 64, [64] * 5, R.PRODUCT, 64)
