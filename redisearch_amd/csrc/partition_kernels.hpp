@@ -558,8 +558,8 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
 template <int FMT, int Q>
 constexpr int MANY_ROWS = FMT == NATIVE && Q != F32 ? 256 : 128;
 template <int FMT, int Q, int FLUSH>
-__global__ __launch_bounds__(256, FMT == NATIVE && Q == F32 ? 1 : 2) void partition_many_kernel(PartitionArgs a, FastDiv page) {
-  constexpr int TQ = 128, TR = MANY_ROWS<FMT, Q>, X = TR / 64, Y = 2, KC = 32, QP = Q == F32 ? 3 : 1, RP = FMT == NATIVE && Q == F32 ? 3 : 1;
+__global__ __launch_bounds__(256, 2) void partition_many_kernel(PartitionArgs a, FastDiv page) {
+  constexpr int TQ = 128, TR = MANY_ROWS<FMT, Q>, X = TR / 64, Y = 2, KC = FMT == NATIVE && Q == F32 ? 16 : 32, QP = Q == F32 ? 3 : 1, RP = FMT == NATIVE && Q == F32 ? 3 : 1;
   constexpr int C8 = KC / 8;                                                 // eights of a half
   constexpr int PIECE = FMT == NATIVE ? 8 : FMT == INT4 ? 32 : 16;           // elements of a row that a thread loads together
   constexpr int PIECE_BYTES = FMT == NATIVE ? 8 * elem_size<Q> : 16, PU = PIECE_BYTES / 16;
