@@ -872,15 +872,25 @@ uint32_t resident(const void *kernel, uint32_t threads) {
 //   INT4 of 100 wide, 300 x 1000 (rows of 64 bytes)   27 / 35, 29 / 41, 45 / 47 / 51
 constexpr uint32_t TWO_TILES = 13, MANY = 48, MANY_LATE = 80;   // late: fp32 queries, and rows of few chunks
 
+// Workgroups of four waves where there are few tiles of theirs: one's waves wait for each other while the queries are
+// laid out, and four have less to wait for.  us with the wide ones / with four waves (int8 rows of 768, one query each):
+//   fp32 queries: 8 x 700 (88 tiles) 14.4 / 8.3, 64 x 512 (512) 14.6 / 11.7, 64 x 1024 (1088) 15.4 / 19.3
+//   fp16 queries: 8 x 700 8.5 / 7.3, 64 x 512 11.3 / 9.9, 64 x 1024 12.4 / 13.4
+// rows of 64 bytes, whose tile is four times as long (INT4 of 100 wide): 300 x 1000 (1200) 20.4 / 17.4, 300 x 4000 36 / 38
+constexpr uint64_t LITTLE = 1024, LITTLE_NARROW = 2048;
+
 template <int FMT, int Q>
 void scores_as(const PartitionArgs &a, hipStream_t s) {
   const FastDiv page(a.page_rows);
   const uint32_t asked = a.n_partitions < a.n_queries ? a.n_partitions : a.n_queries;   // partitions with queries, at most
   const uint32_t each = a.n_queries / a.n_partitions;
+  const auto tiles = [&](uint32_t tq, uint32_t tr) {   // at most
+    return ((uint64_t)a.n_queries / tq + asked) * ((a.most_rows + tr - 1) / tr);
+  };
   // no more workgroups than there can be tiles, and no more than are resident at once
   const auto grid = [&](uint32_t tq, uint32_t tr, uint64_t resident) {
-    const uint64_t tiles = ((uint64_t)a.n_queries / tq + asked) * ((a.most_rows + tr - 1) / tr);
-    return dim3((uint32_t)(tiles < resident ? tiles : resident));
+    const uint64_t n = tiles(tq, tr);
+    return dim3((uint32_t)(n < resident ? n : resident));
   };
   // the rows' chunks of a stage: the number that leaves the fewest places empty, the largest of those
   const uint32_t chunks = a.c.row_bytes / 16;
@@ -905,13 +915,15 @@ void scores_as(const PartitionArgs &a, hipStream_t s) {
       hipLaunchKernelGGL(kernel, grid(tq, tr, resident(reinterpret_cast<const void *>(kernel), 64 * waves)), dim3(64 * waves), 0, s, a, page);
     };
     // at eight queries a partition hardly one has more than the sixteen of a tile, so that its rows are read once
-    const auto sized = [&](auto once) {
+    const auto sized = [&](auto waves, auto once) {
+      constexpr int V = decltype(waves)::value;
       constexpr bool ONCE = decltype(once)::value;
-      if (cs == 16) launch(partition_few_kernel<FMT, Q, W, 1, 1, WAVES, ONCE>, 16, 16 * WAVES, WAVES);
-      else if (cs == 8) launch(partition_few_kernel<FMT, Q, W, 1, 2, WAVES, ONCE>, 16, 32 * WAVES, WAVES);
-      else if constexpr (!widest) launch(partition_few_kernel<FMT, Q, W, 1, 4, WAVES, ONCE>, 16, 64 * WAVES, WAVES);
+      if (cs == 16) launch(partition_few_kernel<FMT, Q, W, 1, 1, V, ONCE>, 16, 16 * V, V);
+      else if (cs == 8) launch(partition_few_kernel<FMT, Q, W, 1, 2, V, ONCE>, 16, 32 * V, V);
+      else if constexpr (!widest) launch(partition_few_kernel<FMT, Q, W, 1, 4, V, ONCE>, 16, 64 * V, V);
     };
-    if (each <= 8) return sized(std::true_type());
+    if (tiles(16, 256 / cs * 4) <= (cs == 4 ? LITTLE_NARROW : LITTLE)) return sized(std::integral_constant<int, 4>(), std::false_type());
+    if (each <= 8) return sized(std::integral_constant<int, WAVES>(), std::true_type());
     if constexpr (Q != F32) {   // (three planes of 32 queries leave no room for whole rows)
       if (each >= TWO_TILES && cs != 4) {
         if (cs == 16) launch(partition_few_kernel<FMT, Q, W, 2, 1, 16, false>, 32, 256, 16);
@@ -919,7 +931,7 @@ void scores_as(const PartitionArgs &a, hipStream_t s) {
         return;
       }
     }
-    sized(std::false_type());
+    sized(std::integral_constant<int, WAVES>(), std::false_type());
   };
   // a lane's piece of a row: as wide as four of them fit into a block
   if constexpr (FMT != NATIVE) {

@@ -733,3 +733,41 @@ def test_overlapping_ranges_of_queries_stay_in_bounds():
     cache = filled(gen, P.F16, 64, R.INT8, 0, 64)
     pages = torch.zeros((5, 1), dtype=torch.int32, device="cuda")
     check_scores(cache.c, cache.codes, cache.scales, values(gen, 20, 64, P.F16), [0, 20, 0, 20, 5, 9], pages, 64, [64] * 5, R.PRODUCT, 64)
+
+
+def check_scores_in_a_wide_table(cache, queries, offsets, pages, page_rows, counts, form, ld):
+    """The same call, in a table and an array of scores that allow 70 000 rows a partition, which is what the kernel is chosen by; the
+    columns that no partition has are compared on the GPU."""
+    wide = -(-70000 // page_rows)
+    table = torch.full((len(counts), wide), -1, dtype=torch.int32, device="cuda")
+    table[:, : pages.shape[1]] = pages
+    out = torch.full((queries.shape[0] + 1, 70001), 123.0, device="cuda")
+
+    class Wide:
+        c = cache.c.c
+
+        def partition_scores(self, q, stride, m, off, n, narrow, max_pages, page_rows, cnt, form, scores, ld, s):
+            cache.c.partition_scores(q, stride, m, off, n, table.data_ptr(), wide, page_rows, cnt, form, out.data_ptr(), 70001, s)
+            # the first columns go where the check looks for them
+            there = torch.arange(m + 1, device="cuda")
+            kept = out[:, :ld].contiguous()
+            R.RowCache(P.F32, ld, R.NATIVE, 0, m + 1, kept.data_ptr(), None).read(there.data_ptr(), m + 1, scores, ld, s)
+            torch.cuda.synchronize()
+
+    check_scores(Wide(), cache.codes, cache.scales, queries, offsets, pages, page_rows, counts, form, ld)
+    assert (out[:, ld:] == 123).all() and (out[-1] == 123).all()
+
+
+@pytest.mark.parametrize("vtype,fmt,block", ALL)
+@pytest.mark.parametrize("dim", [33, 300, 768])
+@pytest.mark.parametrize("offsets", [[0, 0, 4, 7, 20, 22, 23, 24, 40], [0, 17, 20, 20, 33, 49, 60, 72, 100], [0, 40, 41, 90, 90, 100, 101, 133, 180]],
+                         ids=["few", "tens", "dozens"])
+def test_scores_in_tables_of_many_rows(vtype, fmt, block, dim, offsets):
+    """The kernels for long partitions, at partitions of none, one and a tile and a bit."""
+    gen = torch.Generator().manual_seed(dim + len(offsets) + fmt)
+    counts, page_rows = [33, 600, 1, 0, 257, 1100, 64, 16], 32
+    need = [-(-n // page_rows) for n in counts]
+    cache = filled(gen, vtype, dim, fmt, block, page_rows * sum(need))
+    pages = torch.full((8, max(need)), -1, dtype=torch.int32)
+    pages[torch.arange(max(need))[None, :] < torch.tensor(need)[:, None]] = torch.randperm(sum(need), generator=gen).to(torch.int32)
+    check_scores_in_a_wide_table(cache, values(gen, offsets[-1], dim, vtype), offsets, pages.cuda(), page_rows, counts, R.PRODUCT, 1120)
