@@ -46,7 +46,7 @@ __device__ __forceinline__ float f16_to_f32(uint32_t low16) {
 }
 
 // Eight elements as they are in memory; those from `valid` on are zeros.  They are read all the same where `more` says that the
-// memory goes on behind them (another row follows): see cut().
+// memory goes on behind them (another row of at least four elements follows): see cut().
 template <int T>
 struct Raw8 {
   u4 w[elem_size<T> / 2];

@@ -143,7 +143,7 @@ __global__ __launch_bounds__(256) void row_write_kernel(RowCacheArgs c, const vo
       for (int u = 0; u < U; u++) {   // a row that is left out is not read
         const uint32_t at = chunk[u] * 8;
         const bool there = slot[u] >= 0 && (uint64_t)slot[u] < c.capacity;
-        raw[u].load(from + (uint64_t)row[u] * row_stride, at, there && at < c.dim ? c.dim - at : 0, first + row[u] + 1 < n);
+        raw[u].load(from + (uint64_t)row[u] * row_stride, at, there && at < c.dim ? c.dim - at : 0, c.dim >= 4 && first + row[u] + 1 < n);   // (eight are at most two rows)
       }
 #pragma unroll
       for (int u = 0; u < U; u++) {

@@ -771,3 +771,19 @@ def test_scores_in_tables_of_many_rows(vtype, fmt, block, dim, offsets):
     pages = torch.full((8, max(need)), -1, dtype=torch.int32)
     pages[torch.arange(max(need))[None, :] < torch.tensor(need)[:, None]] = torch.randperm(sum(need), generator=gen).to(torch.int32)
     check_scores_in_a_wide_table(cache, values(gen, offsets[-1], dim, vtype), offsets, pages.cuda(), page_rows, counts, R.PRODUCT, 1120)
+
+
+@pytest.mark.parametrize("vtype", list(TYPES), ids=ids)
+@pytest.mark.parametrize("dim", [1, 2, 3, 4, 5, 7])
+def test_narrow_rows_up_to_the_end_of_an_allocation(vtype, dim):
+    """Rows of less than eight elements whose array ends where its allocation (32 MiB, a whole number of pages) does."""
+    size = torch.empty((), dtype=TYPES[vtype]).element_size()
+    whole = torch.zeros(32 * 2 ** 20 // size, dtype=TYPES[vtype], device="cuda")
+    rows = whole[whole.numel() - 9 * dim:].view(9, dim)
+    rows.copy_(values(torch.Generator().manual_seed(dim), 9, dim, vtype))
+    for fmt in FORMATS:
+        cache = Cache(vtype, dim, fmt, 0, 9)
+        cache.write(rows, torch.arange(9, device="cuda"))
+        codes, scales = cache.plain()
+        want_codes, want_scales = P.quantise(as64(rows), fmt, 0)
+        assert (codes == want_codes).all() and (scales == want_scales).all()
