@@ -389,13 +389,13 @@ __global__ __launch_bounds__(256) void adjust_scores_kernel(AdjustArgs a, uint32
       __syncthreads();   // the last piece's counts have been read
       for (uint32_t i = tid; i < COLUMNS / 4; i += 256) reinterpret_cast<u4 *>(times)[i] = reinterpret_cast<u4 *>(boost)[i] = u4{0, 0, 0, 0};
       __syncthreads();
-      for (int32_t i = s0 + (int32_t)tid; i < s1; i += 256) {
+      for (uint32_t i = (uint32_t)s0 + tid; i < (uint32_t)s1; i += 256) {   // (a list may end at the last 31-bit number)
         const uint32_t c = (uint32_t)a.r.seen_ids[i] - c0;
         if (c < mine) atomicAdd(&times[c], 1u);
       }
-      for (int32_t i = b0 + (int32_t)tid; i < b1; i += 256) {
+      for (uint32_t i = (uint32_t)b0 + tid; i < (uint32_t)b1; i += 256) {
         const uint32_t c = (uint32_t)a.r.bias_ids[i] - c0;
-        if (c < mine) atomicMax(&boost[c], (uint32_t)(i - b0) + 1);
+        if (c < mine) atomicMax(&boost[c], i - (uint32_t)b0 + 1);
       }
       __syncthreads();
     }
@@ -443,7 +443,7 @@ __global__ __launch_bounds__(256) void adjust_scores_kernel(AdjustArgs a, uint32
                 p = p > 0.0f ? p / rep : p * rep;
                 p -= __builtin_fmaf((float)n4[e], freq, pres);
               }
-              if (b4[e]) p += a.r.bias_values[b0 + b4[e] - 1];
+              if (b4[e]) p += a.r.bias_values[(uint32_t)b0 + b4[e] - 1];
               v[k][e] = distance ? 1.0f - p : p;
             }
         }

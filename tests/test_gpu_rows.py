@@ -787,3 +787,26 @@ def test_narrow_rows_up_to_the_end_of_an_allocation(vtype, dim):
         codes, scales = cache.plain()
         want_codes, want_scales = P.quantise(as64(rows), fmt, 0)
         assert (codes == want_codes).all() and (scales == want_scales).all()
+
+
+def test_adjust_lists_that_end_at_the_last_entry():
+    """Lists of 2^31 - 1 entries, the queries' own at their ends."""
+    n = 2 ** 31 - 1
+    seen = torch.empty(n, dtype=torch.int32, device="cuda")
+    seen[-300:] = torch.arange(300, dtype=torch.int32, device="cuda")
+    seen[-1] = 7
+    boosts = torch.empty(n, device="cuda")
+    boosts[-2:] = torch.tensor([2.0, 4.0], device="cuda")
+    scores = torch.ones((2, 400), device="cuda")
+    so = torch.tensor([n - 300, n - 1, n], dtype=torch.int32, device="cuda")
+    bo = torch.tensor([n - 2, n, n], dtype=torch.int32, device="cuda")
+    freq = torch.full((2,), 0.5, device="cuda")
+    rules = R.score_rules(seen_offsets=so.data_ptr(), seen_ids=seen.data_ptr(), n_seen=n, bias_offsets=bo.data_ptr(), bias_ids=seen.data_ptr(),
+                          bias_values=boosts.data_ptr(), n_bias=n, frequency=freq.data_ptr())
+    R.adjust_scores(rules, scores.data_ptr(), scores.data_ptr(), 2, 400, 400, None, stream())
+    want = np.ones((2, 400))
+    want[0, :299] -= 0.5
+    want[0, 298] += 2
+    want[0, 7] += 4
+    want[1, 7] -= 0.5
+    assert (scores.cpu().numpy() == want).all()
