@@ -810,3 +810,32 @@ def test_adjust_lists_that_end_at_the_last_entry():
     want[0, 7] += 4
     want[1, 7] -= 0.5
     assert (scores.cpu().numpy() == want).all()
+
+
+@pytest.mark.parametrize("partitions,queries", [(2048, 300), (2049, 5), (2300, 9), (9001, 200), (9001, 12000), (20011, 700), (2050, 2050 * 81)])
+def test_scores_of_thousands_of_partitions(partitions, queries):
+    """More than a thread of a workgroup takes, a few of them with queries; in the last case all."""
+    gen = torch.Generator().manual_seed(partitions + queries)
+    cache = filled(gen, P.F16, 16, R.INT8, 0, 512)
+    counts = torch.randint(0, 12, (partitions,), generator=gen).tolist()
+    counts[-1] = 9
+    who = torch.randint(0, partitions, (queries,), generator=gen)
+    if queries == 5:
+        who[:] = partitions - 1                                    # all of them ask the last partition
+    offsets = torch.searchsorted(who.sort().values, torch.arange(partitions + 1)).tolist()
+    pages = torch.randint(0, 64, (partitions, 2), generator=gen, dtype=torch.int32).cuda()
+    check_scores(cache.c, cache.codes, cache.scales, values(gen, queries, 16, P.F16), offsets, pages, 8, counts, R.PRODUCT, 12)
+
+
+def test_thousands_of_partitions_with_offsets_out_of_order_stay_in_bounds():
+    gen = torch.Generator().manual_seed(3)
+    cache = filled(gen, P.BF16, 16, R.INT4, 0, 512)
+    n = 5000
+    offsets = torch.randint(-50, 400, (n + 1,), generator=gen).to(torch.int32).cuda()
+    counts = torch.randint(-5, 40, (n,), generator=gen).to(torch.int32).cuda()
+    pages = torch.randint(-2, 70, (n, 2), generator=gen).to(torch.int32).cuda()
+    q = values(gen, 300, 16, P.BF16)
+    out = torch.full((302, 16), 5.0, device="cuda")
+    cache.c.partition_scores(q.data_ptr(), 16, 300, offsets.data_ptr(), n, pages.data_ptr(), 2, 8, counts.data_ptr(), R.PRODUCT, out[1:].data_ptr(), 16, stream())
+    torch.cuda.synchronize()
+    assert (out[0] == 5).all() and (out[301] == 5).all()
