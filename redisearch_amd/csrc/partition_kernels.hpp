@@ -315,6 +315,8 @@ struct Piece {
 // back as operands; the sixteen-byte chunks of a row change places with its number, so that neither side meets a bank twice.
 // ONCE: the rows are read past the caches' keeping (a batch of 256 over 64 partitions: 57 us for 63; with three query tiles a
 // partition, which read the rows three times, 170 for 134).
+// 256 queries, 64 partitions x 5461 rows of 768: INT8 with fp16 queries, a scale each 128, 55 us (5.1 TB/s); bf16 rows as they are 94
+// (5.8); x 32 768 rows: INT8 299 (5.7), with fp32 queries 303, INT4 177 (5.0); fp32 rows x 8192 267 (6.1).
 // Every part of the loop is in the code once: a small call is mostly the first pass of its instructions through the caches.
 template <int FMT, int Q, int W, int QT, int S, int WAVES, bool ONCE>
 __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionArgs a, FastDiv page) {
@@ -591,13 +593,16 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
   }
 }
 
-// Many queries a partition: the matrix cores' work.  A workgroup has a run of tiles of 128 queries x 128 rows, a wavefront 64 x 64 of
-// each; both sides go through LDS as operands of the 32 x 32 x 16 product, the rows' codes widened once on the way there.  A stage is
-// 64 elements in two halves: one half is multiplied, the next is in the other half of LDS, and the two behind it are on their way in
-// registers, of this tile or the next one's (with one on its way every half waited for memory: 132 us instead of the figure at the
-// launch below).  In LDS an operand's 32 rows change places with the number of its eight elements, so that neither side meets a bank
-// twice.  A block's products are summed by themselves and multiplied by the row's scale at every FLUSH elements.
-// rows of a tile: 128 queries meet 256 rows where the sums of a tile are all that the registers hold
+// Many queries a partition: the matrix cores' work.  A workgroup has a run of tiles of 128 queries x MANY_ROWS rows, a wavefront 64 x 64
+// or 128 x 64 of each; both sides go through LDS as operands of the 32 x 32 x 16 product, the rows' codes widened once on the way
+// there.  A stage is 64 elements (32 where both sides are fp32) in two halves: one half is multiplied, the next is in the other half of
+// LDS, and the two behind it are on their way in registers, of this tile or the next one's; with one on its way every half waited for
+// memory.  In LDS an operand's 32 rows change places with the number of its eight elements, so that neither side meets a bank twice.  A
+// block's products are summed by themselves and multiplied by the row's scale at every FLUSH elements.
+// 16 partitions x 512 queries x 6144 bf16 rows of 768: 92 us, 0.84 PFLOP/s, of which the products are three quarters (1.2 - 1.3
+// PFLOP/s, what a large matrix product of the library reaches) and the scores' way to memory, 201 MB that all workgroups write at about
+// the same time, the rest.  (Begun at different times, or a tile's scores kept for the next tile's products to hide: no faster.)
+// rows of a tile: 128 queries meet 256 rows where the sums of a tile are all that the registers hold, for half the reads of the queries
 template <int FMT, int Q>
 constexpr int MANY_ROWS = FMT == NATIVE && Q != F32 ? 256 : 128;
 template <int FMT, int Q, int FLUSH>
@@ -834,7 +839,7 @@ __global__ __launch_bounds__(256, 2) void partition_many_kernel(PartitionArgs a,
         }
       }
       if (a.form == RSGPU_SCORES_DISTANCE) p = 1.0f - p;
-      __builtin_nontemporal_store(there >> y & 1 ? p : gone, at + (uint64_t)q * a.ld);
+      __builtin_nontemporal_store(there >> y & 1 ? p : gone, at + (uint64_t)q * a.ld);   // (kept in the caches, rows of 1536 took 139 us for 106)
     }
   };
   const std::integral_constant<int, 0> first_half;

@@ -92,11 +92,7 @@ class RowCache:
 
 def score_rules(form=PRODUCT, device=-1, **arrays):
     """RSGPU_ScoreRules by field name; what is not given does not apply."""
-    r = ScoreRules()
-    r.device, r.form = device, form
-    for name, value in arrays.items():
-        setattr(r, name, value)
-    return r
+    return ScoreRules(device=device, form=form, **arrays)
 
 
 def adjust_scores(rules, scores_in, scores_out, n_queries, n_columns, ld, counts=None, stream=None):
