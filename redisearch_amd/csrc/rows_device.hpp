@@ -14,6 +14,7 @@ typedef u4 u4_any __attribute__((aligned(2)));
 typedef u4 u4_any4 __attribute__((aligned(4)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef uint16_t ushort2v __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -106,6 +107,24 @@ struct Raw8 {
     for (int i = 0; i < 2 * (int)elem_size<T>; i++) {
       if constexpr (T == F32) w[i / 4][i % 4] = (uint32_t)i < valid ? w[i / 4][i % 4] : 0;
       else w[0][i] &= (uint32_t)(2 * i + 1) < valid ? 0xffffffffu : (uint32_t)(2 * i) < valid ? 0xffffu : 0;
+    }
+  }
+  // the bits, as fp32, of the largest magnitude: as integers, so that an infinity or a NaN is larger than every number
+  __device__ __forceinline__ uint32_t most() const {
+    if constexpr (T == F32) {
+      uint32_t a = 0;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const uint32_t b = w[i / 4][i % 4] & 0x7fffffffu;
+        a = a > b ? a : b;
+      }
+      return a;
+    } else {   // two at a time
+      ushort2v a = __builtin_bit_cast(ushort2v, w[0][0] & 0x7fff7fffu);
+#pragma unroll
+      for (int i = 1; i < 4; i++) a = __builtin_elementwise_max(a, __builtin_bit_cast(ushort2v, w[0][i] & 0x7fff7fffu));
+      const uint32_t b = a[0] > a[1] ? a[0] : a[1];
+      return T == BF16 ? b << 16 : __float_as_uint(f16_to_f32(b));
     }
   }
   __device__ __forceinline__ void floats(float (&v)[8]) const {

@@ -7,16 +7,10 @@ namespace {
 
 // ---- writing ---------------------------------------------------------------------------------------------------------------
 
-// the bits of the largest magnitude: as integers, so that an infinity or a NaN is larger than every number
-__device__ __forceinline__ uint32_t most8(const float (&v)[8]) {
-  uint32_t a = 0;
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
-    a = a > b ? a : b;
-  }
-  return a;
-}
+// Pieces of a row that a thread of a workgroup has under way.  Writing (400 009 fp16 rows of 96 to INT4 / of 100 to INT8, in order, us): 1
+// 25.0 / 27.2, 2 21.7 / 25.3, 4 23.8 / 26.1 (its registers leave five wavefronts a SIMD of eight).  Reading (fp16 rows of 768 from INT4 /
+// fp32 ones from INT8): 2 102 / 99, 4 85 / 84, 8 89 / 84.
+constexpr int WRITE_UNDER_WAY = 2, READ_UNDER_WAY = 4;
 
 constexpr uint32_t SMALLEST = (127 - 100) << 23;   // 2^-100: below, a block is kept as zeros
 
@@ -80,13 +74,14 @@ __device__ __forceinline__ void encode8(const float (&v)[8], float s, float inv,
     uint32_t q[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) q[i] = __float_as_uint(u[i]);
+    const auto bytes4 = [&](int i, int step) {   // the low bytes of q[i], q[i + step], ...
+      return __builtin_amdgcn_perm(__builtin_amdgcn_perm(q[i + 3 * step], q[i + 2 * step], 0x0c0c0400u), __builtin_amdgcn_perm(q[i + step], q[i], 0x0c0c0400u), 0x05040100u);
+    };
     if constexpr (FMT == INT8) {
-#pragma unroll
-      for (int i = 0; i < 2; i++)
-        c[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(q[4 * i + 3], q[4 * i + 2], 0x0c0c0400u), __builtin_amdgcn_perm(q[4 * i + 1], q[4 * i], 0x0c0c0400u), 0x05040100u);
+      c[0] = bytes4(0, 1);
+      c[1] = bytes4(4, 1);
     } else {
-#pragma unroll
-      for (int i = 0; i < 8; i++) c[0] |= (q[i] & 15u) << (4 * i);
+      c[0] = (bytes4(0, 2) & 0x0f0f0f0fu) | (bytes4(1, 2) << 4 & 0xf0f0f0f0u);
     }
   }
 }
@@ -118,13 +113,14 @@ __device__ __forceinline__ uint32_t most_of_lanes(uint32_t x) {
 }
 
 // Blocks of 8 L elements: L neighbouring lanes have a block, eight elements each, and find its largest magnitude among themselves, so a
-// row is read once and neither LDS nor a second pass is needed.  The rows' bytes are what it takes; a thread has four eights under way.
-// 262 144 bf16 rows of 768 to E4M3, a scale each 128, into slots in any order: 112 us, 5.4 TB/s (a copy of as much memory: 5.2); 50 021
-// fp32 rows of 1000, 1003 apart, to INT8: 52 us, 4.9 TB/s.  A single row: 2.4 us, an empty kernel's time.
+// row is read once and neither LDS nor a second pass is needed.  The rows' bytes are what it takes.
+// 262 144 bf16 rows of 768 to E4M3, a scale each 128, into slots in any order: 111 us, 5.5 TB/s (a copy of as much memory: 5.2); 50 021
+// fp32 rows of 1000, 1003 apart, to INT8: 50 us, 5.0 TB/s; 400 009 fp16 rows of 100 to INT4: 28 us, 4.1 TB/s, where the arithmetic
+// counts too (130 instructions for eight elements).  A single row: 2.4 us, an empty kernel's time.
 template <int T, int FMT, int L>
 __global__ __launch_bounds__(256) void row_write_kernel(RowCacheArgs c, const void *rows, uint32_t stride, const int64_t *slots, uint32_t n,
                                                         uint32_t rows_per_wg, FastDiv chunks) {
-  constexpr int U = 4;
+  constexpr int U = WRITE_UNDER_WAY;
   const uint32_t padded = rows_padded(c.dim);
   const uint64_t row_stride = (uint64_t)stride * elem_size<T>;
   for (uint64_t first = (uint64_t)blockIdx.x * rows_per_wg; first < n; first += (uint64_t)gridDim.x * rows_per_wg) {
@@ -154,7 +150,7 @@ __global__ __launch_bounds__(256) void row_write_kernel(RowCacheArgs c, const vo
         const uint32_t at = chunk[u] * 8;
         raw[u].cut(at < c.dim ? c.dim - at : 0);
         raw[u].floats(v);
-        const uint32_t most = most_of_lanes<L>(most8(v));
+        const uint32_t most = most_of_lanes<L>(raw[u].most());
         float s, inv;
         scale_of<FMT>(most, s, inv);
         uint32_t code[2];
@@ -195,8 +191,7 @@ __global__ __launch_bounds__(256) void row_write_whole_kernel(RowCacheArgs c, co
       for (int k = 0; k < C; k++) {
         const uint32_t at = (k * 64 + lane) * 8;
         raw[k].cut(at < c.dim ? c.dim - at : 0);
-        raw[k].floats(v);
-        const uint32_t o = most8(v);
+        const uint32_t o = raw[k].most();
         most = most > o ? most : o;
       }
       most = most_of_lanes<64>(most);
@@ -210,8 +205,9 @@ __global__ __launch_bounds__(256) void row_write_whole_kernel(RowCacheArgs c, co
       }
     } else {
       for (uint32_t at = lane * 8; at < c.dim; at += 512) {
-        load8<T>(row, at, c.dim - at, v);
-        const uint32_t o = most8(v);
+        Raw8<T> raw;
+        raw.load(row, at, c.dim - at);
+        const uint32_t o = raw.most();
         most = most > o ? most : o;
       }
       most = most_of_lanes<64>(most);
@@ -226,7 +222,7 @@ __global__ __launch_bounds__(256) void row_write_whole_kernel(RowCacheArgs c, co
   }
 }
 
-// rows kept as they are: sixteen bytes a thread (400 009 bf16 rows of 128: 33 us, 6.4 TB/s)
+// rows kept as they are: sixteen bytes a thread (400 009 bf16 rows of 128: 31.6 us, 6.6 TB/s)
 template <int T>
 __global__ __launch_bounds__(256) void row_copy_in_kernel(RowCacheArgs c, const void *rows, uint32_t stride, const int64_t *slots, uint32_t n,
                                                           uint32_t rows_per_wg, FastDiv chunks) {
@@ -287,14 +283,14 @@ __device__ __forceinline__ void decode(const uint32_t (&w)[2], float (&v)[E]) {
 }
 
 // Sixteen bytes of output a thread, neighbouring threads' next to each other: the output is most of the bytes, so its lines are written
-// whole and the codes, half to an eighth as many bytes, are read in whatever pieces that makes.  A thread has four under way, which hides
+// whole and the codes, half to an eighth as many bytes, are read in whatever pieces that makes.  Four of a thread under way hide
 // slot -> codes -> output, three steps behind each other.  131 072 fp32 rows of 768 from INT8, slots in any order: 109 us, 4.7 TB/s.  Of
 // narrow rows in any order the lines of codes and scales are read for a part of each: 400 009 fp16 rows of 100 from INT4 30 us, in
 // order 22 us (5.2 TB/s).
 template <int T, int FMT>
 __global__ __launch_bounds__(256) void row_read_kernel(RowCacheArgs c, const int64_t *slots, uint32_t n, void *out, uint32_t stride,
                                                        uint32_t rows_per_wg, FastDiv chunks, FastDiv block) {
-  constexpr int U = 4, E = 16 / elem_size<T>;
+  constexpr int U = READ_UNDER_WAY, E = 16 / elem_size<T>;
   for (uint64_t first = (uint64_t)blockIdx.x * rows_per_wg; first < n; first += (uint64_t)gridDim.x * rows_per_wg) {
     const uint32_t mine = n - first < rows_per_wg ? (uint32_t)(n - first) : rows_per_wg, all = mine * chunks.d;
     const uint64_t row_stride = (uint64_t)stride * elem_size<T>;
@@ -474,9 +470,9 @@ __global__ __launch_bounds__(256) void adjust_scores_kernel(AdjustArgs a, uint32
 constexpr uint64_t MOST_WORKGROUPS = 1 << 20;
 uint32_t workgroups(uint64_t work) { return (uint32_t)(work < MOST_WORKGROUPS ? work : MOST_WORKGROUPS); }
 
-// rows of a workgroup so that it has a few chunks a thread, with enough workgroups to fill the chip first
-uint32_t rows_a_workgroup(uint32_t n, uint32_t chunks) {
-  uint32_t rows = (1024 + chunks - 1) / chunks;
+// rows of a workgroup so that it has about `most` chunks, with enough workgroups to fill the chip first
+uint32_t rows_a_workgroup(uint32_t n, uint32_t chunks, uint32_t most) {
+  uint32_t rows = (most + chunks - 1) / chunks;
   while (rows > 1 && (n + rows - 1) / rows < 2048) rows = (rows + 1) / 2;
   return rows;
 }
@@ -494,7 +490,7 @@ void write_as(const RowCacheArgs &c, const void *rows, uint32_t stride, const in
   // the lanes of a block, or of a row that is one
   uint32_t lanes = 4;
   while (lanes * 8 < (c.nb == 1 ? rows_padded(c.dim) : c.block)) lanes *= 2;
-  const uint32_t chunks = c.nb * lanes, per = rows_a_workgroup(n, chunks);
+  const uint32_t chunks = c.nb * lanes, per = rows_a_workgroup(n, chunks, 256 * WRITE_UNDER_WAY);
   const dim3 grid(workgroups(((uint64_t)n + per - 1) / per));
   const FastDiv d(chunks);
   switch (lanes) {
@@ -513,7 +509,7 @@ void write_from(const RowCacheArgs &c, const void *rows, uint32_t stride, const 
     case E4M3: return write_as<T, E4M3>(c, rows, stride, slots, n, s);
     case INT4: return write_as<T, INT4>(c, rows, stride, slots, n, s);
     default: {
-      const uint32_t chunks = c.row_bytes / 16, per = rows_a_workgroup(n, chunks);
+      const uint32_t chunks = c.row_bytes / 16, per = rows_a_workgroup(n, chunks, 256 * WRITE_UNDER_WAY);
       hipLaunchKernelGGL((row_copy_in_kernel<T>), dim3(workgroups(((uint64_t)n + per - 1) / per)), dim3(256), 0, s, c, rows, stride, slots, n, per, FastDiv(chunks));
     }
   }
@@ -522,7 +518,7 @@ void write_from(const RowCacheArgs &c, const void *rows, uint32_t stride, const 
 template <int T>
 void read_to(const RowCacheArgs &c, const int64_t *slots, uint32_t n, void *out, uint32_t stride, hipStream_t s) {
   constexpr uint32_t E = 16 / elem_size<T>;
-  const uint32_t chunks = (c.dim + E - 1) / E, per = rows_a_workgroup(n, chunks);
+  const uint32_t chunks = (c.dim + E - 1) / E, per = rows_a_workgroup(n, chunks, 256 * READ_UNDER_WAY);
   const dim3 grid(workgroups(((uint64_t)n + per - 1) / per));
   const FastDiv d(chunks), b(c.block);
   switch (c.format) {
