@@ -600,8 +600,10 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
 // memory.  In LDS an operand's 32 rows change places with the number of its eight elements, so that neither side meets a bank twice.  A
 // block's products are summed by themselves and multiplied by the row's scale at every FLUSH elements.
 // 16 partitions x 512 queries x 6144 bf16 rows of 768: 92 us, 0.84 PFLOP/s, of which the products are three quarters (1.2 - 1.3
-// PFLOP/s, what a large matrix product of the library reaches) and the scores' way to memory, 201 MB that all workgroups write at about
-// the same time, the rest.  (Begun at different times, or a tile's scores kept for the next tile's products to hide: no faster.)
+// PFLOP/s, what a large matrix product of the library reaches) and the scores' way to memory, 201 MB, the rest: stores and loads are
+// counted in one order, so the next tile's rows are waited for behind this one's scores (rows of 64 elements, almost nothing but
+// scores, take 32 us where 4096 rows of 768 take 66).  Workgroups begun at different times, four columns a lane's store, a tile's scores
+// kept in registers for the next tile's products to hide: no faster.
 // rows of a tile: 128 queries meet 256 rows where the sums of a tile are all that the registers hold, for half the reads of the queries
 template <int FMT, int Q>
 constexpr int MANY_ROWS = FMT == NATIVE && Q != F32 ? 256 : 128;
