@@ -593,23 +593,21 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
   }
 }
 
-// Many queries a partition: the matrix cores' work.  A workgroup has a run of tiles of 128 queries x MANY_ROWS rows, a wavefront 64 x 64
+// Many queries a partition: the matrix cores' work.  A workgroup has a run of tiles of 128 queries x TR = 128 or 256 rows, a wavefront 64 x 64
 // or 128 x 64 of each; both sides go through LDS as operands of the 32 x 32 x 16 product, the rows' codes widened once on the way
 // there.  A stage is 64 elements (32 where both sides are fp32) in two halves: one half is multiplied, the next is in the other half of
 // LDS, and the two behind it are on their way in registers, of this tile or the next one's; with one on its way every half waited for
 // memory.  In LDS an operand's 32 rows change places with the number of its eight elements, so that neither side meets a bank twice.  A
-// block's products are summed by themselves and multiplied by the row's scale at every FLUSH elements.
+// block's products are summed by themselves and multiplied by the row's scale at every FLUSH elements (0: rows that have one scale or
+// none, at the end).
 // 16 partitions x 512 queries x 6144 bf16 rows of 768: 92 us, 0.84 PFLOP/s, of which the products are three quarters (1.2 - 1.3
 // PFLOP/s, what a large matrix product of the library reaches) and the scores' way to memory, 201 MB, the rest: stores and loads are
 // counted in one order, so the next tile's rows are waited for behind this one's scores (rows of 64 elements, almost nothing but
 // scores, take 32 us where 4096 rows of 768 take 66).  Workgroups begun at different times, four columns a lane's store, a tile's scores
 // kept in registers for the next tile's products to hide: no faster.
-// rows of a tile: 128 queries meet 256 rows where the sums of a tile are all that the registers hold, for half the reads of the queries
-template <int FMT, int Q>
-constexpr int MANY_ROWS = FMT == NATIVE && Q != F32 ? 256 : 128;
-template <int FMT, int Q, int FLUSH>
+template <int FMT, int Q, int FLUSH, int TR>
 __global__ __launch_bounds__(256, 2) void partition_many_kernel(PartitionArgs a, FastDiv page) {
-  constexpr int TQ = 128, TR = MANY_ROWS<FMT, Q>, X = TR / 64, Y = 2, KC = FMT == NATIVE && Q == F32 ? 16 : 32, QP = Q == F32 ? 3 : 1, RP = FMT == NATIVE && Q == F32 ? 3 : 1;
+  constexpr int TQ = 128, X = TR / 64, Y = 2, KC = FMT == NATIVE && Q == F32 ? 16 : 32, QP = Q == F32 ? 3 : 1, RP = FMT == NATIVE && Q == F32 ? 3 : 1;
   constexpr int C8 = KC / 8;                                                 // eights of a half
   constexpr int PIECE = FMT == NATIVE ? 8 : FMT == INT4 ? 32 : 16;           // elements of a row that a thread loads together
   constexpr int PIECE_BYTES = FMT == NATIVE ? 8 * elem_size<Q> : 16, PU = PIECE_BYTES / 16;
@@ -703,7 +701,7 @@ __global__ __launch_bounds__(256, 2) void partition_many_kernel(PartitionArgs a,
 #pragma unroll
       for (int u = 0; u < PU; u++) row_held[H][i][u] = p[u];
     }
-    if (FMT != NATIVE) {
+    if (FMT != NATIVE && (FLUSH || H == 1)) {
       const uint32_t b = base / a.c.block;
       scale_held[H] = scale_source[b < a.c.nb ? b : a.c.nb - 1];
     }
@@ -762,12 +760,13 @@ __global__ __launch_bounds__(256, 2) void partition_many_kernel(PartitionArgs a,
         for (int p = 0; p < RP; p++) r_lds[H][place(TR, tid % NP * (PIECE / 8) + f, RP, p, (i * 256 + tid) / NP)] = w[p];
       }
     }
-    if (FMT != NATIVE && tid < TR) s_lds[H][tid] = scale_held[H];
+    if (FMT != NATIVE && (FLUSH || H == 1) && tid < TR) s_lds[H][tid] = scale_held[H];
   };
 
   // ---- the products
   const uint32_t wave_q = X == 2 ? wave / 2 * 64 : 0, wave_r = X == 2 ? wave % 2 * 64 : wave * 64;
   f32x16 acc[X][Y], part[X][Y];
+  float row_scale[Y];
 #pragma unroll
   for (int x = 0; x < X; x++)
 #pragma unroll
@@ -776,8 +775,8 @@ __global__ __launch_bounds__(256, 2) void partition_many_kernel(PartitionArgs a,
       for (int r = 0; r < 16; r++) acc[x][y][r] = 0.0f;
   const auto multiply = [&](auto which) {
     constexpr int H = decltype(which)::value;
-    constexpr bool FRESH = FMT != NATIVE && (H == 0 || FLUSH == KC);   // a block's sums begin
-    f32x16(&sum)[X][Y] = FMT == NATIVE ? acc : part;
+    constexpr bool FRESH = FLUSH && (H == 0 || FLUSH == KC);   // a block's sums begin
+    f32x16(&sum)[X][Y] = FLUSH ? part : acc;
 #pragma unroll
     for (int k = 0; k < KC / 16; k++) {
       u4 q[X][QP], r[Y][RP];
@@ -803,7 +802,11 @@ __global__ __launch_bounds__(256, 2) void partition_many_kernel(PartitionArgs a,
               }
           }
     }
-    if (FMT != NATIVE && (H == 1 || FLUSH == KC)) {
+    if (FMT != NATIVE && !FLUSH && H == 1) {   // here, where nobody writes them
+#pragma unroll
+      for (int y = 0; y < Y; y++) row_scale[y] = s_lds[1][wave_r + y * 32 + col];
+    }
+    if (FLUSH && (H == 1 || FLUSH == KC)) {
 #pragma unroll
       for (int y = 0; y < Y; y++) {
         const float scale = s_lds[H][wave_r + y * 32 + col];
@@ -832,6 +835,7 @@ __global__ __launch_bounds__(256, 2) void partition_many_kernel(PartitionArgs a,
       const uint32_t q = t.q0 + wave_q + x * 32 + 8 * (r / 4) + 4 * half_wave + r % 4;
       if (q >= t.q_end) continue;
       float p = sums[x][y][r] * CODE_UNIT<FMT, Q>;
+      if (FMT != NATIVE && !FLUSH) p *= row_scale[y];
       if constexpr (FMT == NATIVE && Q == F32) {
         // an infinity meets the other side's planes, some of them 0: the sum is taken again, element by element
         if (p != p && (there >> y & 1)) {
@@ -926,6 +930,13 @@ uint32_t resident(const void *kernel, uint32_t threads) {
 //   INT4 of 100 wide, 300 x 1000 (rows of 64 bytes)   27 / 35, 29 / 41, 45 / 47 / 51
 constexpr uint32_t TWO_TILES = 13, MANY = 48, MANY_LATE = 80;   // late: fp32 queries, and rows of few chunks
 
+// Tiles of 256 rows, for half the reads of the queries, where the sums of a tile are all that the registers hold (16-bit queries, rows of
+// one scale or none) and there are as many tiles as the device holds at once.  16 partitions x 4096 rows of 768, 128 / 256 rows, us:
+//   INT8, one scale, fp16 queries: 90 queries a partition (432 tiles at most) 21.8 / 25.2, 128 (512) 25.7 / 25.8, 512 (1280) 74 / 71
+//   INT4, one scale, bf16 queries, 512: 81 / 66; bf16 rows as they are 68 / 66
+// (Scaled at every 64 elements, as rows of more scales are, the 512 take 87 and 93.)
+constexpr uint64_t MANY_TALL = 512;
+
 // Workgroups of four waves where there are few tiles of theirs: one's waves wait for each other while the queries are
 // laid out, and four have less to wait for.  us with the wide ones / with four waves (int8 rows of 768, one query each):
 //   fp32 queries: 8 x 700 (88 tiles) 14.4 / 8.3, 64 x 512 (512) 14.6 / 11.7, 64 x 1024 (1088) 15.4 / 19.3
@@ -953,14 +964,20 @@ void scores_as(const PartitionArgs &a, hipStream_t s) {
   for (uint32_t c : {8u, 4u})
     if (!(widest && c == 4) && (chunks + c - 1) / c * c < (chunks + cs - 1) / cs * cs) cs = c;
   if (each >= (Q == F32 || cs == 4 ? MANY_LATE : MANY) && a.c.dim >= 8) {
-    const auto many = [&](auto kernel) {
-      dim3 g = grid(128, MANY_ROWS<FMT, Q>, resident(reinterpret_cast<const void *>(kernel), 256));
+    const auto many = [&](auto kernel, uint32_t rows) {
+      dim3 g = grid(128, rows, resident(reinterpret_cast<const void *>(kernel), 256));
       g.x = (g.x + DIES - 1) / DIES * DIES;
       hipLaunchKernelGGL(kernel, g, dim3(256), 0, s, a, page);
     };
-    if constexpr (FMT == NATIVE) many(partition_many_kernel<FMT, Q, 64>);
-    else if (a.c.block == 32) many(partition_many_kernel<FMT, Q, 32>);
-    else many(partition_many_kernel<FMT, Q, 64>);
+    if (a.c.nb <= 1) {
+      if constexpr (Q != F32) {
+        if (tiles(128, 256) >= MANY_TALL) return many(partition_many_kernel<FMT, Q, 0, 256>, 256);
+      }
+      many(partition_many_kernel<FMT, Q, 0, 128>, 128);
+    } else if constexpr (FMT != NATIVE) {
+      if (a.c.block == 32) many(partition_many_kernel<FMT, Q, 32, 128>, 128);
+      else many(partition_many_kernel<FMT, Q, 64, 128>, 128);
+    }
     return;
   }
   const auto few = [&](auto w) {

@@ -839,3 +839,18 @@ def test_thousands_of_partitions_with_offsets_out_of_order_stay_in_bounds():
     cache.c.partition_scores(q.data_ptr(), 16, 300, offsets.data_ptr(), n, pages.data_ptr(), 2, 8, counts.data_ptr(), R.PRODUCT, out[1:].data_ptr(), 16, stream())
     torch.cuda.synchronize()
     assert (out[0] == 5).all() and (out[301] == 5).all()
+
+
+@pytest.mark.parametrize("vtype,fmt,block", ALL)
+@pytest.mark.parametrize("dim", [9, 40, 200, 768])
+def test_scores_of_many_queries_in_tables_of_many_rows(vtype, fmt, block, dim):
+    """The tiles of 256 rows (16-bit queries, rows of one scale or none) and those of 128, at their ends: partitions of one row, of a
+    tile but one, of a tile and one, without queries."""
+    gen = torch.Generator().manual_seed(dim + fmt)
+    counts, page_rows = [255, 1, 700, 257], 48
+    need = [-(-n // page_rows) for n in counts]
+    cache = filled(gen, vtype, dim, fmt, block, page_rows * sum(need))
+    pages = torch.full((4, max(need)), -1, dtype=torch.int32)
+    pages[torch.arange(max(need))[None, :] < torch.tensor(need)[:, None]] = torch.randperm(sum(need), generator=gen).to(torch.int32)
+    pages[2, 3] = -1                                                   # one that is gone
+    check_scores_in_a_wide_table(cache, values(gen, 521, dim, vtype), [0, 129, 257, 257, 520], pages.cuda(), page_rows, counts, R.DISTANCE, 704)
