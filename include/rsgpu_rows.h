@@ -60,7 +60,8 @@ int RSGPU_RowCache_Read(const RSGPU_RowCache *cache, const int64_t *slots, size_
  * j % page_rows  of the cache, and the queries query_offsets[g] .. query_offsets[g + 1] - 1 (n_partitions + 1 offsets that do
  * not fall; queries before the first and behind the last belong to nobody).  For each such query m and each j:
  *   scores[m * ld + j] = p  (PRODUCT)  or  1 - p  (DISTANCE: VecSim's inner-product / cosine distance),
- *   p = sum over the elements of query * row, accumulated in fp32
+ *   p = sum over the elements of query * row, accumulated in fp32; of rows kept in codes no sum on the way leaves fp32's range where p
+ *   does not.  Bits of an element below 2^-107 and of p below 2^-119 are not kept.
  * A page that is negative or not in the cache: its rows score -inf (PRODUCT) / +inf (DISTANCE), behind every other.  All other
  * cells of `scores` are left as they were.  A row count counts as no more than max_pages * page_rows and ld; a range of queries
  * that falls or leaves [0, n_queries] is cut to it. */

@@ -66,9 +66,23 @@ __device__ __forceinline__ void planes8(const float (&v)[8], u4 (&p)[3]) {
   }
 }
 
-// eight codes -> eight 16-bit floats (INT4 with bf16: sixteenths of the codes, CODE_UNIT)
-template <int FMT, int Q>
-constexpr float CODE_UNIT = FMT == INT4 && Q != F16 ? 16.0f : 1.0f;
+// bf16 and fp32 queries reach 2^128, and codes are summed before they meet their scale: 65 536 elements times codes of up to 448 would
+// leave fp32 where the score, of rows of thousandths, does not.  So one side goes in by SHRUNK, exactly, and the score is multiplied by
+// what that was when its scales are in it: no sum overflows that is not an infinity in the end.  (fp16 queries times codes stay below
+// 2^41.)  It costs what of a query's elements lies below 2^-107, or of a score below 2^-119.  Which side: codes where their conversion
+// does it for nothing (E4M3) or where rows are converted no more often than queries (many queries: 1 - 3 % of the time), else queries,
+// once a partition (8 x 700 INT8 rows of 768, fp32 queries: queries 8.3 us as without, codes 8.8).
+constexpr float SHRUNK = 0x1p-26f;
+enum { BY_NOTHING = 0, BY_CODES = 1, BY_QUERIES = 2 };
+template <int FMT, int Q, bool MANY>
+constexpr int SHRINK = FMT == NATIVE || Q == F16 ? BY_NOTHING : FMT == E4M3 || MANY ? BY_CODES : BY_QUERIES;
+
+// eight codes -> eight 16-bit floats, STEP for a code of 1 (INT4 with bf16: by sixteenths if not by SHRUNK)
+template <int FMT, int Q, int BY>
+constexpr float STEP = BY == BY_CODES ? SHRUNK : FMT == INT4 && Q != F16 ? 0.0625f : 1.0f;
+// what a sum of products is multiplied by
+template <int FMT, int Q, int BY>
+constexpr float UNIT = 1.0f / STEP<FMT, Q, BY> / (BY == BY_QUERIES ? SHRUNK : 1.0f);
 
 __device__ __forceinline__ uint32_t minus2(uint32_t x, float y) {
   half2v h;
@@ -78,8 +92,9 @@ __device__ __forceinline__ uint32_t minus2(uint32_t x, float y) {
   return x;
 }
 
-template <int FMT, int Q>
+template <int FMT, int Q, int BY>
 __device__ __forceinline__ u4 widen8(uint32_t w0, uint32_t w1) {
+  constexpr float ONE = STEP<FMT, Q, BY>;
   u4 r;
   if constexpr (FMT == E4M3) {
 #pragma unroll
@@ -91,7 +106,7 @@ __device__ __forceinline__ u4 widen8(uint32_t w0, uint32_t w1) {
         __builtin_memcpy(&x, &h, 4);
         r[i] = x;
       } else {
-        const bf16x2 h = i % 2 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false);
+        const bf16x2 h = i % 2 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, ONE, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, ONE, false);
         uint32_t x;
         __builtin_memcpy(&x, &h, 4);
         r[i] = x;
@@ -116,7 +131,14 @@ __device__ __forceinline__ u4 widen8(uint32_t w0, uint32_t w1) {
       else f[i] = __builtin_amdgcn_cvt_off_f32_i4((int)(w0 >> (4 * i)));   // the low four bits, two's complement, by 16
     }
 #pragma unroll
-    for (int i = 0; i < 4; i++) r[i] = upper2(__float_as_uint(f[2 * i]), __float_as_uint(f[2 * i + 1]));
+    for (int i = 0; i < 4; i++) {
+      uint32_t two = upper2(__float_as_uint(f[2 * i]), __float_as_uint(f[2 * i + 1]));
+      if constexpr (BY == BY_CODES) {   // off the exponents; 0 (+0: it comes from an integer) stays 0 by saturation
+        constexpr uint16_t by = (FMT == INT4 ? 22 : 26) << 7;
+        two = __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(__builtin_bit_cast(ushort2v, two), ushort2v{by, by}));
+      }
+      r[i] = two;
+    }
   }
   return r;
 }
@@ -241,23 +263,31 @@ __device__ __forceinline__ Run find_run(const PartitionArgs &a, uint32_t tq, uin
   return run;
 }
 
+// two bf16 in a dword by SHRUNK
+__device__ __forceinline__ uint32_t shrink2(uint32_t w) {
+  return upper2(__float_as_uint(__uint_as_float(w << 16) * SHRUNK), __float_as_uint(__uint_as_float(w & 0xffff0000u) * SHRUNK));
+}
+
 // eight elements of a query as 16-bit fragments (an fp32 query: three planes)
-template <int Q>
+template <int Q, int BY>
 __device__ __forceinline__ void stage8(const PartitionArgs &a, uint32_t query, uint32_t at, u4 (&w)[Q == F32 ? 3 : 1]) {
   const uint8_t *src = static_cast<const uint8_t *>(a.queries) + (size_t)query * a.stride * elem_size<Q>;
   if constexpr (Q == F32) {
     float v[8];
     load8<F32>(src, at, at < a.c.dim ? a.c.dim - at : 0, v);
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] *= BY == BY_QUERIES ? SHRUNK : 1.0f;
     planes8(v, w);
   } else if (at + 8 <= a.c.dim) {
-    w[0] = *reinterpret_cast<const u4_any *>(src + at * 2);
+    const u4 x = *reinterpret_cast<const u4_any *>(src + at * 2);
+    w[0] = BY == BY_QUERIES ? u4{shrink2(x[0]), shrink2(x[1]), shrink2(x[2]), shrink2(x[3])} : x;
   } else {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       uint32_t x = 0;
       if (at + 2 * i < a.c.dim) x = reinterpret_cast<const uint16_t *>(src)[at + 2 * i];
       if (at + 2 * i + 1 < a.c.dim) x |= (uint32_t)reinterpret_cast<const uint16_t *>(src)[at + 2 * i + 1] << 16;
-      w[0][i] = x;
+      w[0][i] = BY == BY_QUERIES ? shrink2(x) : x;
     }
   }
 }
@@ -283,7 +313,7 @@ __device__ __forceinline__ uint32_t next_asked(const PartitionArgs &a, uint32_t 
 }
 
 // W neighbouring elements of a row, as a lane takes them from LDS
-template <int FMT, int Q, int W>
+template <int FMT, int Q, int W, int BY>
 struct Piece {
   static constexpr int BYTES = FMT == NATIVE ? W * elem_size<Q> : FMT == INT4 ? W / 2 : W;
   static constexpr int PLANES = FMT == NATIVE && Q == F32 ? 3 : 1;
@@ -299,9 +329,9 @@ struct Piece {
     } else if constexpr (FMT == NATIVE) {
       out[0] = u4{raw[0], raw[1], raw[2], raw[3]};
     } else if constexpr (FMT == INT4) {
-      out[0] = widen8<INT4, Q>(raw[f], 0);
+      out[0] = widen8<INT4, Q, BY>(raw[f], 0);
     } else {
-      out[0] = widen8<FMT, Q>(raw[2 * f], raw[2 * f + 1]);
+      out[0] = widen8<FMT, Q, BY>(raw[2 * f], raw[2 * f + 1]);
     }
   }
 };
@@ -320,7 +350,8 @@ struct Piece {
 // Every part of the loop is in the code once: a small call is mostly the first pass of its instructions through the caches.
 template <int FMT, int Q, int W, int QT, int S, int WAVES, bool ONCE>
 __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionArgs a, FastDiv page) {
-  typedef Piece<FMT, Q, W> P;
+  constexpr int BY = SHRINK<FMT, Q, false>;
+  typedef Piece<FMT, Q, W, BY> P;
   constexpr int QP = Q == F32 ? 3 : 1, FR = W / 8, TQ = 16 * QT, WR = 16 * S, TR = WR * WAVES;
   constexpr int CS = 16 / S;                                  // chunks of a row in a stage
   constexpr int SP = CS * 16 / (4 * P::BYTES);                // steps of 4 W elements in a stage
@@ -536,7 +567,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
         const uint32_t q = i & ((1u << shift) - 1), e = i >> shift, f = e % FR, h = e / FR % 4, st = e / (4 * FR);
         if (q >= asked) continue;   // what is in LDS behind them is multiplied and not used
         u4 w[QP];
-        stage8<Q>(a, q0 + q, (p0 * SP + st) * (4 * W) + h * W + f * 8, w);
+        stage8<Q, BY>(a, q0 + q, (p0 * SP + st) * (4 * W) + h * W + f * 8, w);
 #pragma unroll
         for (int p = 0; p < QP; p++) staged[(((st * FR + f) * QP + p) * QT + q / 16) * 64 + h * 16 + q % 16] = w[p];
       }
@@ -567,7 +598,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
           for (int e = 0; e < 4 * QT; e++) {
             const uint32_t q = now.q0 + e / 4 * 16 + quarter * 4 + e % 4;
             if (q < now.q_end) {
-              float p = acc[k][e / 4][e % 4] * CODE_UNIT<FMT, Q>;
+              float p = acc[k][e / 4][e % 4] * UNIT<FMT, Q, BY>;
               if constexpr (FMT == NATIVE && Q == F32) {
                 // an infinity meets the other side's planes, some of them 0: the sum is taken again, element by element
                 if (p != p && (there >> k & 1)) {
@@ -613,7 +644,8 @@ __global__ __launch_bounds__(256, 2) void partition_many_kernel(PartitionArgs a,
   constexpr int PIECE_BYTES = FMT == NATIVE ? 8 * elem_size<Q> : 16, PU = PIECE_BYTES / 16;
   constexpr int NP = KC / PIECE, RT = (TR * NP + 255) / 256;                  // pieces of a row in a half, of a thread
   constexpr int QN = TQ * C8 / 256;                                          // eights of the queries in a half, of a thread
-  typedef Piece<FMT, Q, PIECE> P;
+  constexpr int BY = SHRINK<FMT, Q, true>;
+  typedef Piece<FMT, Q, PIECE, BY> P;
   __shared__ u4 q_lds[2][KC / 16 * QP * TQ * 2], r_lds[2][KC / 16 * RP * TR * 2];
   __shared__ float s_lds[2][TR];
   __shared__ RunShared run_shared;
@@ -834,8 +866,9 @@ __global__ __launch_bounds__(256, 2) void partition_many_kernel(PartitionArgs a,
     for (int r = R; r < R + 8; r++) {
       const uint32_t q = t.q0 + wave_q + x * 32 + 8 * (r / 4) + 4 * half_wave + r % 4;
       if (q >= t.q_end) continue;
-      float p = sums[x][y][r] * CODE_UNIT<FMT, Q>;
+      float p = sums[x][y][r];
       if (FMT != NATIVE && !FLUSH) p *= row_scale[y];
+      p *= UNIT<FMT, Q, BY>;
       if constexpr (FMT == NATIVE && Q == F32) {
         // an infinity meets the other side's planes, some of them 0: the sum is taken again, element by element
         if (p != p && (there >> y & 1)) {
