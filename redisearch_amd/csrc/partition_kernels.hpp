@@ -12,7 +12,7 @@ namespace {
 //
 // p[m][j] = sum_k q[m][k] c[j][k] s[j][k / block].  The codes are integers or e4m3 values that a 16-bit float holds exactly, so the
 // matrix cores multiply codes with queries, and a block's sum is multiplied by its scale in fp32: no operand is rounded.
-// fp32 operands go in as three bf16 each (8 + 8 + 8 bits of the significand, cut off exactly).
+// fp32 operands go in as three bf16 each, exactly.
 
 template <int Q>
 __device__ __forceinline__ f32x16 mfma(u4 a, u4 b, f32x16 c) {
@@ -44,25 +44,30 @@ __device__ __forceinline__ f32x4 mfma16(u4 a, u4 b, f32x4 c) {
   }
 }
 
-// x = hi + mid + lo, each a bf16 in the upper half of its dword.  An infinity or a NaN is hi alone.
-__device__ __forceinline__ void split3(uint32_t x, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
-  const bool special = (x & 0x7f800000u) == 0x7f800000u;
-  hi = (x & 0xffff0000u) | (special && (x & 0xffffu) ? 0x400000u : 0);   // a NaN whose payload sits in the bits cut off stays one
-  const float r = special ? 0.0f : __uint_as_float(x) - __uint_as_float(hi);
-  mid = __float_as_uint(r) & 0xffff0000u;
-  lo = __float_as_uint(r - __uint_as_float(mid));
-}
 __device__ __forceinline__ uint32_t upper2(uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
+__device__ __forceinline__ float low_bf16(uint32_t two) { return __uint_as_float(two << 16); }
+__device__ __forceinline__ float high_bf16(uint32_t two) { return __uint_as_float(two & 0xffff0000u); }
 
-// eight fp32 -> eight bf16 in each of three planes
+// what is left of x behind the nearest bf16 (`hi`, which is cut off instead where the nearest is an infinity and x is not)
+__device__ __forceinline__ float behind(float x, float &hi) {
+  const float a = __builtin_fabsf(x);
+  if (a >= 0x1.ffp127f) hi = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+  return a == __builtin_inff() ? 0.0f : x - hi;
+}
+
+// Eight fp32 -> eight bf16 in each of three planes, x = hi + mid + lo exactly: hi and mid are rounded to the nearest, so that mid is at
+// most 2^-8 of x's binade and lo 2^-17, of either sign.  (Cut off, as upper halves are, they are twice that and all of x's sign: what the
+// products leave out came to 2^-21 of a product, and to 2^-24 of every sum of products of one sign.)  An infinity is hi alone.
 __device__ __forceinline__ void planes8(const float (&v)[8], u4 (&p)[3]) {
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    uint32_t a[3], b[3];
-    split3(__float_as_uint(v[2 * i]), a[0], a[1], a[2]);
-    split3(__float_as_uint(v[2 * i + 1]), b[0], b[1], b[2]);
-#pragma unroll
-    for (int k = 0; k < 3; k++) p[k][i] = upper2(a[k], b[k]);
+    const uint32_t near = narrow2<BF16>(v[2 * i], v[2 * i + 1]);
+    float a = low_bf16(near), b = high_bf16(near);
+    const float ra = behind(v[2 * i], a), rb = behind(v[2 * i + 1], b);
+    const uint32_t mid = narrow2<BF16>(ra, rb);
+    p[0][i] = upper2(__float_as_uint(a), __float_as_uint(b));
+    p[1][i] = mid;
+    p[2][i] = upper2(__float_as_uint(ra - low_bf16(mid)), __float_as_uint(rb - high_bf16(mid)));
   }
 }
 
@@ -530,7 +535,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
               for (int c = P::PLANES - 1; c >= 0; c--)
 #pragma unroll
                 for (int t = 0; t < QT; t++)
-                  if (p + c < 3) part[k][t] = mfma16<Q>(q[t][p], b[c], part[k][t]);   // the planes left out are below 2^-24 of the product
+                  if (p + c < 3) part[k][t] = mfma16<Q>(q[t][p], b[c], part[k][t]);   // left out: no more than 2^-24 of the product
           }
         }
         // a step's sum, times the scale of the block that it is in (no branch for the block's end: the steps overlap)
@@ -600,8 +605,9 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
             if (q < now.q_end) {
               float p = acc[k][e / 4][e % 4] * UNIT<FMT, Q, BY>;
               if constexpr (FMT == NATIVE && Q == F32) {
-                // an infinity meets the other side's planes, some of them 0: the sum is taken again, element by element
-                if (p != p && (there >> k & 1)) {
+                // an infinity meets the other side's planes, some of them 0, and two hi that were rounded up may pass the type's end: the
+                // sum is taken again, element by element
+                if (!__builtin_isfinite(p) && (there >> k & 1)) {
                   bool is;
                   const uint64_t slot = slot_of(j, a.pages[(size_t)now.g * a.max_pages + page.div(j)], is);
                   p = plain_product(reinterpret_cast<const float *>(a.c.codes + slot * a.c.row_bytes), static_cast<const float *>(a.queries) + q * a.stride, a.c.dim);
@@ -824,7 +830,7 @@ __global__ __launch_bounds__(256, 2) void partition_many_kernel(PartitionArgs a,
       for (int p = QP - 1; p >= 0; p--)   // the smallest first
 #pragma unroll
         for (int c = RP - 1; c >= 0; c--)
-          if (p + c < 3) {   // the planes left out are below 2^-24 of the product
+          if (p + c < 3) {   // left out: no more than 2^-24 of the product
 #pragma unroll
             for (int x = 0; x < X; x++)
 #pragma unroll
@@ -870,8 +876,8 @@ __global__ __launch_bounds__(256, 2) void partition_many_kernel(PartitionArgs a,
       if (FMT != NATIVE && !FLUSH) p *= row_scale[y];
       p *= UNIT<FMT, Q, BY>;
       if constexpr (FMT == NATIVE && Q == F32) {
-        // an infinity meets the other side's planes, some of them 0: the sum is taken again, element by element
-        if (p != p && (there >> y & 1)) {
+        // as above: the sum is taken again, element by element
+        if (!__builtin_isfinite(p) && (there >> y & 1)) {
           bool is;
           const uint64_t slot = slot_of(j, page_of(t, j), is);
           p = plain_product(reinterpret_cast<const float *>(a.c.codes + slot * a.c.row_bytes), static_cast<const float *>(a.queries) + q * a.stride, a.c.dim);

@@ -44,6 +44,37 @@ def test_scores_of_queries_whose_sums_of_codes_leave_fp32(vtype, fmt, block, ask
     check(cache, q.to(TYPES[vtype]).cuda(), rows, wide, R.DISTANCE if block else R.PRODUCT)
 
 
+# A number with 24 bits is three bf16.  Whichever way it is cut into them, what the products of the planes leave out is of the order of
+# 2^-24 at best; a product of single elements shows it, where a sum of hundreds hides it behind its own rounding.
+EDGES = [0x3f80ffff, 0x3fffffff, 0x3f7fffff, 0x3f808000, 0x3f818000, 0x3f80807f, 0x3f808080, 0x3f80ff80, 0x3fb504f3, 0x3f800001]
+
+
+@SIZES
+@pytest.mark.parametrize("dim", [40, 200, 768])
+def test_products_of_single_fp32_elements(asked, wide, dim):
+    """Rows with one element, at every place of a row: each score is one product."""
+    gen = torch.Generator().manual_seed(dim + asked)
+    rows = 800
+    edges = torch.tensor(EDGES, dtype=torch.int32).view(torch.float32)
+    x = 1 + torch.rand((rows,), generator=gen)
+    x[::3] = edges[torch.arange(rows)[::3] % len(EDGES)]
+    x[1::4] *= -2.0 ** torch.randint(-30, 30, (rows,), generator=gen)[1::4]
+    q = 1 + torch.rand((asked, dim), generator=gen)
+    q.view(-1)[::2] = edges[torch.arange(asked * dim)[::2] // 2 % len(EDGES)]
+    q[1::2] *= -1
+    where = torch.arange(rows) % dim
+    data = torch.zeros((rows, dim))
+    data[torch.arange(rows), where] = x
+    cache = Cache(P.F32, dim, R.NATIVE, 0, rows, zero=True)
+    cache.write(data.cuda(), torch.arange(rows, device="cuda"))
+    got = one_partition(cache, q.cuda(), rows, wide)
+    want = as64(q)[:, where.numpy()] * as64(x)[None]
+    # x = hi + mid + lo, each the nearest bf16: |mid| <= 2^-8, |lo| <= 2^-17 of x's binade.  Left out are mid lo + lo mid + lo lo, no more
+    # than 2^-24 + 2^-34 of |x y|.  The six products are exact and added smallest first, each sum rounded or cut off: five sums below
+    # 2^-6 |x y| by 2^-23 of themselves, then the whole by 2^-23.  Zeros change nothing.
+    assert (np.abs(got - want) <= np.abs(want) * (2.0 ** -23 + 5 * 2.0 ** -29 + 2.0 ** -24 + 2.0 ** -33)).all(), np.max(np.abs(got / want - 1)) * 2.0 ** 24
+
+
 def one_partition(cache, q, rows, wide, page_rows=16):
     """Scores as float64, the call made in a table of the partition's rows or one that allows 70 000."""
     m, ld = q.shape[0], 70001 if wide else rows
