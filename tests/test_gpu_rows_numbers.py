@@ -113,6 +113,33 @@ def test_products_of_the_largest_fp32_numbers(fmt, asked, wide):
 
 
 @SIZES
+@pytest.mark.parametrize("vtype,fmt,block", [(P.F32, R.NATIVE, 0), (P.BF16, R.NATIVE, 0), (P.F16, R.NATIVE, 0), (P.F32, R.INT8, 32), (P.BF16, R.INT8, 0),
+                                             (P.F16, R.E4M3, 0), (P.BF16, R.E4M3, 128), (P.F16, R.INT4, 0), (P.F32, R.INT4, 0), (P.BF16, R.INT4, 64)])
+def test_scores_with_infinities_and_nan_in_every_kernel(vtype, fmt, block, asked, wide):
+    """A NaN, an infinity or a block kept as NaN reach the scores of their own row, a query's those of its own line, and no others: at the
+    first and the last row, the first and the last element, on both sides of the tiles' borders."""
+    gen = torch.Generator().manual_seed(fmt)
+    dim, rows = 135, 530
+    data = values(gen, rows, dim, vtype)
+    inf, nan = float("inf"), float("nan")
+    for row, at, value in [(0, 0, nan), (63, dim - 1, inf), (64, 31, -inf), (127, 32, inf), (128, dim - 1, nan), (255, 0, inf), (256, dim - 1, -inf),
+                           (257, 64, nan), (511, 127, inf), (512, 128, nan), (rows - 1, dim - 1, inf)]:
+        data[row, at] = value
+    data[300, 5] = inf
+    data[300, 90] = -inf
+    q = values(gen, asked, dim, vtype)
+    q[0, 0] = inf
+    q[1, dim - 1] = -inf
+    q[2, 64] = nan
+    q[asked - 1, dim - 1] = nan
+    if asked > 100:
+        q[63, 3], q[64, 133], q[127, 134], q[128, 0] = inf, nan, -inf, inf
+    cache = Cache(vtype, dim, fmt, block, rows, zero=True)
+    cache.write(data, torch.arange(rows, device="cuda"))
+    check(cache, q, rows, wide)
+
+
+@SIZES
 @pytest.mark.parametrize("vtype", [P.F32, P.BF16], ids=ids)
 @pytest.mark.parametrize("fmt,block", [(R.NATIVE, 0), (R.INT8, 0), (R.E4M3, 32), (R.INT4, 128)])
 def test_scores_of_tiny_queries(vtype, fmt, block, asked, wide):
