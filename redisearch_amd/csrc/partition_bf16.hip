@@ -2,8 +2,5 @@
 #include "partition_kernels.hpp"
 
 namespace rsgpu {
-void launch_partition_scores_bf16(const PartitionArgs &a, hipStream_t s) {
-  scores_from<BF16>(a, s);
-  HIP_CHECK(hipGetLastError());
-}
+void launch_partition_scores_bf16(const PartitionArgs &a, hipStream_t s) { scores_from<BF16>(a, s); }
 }  // namespace rsgpu

@@ -1006,7 +1006,7 @@ void scores_as(const PartitionArgs &a, hipStream_t s) {
     const auto many = [&](auto kernel, uint32_t rows) {
       dim3 g = grid(128, rows, resident(reinterpret_cast<const void *>(kernel), 256));
       g.x = (g.x + DIES - 1) / DIES * DIES;
-      hipLaunchKernelGGL(kernel, g, dim3(256), 0, s, a, page);
+      launch(kernel, g, 256, s, a, page);
     };
     if (a.c.nb <= 1) {
       if constexpr (Q != F32) {
@@ -1021,23 +1021,23 @@ void scores_as(const PartitionArgs &a, hipStream_t s) {
   }
   const auto few = [&](auto w) {
     constexpr int W = decltype(w)::value, WAVES = Q == F32 ? 16 : 8;
-    const auto launch = [&](auto kernel, uint32_t tq, uint32_t tr, uint32_t waves) {
-      hipLaunchKernelGGL(kernel, grid(tq, tr, resident(reinterpret_cast<const void *>(kernel), 64 * waves)), dim3(64 * waves), 0, s, a, page);
+    const auto go = [&](auto kernel, uint32_t tq, uint32_t tr, uint32_t waves) {
+      launch(kernel, grid(tq, tr, resident(reinterpret_cast<const void *>(kernel), 64 * waves)), 64 * waves, s, a, page);
     };
     // at eight queries a partition hardly one has more than the sixteen of a tile, so that its rows are read once
     const auto sized = [&](auto waves, auto once) {
       constexpr int V = decltype(waves)::value;
       constexpr bool ONCE = decltype(once)::value;
-      if (cs == 16) launch(partition_few_kernel<FMT, Q, W, 1, 1, V, ONCE>, 16, 16 * V, V);
-      else if (cs == 8) launch(partition_few_kernel<FMT, Q, W, 1, 2, V, ONCE>, 16, 32 * V, V);
-      else if constexpr (!widest) launch(partition_few_kernel<FMT, Q, W, 1, 4, V, ONCE>, 16, 64 * V, V);
+      if (cs == 16) go(partition_few_kernel<FMT, Q, W, 1, 1, V, ONCE>, 16, 16 * V, V);
+      else if (cs == 8) go(partition_few_kernel<FMT, Q, W, 1, 2, V, ONCE>, 16, 32 * V, V);
+      else if constexpr (!widest) go(partition_few_kernel<FMT, Q, W, 1, 4, V, ONCE>, 16, 64 * V, V);
     };
     if (tiles(16, 256 / cs * 4) <= (cs == 4 ? LITTLE_NARROW : LITTLE)) return sized(std::integral_constant<int, 4>(), std::false_type());
     if (each <= 8) return sized(std::integral_constant<int, WAVES>(), std::true_type());
     if constexpr (Q != F32) {   // (three planes of 32 queries leave no room for whole rows)
       if (each >= TWO_TILES && cs != 4) {
-        if (cs == 16) launch(partition_few_kernel<FMT, Q, W, 2, 1, 16, false>, 32, 256, 16);
-        else launch(partition_few_kernel<FMT, Q, W, 2, 2, 16, false>, 32, 512, 16);
+        if (cs == 16) go(partition_few_kernel<FMT, Q, W, 2, 1, 16, false>, 32, 256, 16);
+        else go(partition_few_kernel<FMT, Q, W, 2, 2, 16, false>, 32, 512, 16);
         return;
       }
     }

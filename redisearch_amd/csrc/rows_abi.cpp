@@ -204,6 +204,7 @@ int RSGPU_FlatIndex_CacheRows(VecSimIndex *index, size_t row_begin, size_t n, co
     need(!n || (slots && aligned(slots, 8)), "slots are 8-byte aligned");
     OnDevice on(cache->device, c.codes);
     need(on.now == index->flat->device, "the cache is on another device than the index");
+    (void)hipGetLastError();   // the index asks for the last error of its own launches, not for what the caller's thread has left
     HIP_CHECK(hipStreamSynchronize((hipStream_t)wait_stream));
     index->flat->cache_rows(row_begin, n, c, slots);
     return 0;
@@ -220,6 +221,7 @@ int RSGPU_FlatIndex_AddCachedRows(VecSimIndex *index, const RSGPU_RowCache *cach
     need(!n || (slots && aligned(slots, 8)), "slots are 8-byte aligned");
     OnDevice on(cache->device, c.codes);
     need(on.now == index->flat->device, "the cache is on another device than the index");
+    (void)hipGetLastError();   // the index asks for the last error of its own launches, not for what the caller's thread has left
     HIP_CHECK(hipStreamSynchronize((hipStream_t)wait_stream));
     return index->flat->add_cached_rows(c, slots, n, first_label);
   });

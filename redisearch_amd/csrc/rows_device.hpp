@@ -2,6 +2,8 @@
 #pragma once
 #include <hip/hip_runtime.h>
 
+#include <tuple>
+
 #include "rows.hpp"
 
 namespace rsgpu {
@@ -156,6 +158,17 @@ __device__ __forceinline__ uint32_t narrow2(float a, float b) {
     __builtin_memcpy(&w, &h, 4);
   }
   return w;
+}
+
+// A launch whose own error is what it returns: hipGetLastError() behind it would also hand over one that an earlier call of the caller's
+// thread has left (an event asked before it was ready is one), for work that is already under way.
+template <typename... P, typename... A>
+void launch(void (*kernel)(P...), dim3 grid, uint32_t threads, hipStream_t s, const A &...args) {
+  std::tuple<P...> held(args...);
+  std::apply([&](P &...x) {
+    void *at[] = {static_cast<void *>(&x)...};
+    HIP_CHECK(hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, dim3(threads), at, 0, s));
+  }, held);
 }
 
 // a count or an offset from the device, within its range

@@ -481,10 +481,10 @@ template <int T, int FMT>
 void write_as(const RowCacheArgs &c, const void *rows, uint32_t stride, const int64_t *slots, uint32_t n, hipStream_t s) {
   if (c.nb == 1 && c.dim > 512) {
     const dim3 grid(workgroups(((uint64_t)n + 3) / 4));
-    if (c.dim <= 1024) hipLaunchKernelGGL((row_write_whole_kernel<T, FMT, 2>), grid, dim3(256), 0, s, c, rows, stride, slots, n);
-    else if constexpr (T == F32) hipLaunchKernelGGL((row_write_whole_kernel<T, FMT, 0>), grid, dim3(256), 0, s, c, rows, stride, slots, n);
-    else if (c.dim <= 2048) hipLaunchKernelGGL((row_write_whole_kernel<T, FMT, 4>), grid, dim3(256), 0, s, c, rows, stride, slots, n);
-    else hipLaunchKernelGGL((row_write_whole_kernel<T, FMT, 0>), grid, dim3(256), 0, s, c, rows, stride, slots, n);
+    if (c.dim <= 1024) launch(row_write_whole_kernel<T, FMT, 2>, grid, 256, s, c, rows, stride, slots, n);
+    else if constexpr (T == F32) launch(row_write_whole_kernel<T, FMT, 0>, grid, 256, s, c, rows, stride, slots, n);
+    else if (c.dim <= 2048) launch(row_write_whole_kernel<T, FMT, 4>, grid, 256, s, c, rows, stride, slots, n);
+    else launch(row_write_whole_kernel<T, FMT, 0>, grid, 256, s, c, rows, stride, slots, n);
     return;
   }
   // the lanes of a block, or of a row that is one
@@ -494,11 +494,11 @@ void write_as(const RowCacheArgs &c, const void *rows, uint32_t stride, const in
   const dim3 grid(workgroups(((uint64_t)n + per - 1) / per));
   const FastDiv d(chunks);
   switch (lanes) {
-    case 4: hipLaunchKernelGGL((row_write_kernel<T, FMT, 4>), grid, dim3(256), 0, s, c, rows, stride, slots, n, per, d); break;
-    case 8: hipLaunchKernelGGL((row_write_kernel<T, FMT, 8>), grid, dim3(256), 0, s, c, rows, stride, slots, n, per, d); break;
-    case 16: hipLaunchKernelGGL((row_write_kernel<T, FMT, 16>), grid, dim3(256), 0, s, c, rows, stride, slots, n, per, d); break;
-    case 32: hipLaunchKernelGGL((row_write_kernel<T, FMT, 32>), grid, dim3(256), 0, s, c, rows, stride, slots, n, per, d); break;
-    default: hipLaunchKernelGGL((row_write_kernel<T, FMT, 64>), grid, dim3(256), 0, s, c, rows, stride, slots, n, per, d); break;
+    case 4: launch(row_write_kernel<T, FMT, 4>, grid, 256, s, c, rows, stride, slots, n, per, d); break;
+    case 8: launch(row_write_kernel<T, FMT, 8>, grid, 256, s, c, rows, stride, slots, n, per, d); break;
+    case 16: launch(row_write_kernel<T, FMT, 16>, grid, 256, s, c, rows, stride, slots, n, per, d); break;
+    case 32: launch(row_write_kernel<T, FMT, 32>, grid, 256, s, c, rows, stride, slots, n, per, d); break;
+    default: launch(row_write_kernel<T, FMT, 64>, grid, 256, s, c, rows, stride, slots, n, per, d); break;
   }
 }
 
@@ -510,7 +510,7 @@ void write_from(const RowCacheArgs &c, const void *rows, uint32_t stride, const 
     case INT4: return write_as<T, INT4>(c, rows, stride, slots, n, s);
     default: {
       const uint32_t chunks = c.row_bytes / 16, per = rows_a_workgroup(n, chunks, 256 * WRITE_UNDER_WAY);
-      hipLaunchKernelGGL((row_copy_in_kernel<T>), dim3(workgroups(((uint64_t)n + per - 1) / per)), dim3(256), 0, s, c, rows, stride, slots, n, per, FastDiv(chunks));
+      launch(row_copy_in_kernel<T>, dim3(workgroups(((uint64_t)n + per - 1) / per)), 256, s, c, rows, stride, slots, n, per, FastDiv(chunks));
     }
   }
 }
@@ -522,10 +522,10 @@ void read_to(const RowCacheArgs &c, const int64_t *slots, uint32_t n, void *out,
   const dim3 grid(workgroups(((uint64_t)n + per - 1) / per));
   const FastDiv d(chunks), b(c.block);
   switch (c.format) {
-    case INT8: hipLaunchKernelGGL((row_read_kernel<T, INT8>), grid, dim3(256), 0, s, c, slots, n, out, stride, per, d, b); break;
-    case E4M3: hipLaunchKernelGGL((row_read_kernel<T, E4M3>), grid, dim3(256), 0, s, c, slots, n, out, stride, per, d, b); break;
-    case INT4: hipLaunchKernelGGL((row_read_kernel<T, INT4>), grid, dim3(256), 0, s, c, slots, n, out, stride, per, d, b); break;
-    default: hipLaunchKernelGGL((row_read_kernel<T, NATIVE>), grid, dim3(256), 0, s, c, slots, n, out, stride, per, d, b); break;
+    case INT8: launch(row_read_kernel<T, INT8>, grid, 256, s, c, slots, n, out, stride, per, d, b); break;
+    case E4M3: launch(row_read_kernel<T, E4M3>, grid, 256, s, c, slots, n, out, stride, per, d, b); break;
+    case INT4: launch(row_read_kernel<T, INT4>, grid, 256, s, c, slots, n, out, stride, per, d, b); break;
+    default: launch(row_read_kernel<T, NATIVE>, grid, 256, s, c, slots, n, out, stride, per, d, b); break;
   }
 }
 
@@ -536,21 +536,18 @@ void launch_row_write(const RowCacheArgs &c, const void *rows, uint32_t stride, 
   if (c.type == F32) write_from<F32>(c, rows, stride, slots, n, s);
   else if (c.type == F16) write_from<F16>(c, rows, stride, slots, n, s);
   else write_from<BF16>(c, rows, stride, slots, n, s);
-  HIP_CHECK(hipGetLastError());
 }
 
 void launch_row_read(const RowCacheArgs &c, const int64_t *slots, uint32_t n, void *out, uint32_t stride, hipStream_t s) {
   if (c.type == F32) read_to<F32>(c, slots, n, out, stride, s);
   else if (c.type == F16) read_to<F16>(c, slots, n, out, stride, s);
   else read_to<BF16>(c, slots, n, out, stride, s);
-  HIP_CHECK(hipGetLastError());
 }
 
 void launch_adjust_scores(const AdjustArgs &a, hipStream_t s) {
   const uint32_t tiles = (a.n_columns + COLUMNS - 1) / COLUMNS;
   const uint64_t work = (uint64_t)tiles * a.n_queries;
-  hipLaunchKernelGGL(adjust_scores_kernel, dim3(workgroups(work)), dim3(256), 0, s, a, tiles, work);
-  HIP_CHECK(hipGetLastError());
+  launch(adjust_scores_kernel, dim3(workgroups(work)), 256, s, a, tiles, work);
 }
 
 }  // namespace rsgpu
