@@ -689,6 +689,7 @@ int FlatIndex::remove(size_t label) {
 // a single-value index holds one vector per label: a bulk load may not collide with a stored label
 // (AddVector's overwrite semantics would need a row-by-row path; the caller uses AddVector for that)
 void FlatIndex::check_bulk_labels(size_t n, size_t first_label) const {
+  if (n && n - 1 > SIZE_MAX - first_label) throw std::runtime_error("bulk load: labels end at 2^64 - 1");
   if (multi) return;
   if (labels_.any_in_range(first_label, n)) throw std::runtime_error("bulk load: label range overlaps stored labels");
 }

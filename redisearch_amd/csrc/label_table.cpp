@@ -109,14 +109,14 @@ size_t LabelTable::label_count() const {
 bool LabelTable::any_in_range(uint64_t first, size_t n) const {
   if (!n) return false;
   switch (mode_) {
-    case IDENTITY: {
-      const uint64_t lo = identity_base_, hi = identity_base_ + row_label_->size();
-      return !row_label_->empty() && first < hi && first + n > lo;
-    }
+    // (distances, not ends: a range or the table may reach the last label there is)
+    case IDENTITY: return !row_label_->empty() && (first >= identity_base_ ? first - identity_base_ < row_label_->size() : identity_base_ - first < n);
     case DIRECT: {
-      const uint64_t lo = std::max(first, base_), hi = std::min(first + n, base_ + (uint64_t)enc_cap_);
-      for (uint64_t l = lo; l < hi; l++)
-        if (head_at((size_t)(l - base_)) != kNoRow) return true;
+      const uint64_t skip = first < base_ ? base_ - first : 0, off = first < base_ ? 0 : first - base_;
+      if (skip >= n || off >= enc_cap_) return false;
+      const uint64_t many = std::min<uint64_t>(n - skip, enc_cap_ - off);
+      for (uint64_t i = 0; i < many; i++)
+        if (head_at((size_t)(off + i)) != kNoRow) return true;
       return false;
     }
     case HASH:
@@ -316,16 +316,16 @@ void LabelTable::grow_span(size_t need, hipStream_t s) {
 bool LabelTable::slot_for(uint64_t label, size_t n, hipStream_t s, size_t *off) {
   if (label < base_) {
     const uint64_t nb = label < kSmallBase ? 0 : label;
-    const uint64_t need = (base_ - nb) + enc_cap_;
-    if (need > span_limit() || label + n - nb > span_limit()) {
+    const uint64_t need = (base_ - nb) + enc_cap_, from = label - nb;
+    if (need > span_limit() || from > span_limit() || n > span_limit() - from) {
       to_hash(s);
       return false;
     }
     rebuild_direct(nb, (size_t)std::max<uint64_t>(need, label + n - nb), s);
   }
   const uint64_t o = label - base_;
-  if (o + n > enc_cap_) {
-    if (o + n > span_limit()) {
+  if (o > enc_cap_ || n > enc_cap_ - o) {
+    if (o > span_limit() || n > span_limit() - o) {   // (o + n may pass 2^64)
       to_hash(s);
       return false;
     }

@@ -65,3 +65,35 @@ def test_an_error_left_by_an_earlier_call_is_not_this_ones():
         lib.hipGetLastError()
     assert index.index_size() == n and (index.read_rows(0, n) == back.cpu().numpy()).all()
     assert np.abs(P.dequantise(*cache.plain(), dim, R.INT8, 32) - stored).max() <= 1e-6 * np.abs(stored).max()
+
+
+@pytest.mark.parametrize("mode", [0, 1, 2], ids=["identity", "direct", "hash"])
+def test_labels_that_would_pass_the_last_one(mode):
+    """Labels are 64 bits: a range that would go on at 0 is refused, whatever form the index keeps its labels in; one that ends at the
+    last label is not."""
+    dim, n = 32, 8
+    index = V.VecSimIndex(P.F32, dim, V.VecSimMetric_L2)
+    x = np.random.default_rng(mode).standard_normal((12, dim)).astype(np.float32)
+    index.add_bulk(x[:4], 1)
+    if mode == 1:
+        index.delete_vector(2)
+    if mode == 2:
+        index.add_vector(x[4], 10 ** 15)
+    assert index.label_table() == mode
+    before = index.index_size()
+    cache = Cache(P.F32, dim, R.NATIVE, 0, n, zero=True)
+    slots = torch.arange(n, device="cuda")
+    cache.write(torch.from_numpy(x[4:]).cuda(), slots)
+    for first, many in ((2 ** 64 - 2, 4), (2 ** 64 - 1, 2), (2 ** 64 - 7, 8)):
+        with pytest.raises(RuntimeError, match="labels end at"):
+            cache.c.add_to(index, slots.data_ptr(), many, first, stream())
+    assert index.index_size() == before
+    assert cache.c.add_to(index, slots[4:].data_ptr(), 2, 2 ** 64 - 3, stream()) == 2
+    assert cache.c.add_to(index, slots[6:].data_ptr(), 1, 2 ** 64 - 1, stream()) == 1
+    for first, many in ((2 ** 64 - 4, 2), (2 ** 64 - 2, 2), (2 ** 64 - 1, 1)):
+        with pytest.raises(RuntimeError, match="label range overlaps"):
+            cache.c.add_to(index, slots.data_ptr(), many, first, stream())
+    assert index.index_size() == before + 3
+    for row, label in ((8, 2 ** 64 - 3), (9, 2 ** 64 - 2), (10, 2 ** 64 - 1)):
+        found, distances = index.topk_query(x[row], 1).results()
+        assert found.astype(np.uint64).tolist() == [label] and distances[0] <= 1e-6
