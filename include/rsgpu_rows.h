@@ -109,7 +109,8 @@ int RSGPU_AdjustScores(const RSGPU_ScoreRules *rules, const float *scores_in, fl
 int RSGPU_FlatIndex_CacheRows(VecSimIndex *index, size_t row_begin, size_t n, const RSGPU_RowCache *cache, const int64_t *slots,
                               void *wait_stream);
 /* n rows of the cache are appended to the index, labelled first_label .. first_label + n - 1, at most 2^64 - 1 (cosine rows are
- * normalised); a slot out of range appends a row of zeros.  Returns rows added or -1. */
+ * normalised); a slot out of range appends a row of zeros, which a cosine index keeps as every row of zeros, as NaN: behind every
+ * other row in its answers.  Returns rows added or -1. */
 int RSGPU_FlatIndex_AddCachedRows(VecSimIndex *index, const RSGPU_RowCache *cache, const int64_t *slots, size_t n, size_t first_label,
                                   void *wait_stream);
 

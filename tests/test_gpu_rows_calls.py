@@ -97,3 +97,30 @@ def test_labels_that_would_pass_the_last_one(mode):
     for row, label in ((8, 2 ** 64 - 3), (9, 2 ** 64 - 2), (10, 2 ** 64 - 1)):
         found, distances = index.topk_query(x[row], 1).results()
         assert found.astype(np.uint64).tolist() == [label] and distances[0] <= 1e-6
+
+
+@pytest.mark.parametrize("vtype", [P.F32, P.F16, P.BF16], ids={P.F32: "f32", P.F16: "f16", P.BF16: "bf16"}.get)
+@pytest.mark.parametrize("metric", [V.VecSimMetric_Cosine, V.VecSimMetric_IP], ids={V.VecSimMetric_Cosine: "cosine", V.VecSimMetric_IP: "ip"}.get)
+def test_slots_out_of_range_come_into_an_index_as_rows_of_zeros_do(vtype, metric):
+    """A row of zeros has no direction: a cosine index keeps it as NaN, by whichever way it came, and finds it behind every other."""
+    dim, n = 48, 9
+    rng = np.random.default_rng(4)
+    x = rng.standard_normal((n, dim)).astype(np.float32)
+    cache = Cache(vtype, dim, R.NATIVE, 0, n, zero=True)
+    cache.write(torch.from_numpy(x).to({P.F32: torch.float32, P.F16: torch.float16, P.BF16: torch.bfloat16}[vtype]).cuda(), torch.arange(n, device="cuda"))
+    cached, loaded = (V.VecSimIndex(vtype, dim, metric) for _ in range(2))
+    slots = torch.tensor([0, -1, 2, 3, n, 5, 6, 2 ** 62, 8], device="cuda")
+    assert cache.c.add_to(cached, slots.data_ptr(), n, 1, stream()) == n
+    x[[1, 4, 7]] = 0
+    as_rows = torch.from_numpy(x).to({P.F32: torch.float32, P.F16: torch.float16, P.BF16: torch.bfloat16}[vtype]).cuda()
+    torch.cuda.synchronize()
+    loaded.add_device_rows(as_rows.data_ptr(), n, 1)
+    a, b = cached.read_rows(0, n), loaded.read_rows(0, n)
+    assert a.tobytes() == b.tobytes()
+    zeros = torch.from_numpy(a[[1, 4, 7]].astype(np.int32) if vtype == P.BF16 else a[[1, 4, 7]].astype(np.float32))
+    assert ((zeros & 0x7fff) > 0x7f80).all() if metric == V.VecSimMetric_Cosine and vtype == P.BF16 else zeros.isnan().all() if metric == V.VecSimMetric_Cosine else not zeros.any()
+    q = x[2] + x[3]
+    near = [index.topk_query(q, n).results()[0].tolist() for index in (cached, loaded)]
+    assert near[0] == near[1]
+    if metric == V.VecSimMetric_Cosine:
+        assert not {2, 5, 8} & set(near[0][:6])
