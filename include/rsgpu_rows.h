@@ -2,10 +2,10 @@
  * rsgpu_rows.h -- rows kept in 8 or 4 bits, the products of a batch's queries with their own partitions' rows, and the rules
  * applied to a batch's scores.  Extensions of the MI355X engine (nothing here exists in VecSim), plain C, pointers and sizes.
  *
- * All arrays below are DEVICE memory and belong to the caller; every call only launches kernels on `stream` (a hipStream_t;
- * NULL: the device's default stream) and returns: no call allocates, copies or waits, so all of them may be captured into a
- * hipGraph.  Two calls that write the same memory are ordered by the caller (one stream, or events).  0 on success, -1 with
- * RSGPU_LastError() otherwise; a refused call has launched nothing.  An index found on the device (a slot, a page, an offset, a
+ * All arrays below are DEVICE memory and belong to the caller; every call but the two RSGPU_FlatIndex_ ones at the end only launches
+ * kernels on `stream` (a hipStream_t; NULL: the device's default stream) and returns: none of them allocates, copies or waits, so they
+ * may be captured into a hipGraph.  Two calls that write the same memory are ordered by the caller (one stream, or events).  0 on
+ * success, -1 with RSGPU_LastError() otherwise; a refused call has launched nothing.  An index found on the device (a slot, a page, an offset, a
  * list's entry) that is out of its range never leads to an access out of range: what it means is said at each call.
  */
 #ifndef RSGPU_ROWS_H
@@ -63,7 +63,8 @@ int RSGPU_RowCache_Read(const RSGPU_RowCache *cache, const int64_t *slots, size_
  *   p = sum over the elements of query * row, accumulated in fp32; of rows kept in codes no sum on the way leaves fp32's range where p
  *   does not.  Bits of an element below 2^-107 and of p below 2^-119 are not kept.
  * A page that is negative or not in the cache: its rows score -inf (PRODUCT) / +inf (DISTANCE), behind every other.  All other
- * cells of `scores` are left as they were.  A row count counts as no more than max_pages * page_rows and ld; a range of queries
+ * cells of `scores` are left as they were.  Right for any groups, fast for even ones: the host chooses the kernel by the queries of a
+ * listed partition on average and by max_pages and ld, so list the partitions that are asked.  A row count counts as no more than max_pages * page_rows and ld; a range of queries
  * that falls or leaves [0, n_queries] is cut to it. */
 typedef enum { RSGPU_SCORES_PRODUCT = 0, RSGPU_SCORES_DISTANCE = 1 } RSGPU_ScoreForm;
 
@@ -77,7 +78,7 @@ int RSGPU_RowCache_PartitionScores(const RSGPU_RowCache *cache, const void *quer
  *           p = p > 0 ? p / repetition[m] : p * repetition[m], then p -= n * frequency[m] + presence[m]
  *   boost   the column is in the query's list bias_ids[..]: p += bias_values[..] (of an id that comes again, the last value)
  *   filter  bit (column % 32) of word column / 32 of the query's mask row is 0: -inf (+inf for a DISTANCE)
- * A cell that no rule touches keeps its bits.  Entries of a list out of [0, n_columns) are passed over; a list's range is cut to
+ * A cell that no rule touches keeps its bits.  A query's lists are read once for every 4096 columns.  Entries of a list out of [0, n_columns) are passed over; a list's range is cut to
  * [0, n_seen] / [0, n_bias]. */
 typedef struct RSGPU_ScoreRules {
   int device;                   /* HIP device of the arrays; -1: the one that holds the scores */
@@ -104,8 +105,9 @@ int RSGPU_AdjustScores(const RSGPU_ScoreRules *rules, const float *scores_in, fl
 
 /* ---- a FLAT index and a cache ------------------------------------------------------------------
  * The cache has the index's device, dim and type (FLOAT32, FLOAT16, BFLOAT16).  Both calls return when their work is done;
- * `wait_stream` (hipStream_t or NULL) is synchronised first. */
-/* stored rows [row_begin, row_begin + n) as they are in HBM (cosine rows: normalised) into slots[0 .. n-1].  0 or -1. */
+ * `wait_stream` (hipStream_t or NULL) is synchronised first; neither may be captured.  A sharded handle is refused: use its shards. */
+/* stored rows [row_begin, row_begin + n) as they are in HBM (cosine rows: normalised) into slots[0 .. n-1], in the order they are
+ * stored in: that of their insertion, except that a delete moves the last row into its place.  The cache keeps no labels.  0 or -1. */
 int RSGPU_FlatIndex_CacheRows(VecSimIndex *index, size_t row_begin, size_t n, const RSGPU_RowCache *cache, const int64_t *slots,
                               void *wait_stream);
 /* n rows of the cache are appended to the index, labelled first_label .. first_label + n - 1, at most 2^64 - 1 (cosine rows are

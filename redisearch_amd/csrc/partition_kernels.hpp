@@ -637,11 +637,10 @@ __global__ __launch_bounds__(64 * WAVES, 4) void partition_few_kernel(PartitionA
 // memory.  In LDS an operand's 32 rows change places with the number of its eight elements, so that neither side meets a bank twice.  A
 // block's products are summed by themselves and multiplied by the row's scale at every FLUSH elements (0: rows that have one scale or
 // none, at the end).
-// 16 partitions x 512 queries x 6144 bf16 rows of 768: 92 us, 0.84 PFLOP/s, of which the products are three quarters (1.2 - 1.3
-// PFLOP/s, what a large matrix product of the library reaches) and the scores' way to memory, 201 MB, the rest: stores and loads are
-// counted in one order, so the next tile's rows are waited for behind this one's scores (rows of 64 elements, almost nothing but
-// scores, take 32 us where 4096 rows of 768 take 66).  Workgroups begun at different times, four columns a lane's store, a tile's scores
-// kept in registers for the next tile's products to hide: no faster.
+// 16 partitions x 512 queries x 4096 bf16 rows of 768: 75 us, 0.69 PFLOP/s.  Rows of 64 elements, almost nothing but the scores' way
+// to memory (134 MB), take 35; the next 704 elements 40 (1.17 PFLOP/s), 768 more 48 (1.08; a large matrix product of the library 1.27).
+// Stores and loads are counted in one order, so the next tile's rows are waited for behind this one's scores.  Workgroups begun at
+// different times, four columns a lane's store, a tile's scores kept in registers for the next tile's products to hide: no faster.
 template <int FMT, int Q, int FLUSH, int TR>
 __global__ __launch_bounds__(256, 2) void partition_many_kernel(PartitionArgs a, FastDiv page) {
   constexpr int TQ = 128, X = TR / 64, Y = 2, KC = FMT == NATIVE && Q == F32 ? 16 : 32, QP = Q == F32 ? 3 : 1, RP = FMT == NATIVE && Q == F32 ? 3 : 1;
@@ -962,7 +961,10 @@ uint32_t resident(const void *kernel, uint32_t threads) {
   return (uint32_t)(units > 0 && each > 0 ? units * each : 256);
 }
 
-// Which kernel, by the queries of a partition on average (64 partitions x 5461 rows of 768, us; 20 / 40 / 60 queries):
+// Which kernel, by the queries of a partition on average: offsets and counts are on the device, and the host does not wait for them.
+// Where the queries crowd on few of the partitions that are listed, tiles for fewer queries read those rows again for every 16 or 32
+// (2000 queries for one of 400 partitions, 20 000 INT8 rows of 768: 358 us; that one listed alone: 93).
+// 64 partitions x 5461 rows of 768, us; 20 / 40 / 60 queries:
 //   int8 with fp16 queries    16 a tile 92 / 134 / -, 32 a tile 60 / 97 / -, the tiles of 128 107 / 115 / 126
 //   bf16 as it is             160 / 340, 120 / 166, 134 / 149 / 168
 //   int8 with fp32 queries    95 / 146, (no 32 a tile), 229 / 232 / 237
@@ -972,12 +974,13 @@ constexpr uint32_t TWO_TILES = 13, MANY = 48, MANY_LATE = 80;   // late: fp32 qu
 // Tiles of 256 rows, for half the reads of the queries, where the sums of a tile are all that the registers hold (16-bit queries, rows of
 // one scale or none) and there are as many tiles as the device holds at once.  16 partitions x 4096 rows of 768, 128 / 256 rows, us:
 //   INT8, one scale, fp16 queries: 90 queries a partition (432 tiles at most) 21.8 / 25.2, 128 (512) 25.7 / 25.8, 512 (1280) 74 / 71
-//   INT4, one scale, bf16 queries, 512: 81 / 66; bf16 rows as they are 68 / 66
+//   INT4, one scale, bf16 queries, 512: 81 / 66 (without SHRUNK: 1 - 2 % to either); bf16 rows as they are 68 / 66
 // (Scaled at every 64 elements, as rows of more scales are, the 512 take 87 and 93.)
 constexpr uint64_t MANY_TALL = 512;
 
-// Workgroups of four waves where there are few tiles of theirs: one's waves wait for each other while the queries are
-// laid out, and four have less to wait for.  us with the wide ones / with four waves (int8 rows of 768, one query each):
+// Workgroups of four waves where there are few tiles of theirs, every partition counted as long as the page table and the scores' rows
+// allow (8 x 700 in a table for 70 000 takes the wide ones: 14.4 us): one's waves wait for each other while the queries are laid out,
+// and four have less to wait for.  us with the wide ones / with four waves (int8 rows of 768, one query each):
 //   fp32 queries: 8 x 700 (88 tiles) 14.4 / 8.3, 64 x 512 (512) 14.6 / 11.7, 64 x 1024 (1088) 15.4 / 19.3
 //   fp16 queries: 8 x 700 8.5 / 7.3, 64 x 512 11.3 / 9.9, 64 x 1024 12.4 / 13.4
 // rows of 64 bytes, whose tile is four times as long (INT4 of 100 wide): 300 x 1000 (1200) 20.4 / 17.4, 300 x 4000 36 / 38

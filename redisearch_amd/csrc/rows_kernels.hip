@@ -368,7 +368,8 @@ constexpr uint32_t COLUMNS = 4096;   // columns of a workgroup, whose counts of 
 
 // A workgroup finds in the lists what falls among its columns (sums and maxima of integers: the same in any order), then goes over
 // them once: eight bytes a cell, whatever the rules are.  256 x 200 003 with all of them: 62 - 67 us, 6.1 - 6.6 TB/s (a copy of
-// as much memory: 5.2).  4096 columns: their counts are 32 KiB of LDS, five workgroups a CU.
+// as much memory: 5.2).  4096 columns: their counts are 32 KiB of LDS, five workgroups a CU.  Each of a query's workgroups reads its
+// lists whole: 16 queries x 1 000 000 columns take 23 us without a list, 28 with 1000 entries each, 69 with 10 000, 461 with 100 000.
 __global__ __launch_bounds__(256) void adjust_scores_kernel(AdjustArgs a, uint32_t tiles, uint64_t work) {
   constexpr int PER = COLUMNS / 1024;
   __shared__ alignas(16) uint32_t times[COLUMNS];   // how often a column was shown
