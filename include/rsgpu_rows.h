@@ -5,8 +5,8 @@
  * All arrays below are DEVICE memory and belong to the caller; every call but the two RSGPU_FlatIndex_ ones at the end only launches
  * kernels on `stream` (a hipStream_t; NULL: the device's default stream) and returns: none of them allocates, copies or waits, so they
  * may be captured into a hipGraph.  Two calls that write the same memory are ordered by the caller (one stream, or events).  0 on
- * success, -1 with RSGPU_LastError() otherwise; a refused call has launched nothing.  An index found on the device (a slot, a page, an offset, a
- * list's entry) that is out of its range never leads to an access out of range: what it means is said at each call.
+ * success, -1 with RSGPU_LastError() otherwise; a refused call has launched nothing.  An index found on the device (a slot, a page,
+ * an offset, a list's entry) that is out of its range never leads to an access out of range: what it means is said at each call.
  */
 #ifndef RSGPU_ROWS_H
 #define RSGPU_ROWS_H
@@ -60,12 +60,12 @@ int RSGPU_RowCache_Read(const RSGPU_RowCache *cache, const int64_t *slots, size_
  * j % page_rows  of the cache, and the queries query_offsets[g] .. query_offsets[g + 1] - 1 (n_partitions + 1 offsets that do
  * not fall; queries before the first and behind the last belong to nobody).  For each such query m and each j:
  *   scores[m * ld + j] = p  (PRODUCT)  or  1 - p  (DISTANCE: VecSim's inner-product / cosine distance),
- *   p = sum over the elements of query * row, accumulated in fp32; of rows kept in codes no sum on the way leaves fp32's range where p
- *   does not.  Bits of an element below 2^-107 and of p below 2^-119 are not kept.
+ *   p = sum over the elements of query * row, accumulated in fp32 (of rows kept in codes nothing on the way leaves fp32's range
+ *   unless such a sum does; bits of an element below 2^-107 and of p below 2^-119 are not kept)
  * A page that is negative or not in the cache: its rows score -inf (PRODUCT) / +inf (DISTANCE), behind every other.  All other
  * cells of `scores` are left as they were.  Right for any groups, fast for even ones: the host chooses the kernel by the queries of a
- * listed partition on average and by max_pages and ld, so list the partitions that are asked.  A row count counts as no more than max_pages * page_rows and ld; a range of queries
- * that falls or leaves [0, n_queries] is cut to it. */
+ * listed partition on average and by max_pages and ld, so list the partitions that are asked.  A row count counts as no more than
+ * max_pages * page_rows and ld; a range of queries that falls or leaves [0, n_queries] is cut to it. */
 typedef enum { RSGPU_SCORES_PRODUCT = 0, RSGPU_SCORES_DISTANCE = 1 } RSGPU_ScoreForm;
 
 int RSGPU_RowCache_PartitionScores(const RSGPU_RowCache *cache, const void *queries, size_t stride, size_t n_queries,
@@ -78,8 +78,8 @@ int RSGPU_RowCache_PartitionScores(const RSGPU_RowCache *cache, const void *quer
  *           p = p > 0 ? p / repetition[m] : p * repetition[m], then p -= n * frequency[m] + presence[m]
  *   boost   the column is in the query's list bias_ids[..]: p += bias_values[..] (of an id that comes again, the last value)
  *   filter  bit (column % 32) of word column / 32 of the query's mask row is 0: -inf (+inf for a DISTANCE)
- * A cell that no rule touches keeps its bits.  A query's lists are read once for every 4096 columns.  Entries of a list out of [0, n_columns) are passed over; a list's range is cut to
- * [0, n_seen] / [0, n_bias]. */
+ * A cell that no rule touches keeps its bits.  Entries of a list out of [0, n_columns) are passed over; a list's range is cut to
+ * [0, n_seen] / [0, n_bias].  (Lists are read once for every 4096 columns: they are meant to be short next to a row of scores.) */
 typedef struct RSGPU_ScoreRules {
   int device;                   /* HIP device of the arrays; -1: the one that holds the scores */
   int form;                     /* RSGPU_ScoreForm */

@@ -73,9 +73,9 @@ __device__ __forceinline__ void planes8(const float (&v)[8], u4 (&p)[3]) {
 
 // bf16 and fp32 queries reach 2^128, and codes are summed before they meet their scale: 65 536 elements times codes of up to 448 would
 // leave fp32 where the score, of rows of thousandths, does not.  So one side goes in by SHRUNK, exactly, and the score is multiplied by
-// what that was when its scales are in it: no sum overflows that is not an infinity in the end.  (fp16 queries times codes stay below
+// what that was when its scales are in it: no sum overflows unless the score's own sums do.  (fp16 queries times codes stay below
 // 2^41.)  It costs what of a query's elements lies below 2^-107, or of a score below 2^-119.  Which side: codes where their conversion
-// does it for nothing (E4M3) or where rows are converted no more often than queries (many queries: 1 - 3 % of the time), else queries,
+// does it for nothing (E4M3) or where rows are converted no more often than queries (many queries: 1 - 4 % of the time), else queries,
 // once a partition (8 x 700 INT8 rows of 768, fp32 queries: queries 8.3 us as without, codes 8.8).
 constexpr float SHRUNK = 0x1p-26f;
 enum { BY_NOTHING = 0, BY_CODES = 1, BY_QUERIES = 2 };
